@@ -245,7 +245,7 @@ def prepare(case, seed):
     if case["op"] == "read":
         lens = _base(case)
         s.update(_filled(g, case, lens))
-        s["cu_rows"], s["max_rows"] = _cu(lens), max(lens)
+        s["cu_rows"] = _cu(lens)
         for n in ("k", "v"):
             s[n + "_out"] = torch.empty(sum(lens), case["kv_heads"] * hd, device=DEV)
         return s
@@ -377,9 +377,9 @@ def _plan(s):
         return (ops.make_paged_append(cache, s["cu_new"], s["base_len"], s["k"], s["v"], q=s["q"], q_out=s["q_out"],
                                       num_heads=c["heads"], q_gain=s["q_gain"], k_gain=s["k_gain"], eps=EPS,
                                       rope_cos=s["cos"], rope_sin=s["sin"]),
-                ops.make_paged_read(cache, s["cu_new"], s["k_back"], s["v_back"], start=s["base_len"], max_rows=s["max_new"]))
+                ops.make_paged_read(cache, s["cu_new"], s["k_back"], s["v_back"], start=s["base_len"]))
     if c["op"] == "read":
-        return ops.make_paged_read(cache, s["cu_rows"], s["k_out"], s["v_out"], max_rows=s["max_rows"])
+        return ops.make_paged_read(cache, s["cu_rows"], s["k_out"], s["v_out"])
     d = ops.make_paged_attn(cache, s["cu_new"], s["base_len"], s["q"], s["out"], c["heads"], s["max_new"], s["max_len"],
                             1 / math.sqrt(c["hd"]), block_mode=c["block"], window=c["window"])
     return d, ops.paged_attn_workspace(d)
