@@ -8,6 +8,12 @@
 #include "common.cuh"
 
 #include <math.h>
+#include <string.h>
+
+namespace fblt {
+int paged_append_check(const fblt_paged_append_desc *d); // paged_cache.cu
+int paged_attn_check(const fblt_paged_attn_desc *d);     // paged_attn.cu
+} // namespace fblt
 
 namespace fblt {
 int matmul_qkv_rotated(const float *a, int64_t lda, const void *packed_qkv, int64_t rows, int64_t E, int32_t head_dim,
@@ -199,5 +205,75 @@ extern "C" int fblt_kv_self_attention_step(const fblt_kv_step_desc *d, void *str
     if (st != FBLT_OK) return st;
 
     return fblt_matmul(d->combined_work, E, d->packed_proj, nullptr, d->output, d->output_stride, rows, E, E, d->precision,
+                       stream);
+}
+
+// The same step over the 8-bit paged cache: projection, norm + rotation + quantised write-through (which leaves the
+// rotated query rows in place), attention over the pages, projection. Four launches, five where the keys are split.
+extern "C" int fblt_paged_self_attention_step(const fblt_paged_step_desc *d, void *stream) {
+    fblt::NvtxRange nvtx_range("fblt_paged_self_attention_step");
+    using namespace fblt;
+    if (!d) return fail(FBLT_ERR_ARG, "paged step: NULL descriptor");
+    if (d->batch < 0 || d->num_heads <= 0 || d->total_rows < 0 || d->cache.num_kv_heads <= 0 || d->cache.head_dim <= 0)
+        return fail(FBLT_ERR_ARG, "paged step: bad sizes");
+    const int64_t hd = d->cache.head_dim, E = (int64_t)d->num_heads * hd, W = E + 2 * d->cache.num_kv_heads * hd;
+
+    fblt_paged_append_desc w;
+    memset(&w, 0, sizeof(w));
+    w.cache = d->cache;
+    w.batch = d->batch;
+    w.num_heads = d->num_heads;
+    w.total_rows = d->total_rows;
+    w.rope_len = d->rope_len;
+    w.cu_new = d->cu_new;
+    w.base_len = d->base_len;
+    w.q = w.q_out = d->qkv_work;
+    w.k = d->qkv_work + E;
+    w.v = d->qkv_work + E + d->cache.num_kv_heads * hd;
+    w.q_stride = w.q_out_stride = w.k_stride = w.v_stride = W;
+    w.q_out = d->qkv_work;
+    w.q_gain = d->q_gain;
+    w.k_gain = d->k_gain;
+    w.eps = d->eps;
+    w.rope_cos = d->rope_cos;
+    w.rope_sin = d->rope_sin;
+
+    fblt_paged_attn_desc a;
+    memset(&a, 0, sizeof(a));
+    a.cache = d->cache;
+    a.batch = d->batch;
+    a.num_heads = d->num_heads;
+    a.total_rows = d->total_rows;
+    a.max_new = d->max_new;
+    a.max_len = d->max_len;
+    a.block_mode = d->block_mode;
+    a.window = d->window;
+    a.cu_new = d->cu_new;
+    a.base_len = d->base_len;
+    a.q = d->qkv_work;
+    a.q_stride = W;
+    a.out = d->combined_work;
+    a.out_stride = E;
+    a.scale = 1.0f / sqrtf((float)hd);
+
+    // every refusal comes before the first launch: a step that fails has not touched the cache
+    int st = paged_append_check(&w);
+    if (st != FBLT_OK) return st;
+    st = paged_attn_check(&a);
+    if (st != FBLT_OK) return st;
+    if (d->batch == 0 || d->total_rows == 0) return FBLT_OK;
+    if (!d->input || !d->output || !d->packed_qkv || !d->packed_proj || !d->qkv_work || !d->combined_work)
+        return fail(FBLT_ERR_ARG, "paged step: buffers must not be NULL");
+    if (d->input_stride < E || d->output_stride < E) return fail(FBLT_ERR_ARG, "paged step: row strides below embed_dim");
+    if (d->max_new < 1) return fail(FBLT_ERR_ARG, "paged step: max_new must bound the new rows");
+    if (fblt_paged_attn_workspace(&a) > d->workspace_bytes || !d->workspace) a.splits = 1;
+
+    st = fblt_matmul(d->input, d->input_stride, d->packed_qkv, nullptr, d->qkv_work, W, d->total_rows, E, W, d->precision, stream);
+    if (st != FBLT_OK) return st;
+    st = fblt_paged_append(&w, stream);
+    if (st != FBLT_OK) return st;
+    st = fblt_paged_attn(&a, d->workspace, d->workspace_bytes, stream);
+    if (st != FBLT_OK) return st;
+    return fblt_matmul(d->combined_work, E, d->packed_proj, nullptr, d->output, d->output_stride, d->total_rows, E, E, d->precision,
                        stream);
 }

@@ -1,0 +1,147 @@
+// The 8-bit paged KV cache as the kernels see it: page lookup with bounds, the code <-> value
+// conversions and the checks every host entry point makes of the cache description.
+#pragma once
+
+#include "common.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <limits.h>
+#include <string.h>
+
+namespace fblt {
+
+struct PagedView {
+    uint8_t *kc, *vc;
+    int8_t *ke, *ve;
+    const int32_t *table;
+    int64_t table_stride;
+    int num_pages, max_pages, page_size, kvh;
+    int32_t *status;
+
+    __device__ __forceinline__ void raise(int bit) const {
+        if (status) atomicOr(status, bit);
+    }
+    // Page that holds entry `pi` of sequence b's table, -1 if there is none.
+    __device__ __forceinline__ int page(int b, int pi) const {
+        if (pi >= max_pages) return -1;
+        const int id = __ldg(table + (int64_t)b * table_stride + pi);
+        return (unsigned)id < (unsigned)num_pages ? id : -1;
+    }
+    // Row index of (page, kv head, slot): element offset of its exponent; times head_dim that of its codes.
+    __device__ __forceinline__ int64_t row(int page, int head, int slot) const {
+        return ((int64_t)page * kvh + head) * page_size + slot;
+    }
+};
+
+inline PagedView paged_view(const fblt_paged_cache &c) {
+    PagedView v;
+    v.kc = c.k_codes;
+    v.vc = c.v_codes;
+    v.ke = c.k_exp;
+    v.ve = c.v_exp;
+    v.table = c.page_table;
+    v.table_stride = c.page_table_stride;
+    v.num_pages = c.num_pages;
+    v.max_pages = c.max_pages;
+    v.page_size = c.page_size;
+    v.kvh = c.num_kv_heads;
+    v.status = c.status;
+    return v;
+}
+
+int validate_paged_cache(const fblt_paged_cache &c, int batch, const char *who); // paged_cache.cu
+
+// New rows of sequence b: packed rows [r0, r0 + n), first position base. False (and the status bit) where the tables
+// do not describe a sequence.
+__device__ __forceinline__ bool paged_seq(const PagedView &pv, const int32_t *cu, const int32_t *base_len, int total, int b,
+                                          int &r0, int &n, int &base) {
+    r0 = cu[b];
+    const int r1 = cu[b + 1];
+    base = base_len ? base_len[b] : 0;
+    n = r1 - r0;
+    if (r0 < 0 || r1 < r0 || r1 > total || base < 0 || base > INT_MAX - n) {
+        pv.raise(FBLT_PAGED_BAD_LENGTH);
+        n = 0;
+        return false;
+    }
+    return true;
+}
+
+// 2^e as a float, -126 <= e <= 127.
+__device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }
+
+template <int FMT>
+struct KvFormat;
+
+// e4m3: sign, 4 exponent bits (bias 7), 3 mantissa bits.
+template <>
+struct KvFormat<FBLT_KV_E4M3> {
+    static constexpr int kEmin = -117, kEmax = 119, kQmax = 448;
+    // The byte's fields moved into a half's (bias 15) give code * 2^-8, subnormal codes included: half subnormals
+    // are fixed point like e4m3's. value = half * 2^(e + kShift).
+    static constexpr int kShift = 8;
+    // least e with a <= 448 * 2^e, from the bits of a = 1.m * 2^x: x - 8, one more where the significand passes 1.75
+    static __device__ __forceinline__ int exponent(float a) {
+        const int b = __float_as_int(a);
+        const int e = (b >> 23) - 127 - 8 + ((b & 0x7fffff) > 0x600000 ? 1 : 0);
+        return min(max(e, kEmin), kEmax);
+    }
+    // two bytes at the upper halves of their 16-bit lanes -> two halves
+    static __device__ __forceinline__ uint32_t widen(uint32_t x) {
+        return (x & 0x80008000u) | ((x >> 1) & 0x7fff7fffu & 0x3f803f80u);
+    }
+    // four codes (one word) -> halves of codes 0, 1 and of codes 2, 3
+    static __device__ __forceinline__ void halves(uint32_t w, uint32_t &h01, uint32_t &h23) {
+        h01 = widen(__byte_perm(w, 0, 0x1404));
+        h23 = widen(__byte_perm(w, 0, 0x3424));
+    }
+    // four scaled finite values -> one word of codes
+    static __device__ __forceinline__ uint32_t codes(float a, float b, float c, float d) {
+        uint16_t lo, hi;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+        return (uint32_t)lo | ((uint32_t)hi << 16);
+    }
+};
+
+template <>
+struct KvFormat<FBLT_KV_INT8> {
+    static constexpr int kEmin = -126, kEmax = 121, kQmax = 127;
+    static constexpr int kShift = 0;
+    // least e with a <= 127 * 2^e: x - 6, one more where the significand passes 127 / 64
+    static __device__ __forceinline__ int exponent(float a) {
+        const int b = __float_as_int(a);
+        const int e = (b >> 23) - 127 - 6 + ((b & 0x7fffff) > 0x7e0000 ? 1 : 0);
+        return min(max(e, kEmin), kEmax);
+    }
+    // byte ^ 0x80 below the exponent of 1024 is the half 1024 + 128 + code: exact, and so is the difference
+    static __device__ __forceinline__ void halves(uint32_t w, uint32_t &h01, uint32_t &h23) {
+        w ^= 0x80808080u;
+        const __half2 off = __float2half2_rn(1152.0f);
+        uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), off), y = __hsub2(*reinterpret_cast<__half2 *>(&b), off);
+        h01 = *reinterpret_cast<const uint32_t *>(&x);
+        h23 = *reinterpret_cast<const uint32_t *>(&y);
+    }
+    static __device__ __forceinline__ uint32_t codes(float a, float b, float c, float d) {
+        const uint32_t i = (uint32_t)__float2int_rn(a) & 0xff, j = (uint32_t)__float2int_rn(b) & 0xff;
+        const uint32_t k = (uint32_t)__float2int_rn(c) & 0xff, l = (uint32_t)__float2int_rn(d) & 0xff;
+        return i | (j << 8) | (k << 16) | (l << 24);
+    }
+};
+
+// Four codes of one word -> their values, `s` = 2^(e + kShift).
+template <int FMT>
+__device__ __forceinline__ float4 kv_values(uint32_t w, float s) {
+    uint32_t a, b;
+    KvFormat<FMT>::halves(w, a, b);
+    const float2 x = __half22float2(*reinterpret_cast<__half2 *>(&a)), y = __half22float2(*reinterpret_cast<__half2 *>(&b));
+    return make_float4(x.x * s, x.y * s, y.x * s, y.y * s);
+}
+template <int FMT>
+__device__ __forceinline__ float kv_scale(int e) { // exponents outside the format's range are not written by the library
+    return exp2_int(min(max(e, KvFormat<FMT>::kEmin), KvFormat<FMT>::kEmax) + KvFormat<FMT>::kShift);
+}
+
+} // namespace fblt

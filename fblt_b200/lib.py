@@ -20,6 +20,9 @@ BACKEND_CPU, BACKEND_CUDA = 0, 1
 GROUP_NONE, GROUP_PATCH_ENC, GROUP_PATCH_DEC, GROUP_PATCH_LEQ, GROUP_IDS = range(5)
 IMPL_AUTO, IMPL_ROW, IMPL_TILE, IMPL_TCGEN05, IMPL_ROW_QUAD, IMPL_UNIT = range(6)
 PREC_FP32, PREC_TF32 = 0, 1
+KV_E4M3, KV_INT8 = 0, 1
+PAGED_BAD_PAGE, PAGED_NONFINITE, PAGED_BAD_POSITION, PAGED_BAD_LENGTH = 1, 2, 4, 8
+PAGED_OUT_FP32, PAGED_OUT_BF16 = 0, 1
 
 
 class HeadArgs(C.Structure):
@@ -145,6 +148,69 @@ class DecodeDesc(C.Structure):
     ]
 
 
+class PagedCache(C.Structure):
+    """fblt_paged_cache: the 8-bit pages and their table."""
+    _fields_ = [
+        ("format", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32),
+        ("num_pages", C.c_int32), ("max_pages", C.c_int32),
+        ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p),
+        ("page_table", C.c_void_p), ("page_table_stride", C.c_int64), ("status", C.c_void_p),
+    ]
+
+
+class QkNormRopeDesc(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("num_heads", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("rope_len", C.c_int32),
+        ("q", C.c_void_p), ("q_stride", C.c_int64), ("k", C.c_void_p), ("k_stride", C.c_int64),
+        ("q_out", C.c_void_p), ("q_out_stride", C.c_int64), ("k_out", C.c_void_p), ("k_out_stride", C.c_int64),
+        ("q_gain", C.c_void_p), ("k_gain", C.c_void_p), ("eps", C.c_float), ("reserved", C.c_int32),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("pos", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+class PagedAppendDesc(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("batch", C.c_int32), ("num_heads", C.c_int32), ("total_rows", C.c_int32),
+        ("rope_len", C.c_int32), ("cu_new", C.c_void_p), ("base_len", C.c_void_p),
+        ("k", C.c_void_p), ("k_stride", C.c_int64), ("v", C.c_void_p), ("v_stride", C.c_int64),
+        ("q", C.c_void_p), ("q_stride", C.c_int64), ("q_out", C.c_void_p), ("q_out_stride", C.c_int64),
+        ("q_gain", C.c_void_p), ("k_gain", C.c_void_p), ("eps", C.c_float), ("reserved", C.c_int32),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
+    ]
+
+
+class PagedReadDesc(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("batch", C.c_int32), ("total_rows", C.c_int32), ("out_type", C.c_int32),
+        ("reserved", C.c_int32), ("cu_rows", C.c_void_p), ("start", C.c_void_p),
+        ("k_out", C.c_void_p), ("k_out_stride", C.c_int64), ("v_out", C.c_void_p), ("v_out_stride", C.c_int64),
+    ]
+
+
+class PagedAttnDesc(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("batch", C.c_int32), ("num_heads", C.c_int32), ("total_rows", C.c_int32),
+        ("max_new", C.c_int32), ("max_len", C.c_int32), ("block_mode", C.c_int32), ("window", C.c_int32),
+        ("splits", C.c_int32), ("cu_new", C.c_void_p), ("base_len", C.c_void_p),
+        ("q", C.c_void_p), ("q_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64),
+        ("scale", C.c_float), ("reserved", C.c_int32),
+    ]
+
+
+class PagedStepDesc(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("batch", C.c_int32), ("num_heads", C.c_int32), ("total_rows", C.c_int32),
+        ("max_new", C.c_int32), ("max_len", C.c_int32), ("block_mode", C.c_int32), ("window", C.c_int32),
+        ("precision", C.c_int32), ("cu_new", C.c_void_p), ("base_len", C.c_void_p),
+        ("input", C.c_void_p), ("input_stride", C.c_int64), ("packed_qkv", C.c_void_p), ("packed_proj", C.c_void_p),
+        ("output", C.c_void_p), ("output_stride", C.c_int64), ("qkv_work", C.c_void_p), ("combined_work", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("q_gain", C.c_void_p), ("k_gain", C.c_void_p), ("eps", C.c_float), ("rope_len", C.c_int32),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes): every symbol include/fblt_attn.h declares
 SYMBOLS = {
     "fblt_last_error": (C.c_char_p, []),
@@ -199,6 +265,12 @@ SYMBOLS = {
     "fblt_mha_forward": (C.c_int, [C.POINTER(MhaDesc), C.c_void_p]),
     "fblt_cross_attention_forward": (C.c_int, [C.POINTER(CrossDesc), C.c_void_p]),
     "fblt_kv_self_attention_step": (C.c_int, [C.POINTER(KvStepDesc), C.c_void_p]),
+    "fblt_qk_norm_rope": (C.c_int, [C.POINTER(QkNormRopeDesc), C.c_void_p]),
+    "fblt_paged_append": (C.c_int, [C.POINTER(PagedAppendDesc), C.c_void_p]),
+    "fblt_paged_read": (C.c_int, [C.POINTER(PagedReadDesc), C.c_void_p]),
+    "fblt_paged_attn_workspace": (C.c_size_t, [C.POINTER(PagedAttnDesc)]),
+    "fblt_paged_attn": (C.c_int, [C.POINTER(PagedAttnDesc), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fblt_paged_self_attention_step": (C.c_int, [C.POINTER(PagedStepDesc), C.c_void_p]),
     "fblt_session_create": (C.c_int, [C.POINTER(C.c_void_p), C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_int64,
                                       C.c_int32, C.c_int32]),
     "fblt_session_destroy": (None, [C.c_void_p]),
@@ -245,7 +317,9 @@ def load() -> C.CDLL:
         fn.argtypes = args
     sizes = (C.c_size_t * 16)()
     n = lib.fblt_abi_sizes(sizes, 16)
-    want = [C.sizeof(HeadArgs), C.sizeof(PatchInfo), C.sizeof(MaskDesc), C.sizeof(AttnDesc), C.sizeof(DecodeDesc), C.sizeof(MhaDesc), C.sizeof(CrossDesc), C.sizeof(KvStepDesc)]
+    want = [C.sizeof(HeadArgs), C.sizeof(PatchInfo), C.sizeof(MaskDesc), C.sizeof(AttnDesc), C.sizeof(DecodeDesc), C.sizeof(MhaDesc), C.sizeof(CrossDesc), C.sizeof(KvStepDesc),
+            C.sizeof(PagedCache), C.sizeof(QkNormRopeDesc), C.sizeof(PagedAppendDesc), C.sizeof(PagedReadDesc),
+            C.sizeof(PagedAttnDesc), C.sizeof(PagedStepDesc)]
     if list(sizes[:n]) != want:
         raise ImportError(f"ABI mismatch between lib.py and libfblt_attn.so: {list(sizes[:n])} vs {want}")
     _lib = lib

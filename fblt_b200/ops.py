@@ -533,6 +533,241 @@ def dv_commit(logits: torch.Tensor, width: int, x: torch.Tensor, l: torch.Tensor
     return accepted
 
 
+# --------------------------------------------------------------------------- paged 8-bit KV cache
+
+_KV_FORMATS = {"e4m3": L.KV_E4M3, "int8": L.KV_INT8}
+
+
+def _rows(t: torch.Tensor, cols: int, what: str, dtypes=(torch.float32,)) -> torch.Tensor:
+    """Checks a 2-D row view that is handed to the library by pointer and row stride."""
+    if not (t.is_cuda and t.dim() == 2 and t.dtype in dtypes and t.shape[1] == cols and (t.stride(1) == 1 or cols == 1)):
+        raise ValueError(f"{what}: a CUDA [rows, {cols}] view of {'/'.join(str(d) for d in dtypes)} with unit column stride is needed")
+    return t
+
+
+def _table(t: torch.Tensor, n: int, what: str) -> torch.Tensor:
+    if not (t.is_cuda and t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] >= n and (t.stride(0) == 1 or n <= 1)):
+        raise ValueError(f"{what}: a contiguous CUDA int32 tensor of {n} entries is needed")
+    return t
+
+
+def _vector(t: Optional[torch.Tensor], n: int, what: str) -> Optional[int]:
+    if t is None:
+        return None
+    if not (t.is_cuda and t.dtype == torch.float32 and t.shape == (n,) and t.is_contiguous()):
+        raise ValueError(f"{what}: a contiguous CUDA float32 tensor of {n} values is needed")
+    return t.data_ptr()
+
+
+def _rope(d, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], head_dim: int) -> None:
+    if (cos is None) != (sin is None):
+        raise ValueError("rope_cos and rope_sin go together")
+    if cos is None:
+        return
+    for t in (cos, sin):
+        if not (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.dim() == 2
+                and t.shape[1] == head_dim // 2 and t.shape[0] == cos.shape[0]):
+            raise ValueError(f"rotary tables: contiguous CUDA float32 [positions, {head_dim // 2}] tensors are needed")
+    d.rope_cos, d.rope_sin, d.rope_len = cos.data_ptr(), sin.data_ptr(), int(cos.shape[0])
+
+
+class PagedKvCache:
+    """K and V in 8 bits with one power-of-two exponent for every (position, kv head), in pages.
+
+    k_codes / v_codes: uint8 [num_pages, num_kv_heads, page_size, head_dim]; k_exp / v_exp: int8 [num_pages,
+    num_kv_heads, page_size]; page_table: int32 [batch, max_pages], page of positions j * page_size ... of a sequence.
+    fmt: "e4m3" or "int8". `status` collects the FBLT_PAGED_* bits that kernels raise (status_bits() reads them)."""
+
+    def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor,
+                 page_table: torch.Tensor, fmt: str):
+        if fmt not in _KV_FORMATS:
+            raise ValueError(f"fmt {fmt!r} (e4m3 or int8)")
+        shape = k_codes.shape
+        if k_codes.dim() != 4 or v_codes.shape != shape or k_exp.shape != shape[:3] or v_exp.shape != shape[:3]:
+            raise ValueError("codes are [pages, kv_heads, page_size, head_dim], exponents [pages, kv_heads, page_size]")
+        for t, dt in ((k_codes, torch.uint8), (v_codes, torch.uint8), (k_exp, torch.int8), (v_exp, torch.int8)):
+            if not (t.is_cuda and t.dtype == dt and t.is_contiguous()):
+                raise ValueError("codes are contiguous CUDA uint8 tensors, exponents int8")
+        if not (page_table.is_cuda and page_table.dtype == torch.int32 and page_table.dim() == 2
+                and (page_table.stride(1) == 1 or page_table.shape[1] == 1)):
+            raise ValueError("page_table: a CUDA int32 [batch, max_pages] tensor with unit column stride is needed")
+        self.k_codes, self.v_codes, self.k_exp, self.v_exp, self.page_table, self.fmt = k_codes, v_codes, k_exp, v_exp, page_table, fmt
+        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = (int(n) for n in shape)
+        self.batch = int(page_table.shape[0])
+        self.status = torch.zeros(1, dtype=torch.int32, device=k_codes.device)
+        c = self.desc = L.PagedCache()
+        c.format, c.num_kv_heads, c.head_dim, c.page_size = _KV_FORMATS[fmt], self.num_kv_heads, self.head_dim, self.page_size
+        c.num_pages, c.max_pages = self.num_pages, int(page_table.shape[1])
+        c.k_codes, c.v_codes, c.k_exp, c.v_exp = k_codes.data_ptr(), v_codes.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr()
+        c.page_table, c.page_table_stride = page_table.data_ptr(), max(page_table.stride(0), int(page_table.shape[1]))
+        c.status = self.status.data_ptr()
+
+    @classmethod
+    def empty(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, page_table: torch.Tensor, fmt: str) -> "PagedKvCache":
+        """A pool of zeroed pages on the page table's device."""
+        dev = page_table.device
+        codes = [torch.zeros(num_pages, num_kv_heads, page_size, head_dim, dtype=torch.uint8, device=dev) for _ in range(2)]
+        exps = [torch.zeros(num_pages, num_kv_heads, page_size, dtype=torch.int8, device=dev) for _ in range(2)]
+        return cls(*codes, *exps, page_table, fmt)
+
+    def status_bits(self) -> int:
+        """The status word (waits for the device); it is cleared."""
+        bits = int(self.status.item())
+        self.status.zero_()
+        return bits
+
+
+def make_qk_norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], pos: Optional[torch.Tensor], num_heads: int,
+                      num_kv_heads: int, head_dim: int, *, q_out: Optional[torch.Tensor] = None,
+                      k_out: Optional[torch.Tensor] = None, q_gain: Optional[torch.Tensor] = None,
+                      k_gain: Optional[torch.Tensor] = None, eps: float = 1e-6, rope_cos: Optional[torch.Tensor] = None,
+                      rope_sin: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> L.QkNormRopeDesc:
+    """q [rows, num_heads * head_dim] and k [rows, num_kv_heads * head_dim] (views of a packed projection will do);
+    without q_out / k_out the rows are changed in place. pos: int32 [rows]."""
+    d = L.QkNormRopeDesc()
+    rows = int((q if q is not None else k).shape[0])
+    d.rows, d.num_heads, d.num_kv_heads, d.head_dim, d.eps = rows, num_heads, num_kv_heads, head_dim, float(eps)
+    for name, x, out, heads in (("q", q, q_out, num_heads), ("k", k, k_out, num_kv_heads)):
+        if x is None:
+            continue
+        out = x if out is None else out
+        for t in (_rows(x, heads * head_dim, name), _rows(out, heads * head_dim, name + "_out")):
+            if t.shape[0] != rows:
+                raise ValueError("q, k and their outputs have one row count")
+        setattr(d, name, x.data_ptr())
+        setattr(d, name + "_stride", x.stride(0))
+        setattr(d, name + "_out", out.data_ptr())
+        setattr(d, name + "_out_stride", out.stride(0))
+    d.q_gain, d.k_gain = _vector(q_gain, head_dim, "q_gain"), _vector(k_gain, head_dim, "k_gain")
+    _rope(d, rope_cos, rope_sin, head_dim)
+    if pos is not None:
+        d.pos = _table(pos, rows, "pos").data_ptr()
+    if status is not None:
+        d.status = _table(status, 1, "status").data_ptr()
+    return d
+
+
+def qk_norm_rope(d: L.QkNormRopeDesc, stream=None) -> None:
+    L.check(L.load().fblt_qk_norm_rope(C.byref(d), _stream_ptr(stream)))
+
+
+def make_paged_append(cache: PagedKvCache, cu_new: torch.Tensor, base_len: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+                      q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None, num_heads: int = 0,
+                      q_gain: Optional[torch.Tensor] = None, k_gain: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                      rope_cos: Optional[torch.Tensor] = None, rope_sin: Optional[torch.Tensor] = None) -> L.PagedAppendDesc:
+    """k / v: [rows, kv_heads * head_dim], packed by sequence (cu_new int32 [batch + 1]) at positions base_len[b] + i.
+    With q ([rows, num_heads * head_dim]) the query rows are normalised and rotated too (into q_out, or in place)."""
+    d = L.PagedAppendDesc()
+    hd, kc, rows = cache.head_dim, cache.num_kv_heads * cache.head_dim, int(k.shape[0])
+    d.cache, d.batch, d.num_heads, d.total_rows, d.eps = cache.desc, cache.batch, num_heads, rows, float(eps)
+    d.cu_new, d.base_len = _table(cu_new, cache.batch + 1, "cu_new").data_ptr(), _table(base_len, cache.batch, "base_len").data_ptr()
+    d.k, d.k_stride = _rows(k, kc, "k").data_ptr(), k.stride(0)
+    d.v, d.v_stride = _rows(v, kc, "v").data_ptr(), v.stride(0)
+    out = q if q_out is None else q_out
+    if q is not None:
+        d.q, d.q_stride = _rows(q, num_heads * hd, "q").data_ptr(), q.stride(0)
+        d.q_out, d.q_out_stride = _rows(out, num_heads * hd, "q_out").data_ptr(), out.stride(0)
+    if any(t is not None and t.shape[0] != rows for t in (v, q, out)):
+        raise ValueError("q, q_out, k and v have one row count")
+    d.q_gain, d.k_gain = _vector(q_gain, hd, "q_gain"), _vector(k_gain, hd, "k_gain")
+    _rope(d, rope_cos, rope_sin, hd)
+    return d
+
+
+def paged_append(d: L.PagedAppendDesc, stream=None) -> None:
+    L.check(L.load().fblt_paged_append(C.byref(d), _stream_ptr(stream)))
+
+
+def make_paged_read(cache: PagedKvCache, cu_rows: torch.Tensor, k_out: Optional[torch.Tensor], v_out: Optional[torch.Tensor], *,
+                    start: Optional[torch.Tensor] = None) -> L.PagedReadDesc:
+    """Positions start[b] (0 without `start`) .. of every sequence into packed rows of float32 or bfloat16 (both exact)."""
+    d = L.PagedReadDesc()
+    first = k_out if k_out is not None else v_out
+    if first is None or (k_out is not None and v_out is not None and (k_out.dtype != v_out.dtype or k_out.shape != v_out.shape)):
+        raise ValueError("k_out / v_out: at least one, of one shape and type")
+    d.cache, d.batch, d.total_rows = cache.desc, cache.batch, int(first.shape[0])
+    d.out_type = L.PAGED_OUT_BF16 if first.dtype == torch.bfloat16 else L.PAGED_OUT_FP32
+    d.cu_rows = _table(cu_rows, cache.batch + 1, "cu_rows").data_ptr()
+    d.start = None if start is None else _table(start, cache.batch, "start").data_ptr()
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is not None:
+            setattr(d, name, _rows(t, cache.num_kv_heads * cache.head_dim, name, (torch.float32, torch.bfloat16)).data_ptr())
+            setattr(d, name + "_stride", t.stride(0))
+    return d
+
+
+def paged_read(d: L.PagedReadDesc, stream=None) -> None:
+    L.check(L.load().fblt_paged_read(C.byref(d), _stream_ptr(stream)))
+
+
+def make_paged_attn(cache: PagedKvCache, cu_new: torch.Tensor, base_len: torch.Tensor, q: torch.Tensor, out: torch.Tensor,
+                    num_heads: int, max_new: int, max_len: int, scale: float, *, block_mode: bool = False, window: int = 0,
+                    splits: int = 0) -> L.PagedAttnDesc:
+    """q / out: [rows, num_heads * head_dim], packed by sequence; row cu_new[b] + i is at position base_len[b] + i and
+    the cache holds the new rows already. max_new / max_len bound the new rows and base_len + new rows."""
+    d = L.PagedAttnDesc()
+    cols = num_heads * cache.head_dim
+    d.cache, d.batch, d.num_heads, d.total_rows = cache.desc, cache.batch, num_heads, int(q.shape[0])
+    d.max_new, d.max_len, d.block_mode, d.window, d.splits = max_new, max_len, int(block_mode), int(window), splits
+    d.cu_new, d.base_len = _table(cu_new, cache.batch + 1, "cu_new").data_ptr(), _table(base_len, cache.batch, "base_len").data_ptr()
+    d.q, d.q_stride = _rows(q, cols, "q").data_ptr(), q.stride(0)
+    d.out, d.out_stride = _rows(out, cols, "out").data_ptr(), out.stride(0)
+    if q.shape[0] != out.shape[0]:
+        raise ValueError("q and out have one row count")
+    d.scale = float(scale)
+    return d
+
+
+def paged_attn_workspace(d: L.PagedAttnDesc) -> Optional[torch.Tensor]:
+    n = L.load().fblt_paged_attn_workspace(C.byref(d))
+    return torch.empty(n, dtype=torch.uint8, device="cuda") if n else None
+
+
+def paged_attn(d: L.PagedAttnDesc, workspace: Optional[torch.Tensor] = None, stream=None) -> None:
+    wp = workspace.data_ptr() if workspace is not None else None
+    wn = workspace.numel() if workspace is not None else 0
+    L.check(L.load().fblt_paged_attn(C.byref(d), wp, wn, _stream_ptr(stream)))
+
+
+class PagedStepPlan:
+    """The self-attention block of a step over the paged cache with every buffer allocated up front (KvStepPlan's
+    counterpart): run() only enqueues launches, so steps can be captured in a CUDA graph and replayed while the caches
+    grow. x is the static input [total_rows, E], out the static output; rows are packed by cu_new (device), whose last
+    entry is total_rows; max_new / max_len bound the new rows and base_len + new rows over every replay.
+    w_qkv packs [E, (num_heads + 2 kv_heads) * head_dim] (q | k | v columns), w_proj [E, E]."""
+
+    def __init__(self, w_qkv: PackedWeights, w_proj: PackedWeights, cache: PagedKvCache, cu_new: torch.Tensor,
+                 base_len: torch.Tensor, num_heads: int, total_rows: int, max_new: int, max_len: int, *,
+                 q_gain: Optional[torch.Tensor] = None, k_gain: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 rope_cos: Optional[torch.Tensor] = None, rope_sin: Optional[torch.Tensor] = None,
+                 block_mode: bool = False, window: int = 0, precision: int = L.PREC_FP32):
+        hd, dev = cache.head_dim, cache.k_codes.device
+        E, W = num_heads * hd, (num_heads + 2 * cache.num_kv_heads) * hd
+        if (w_qkv.K, w_qkv.N) != (E, W) or (w_proj.K, w_proj.N) != (E, E):
+            raise ValueError(f"weights must be [{E}, {W}] and [{E}, {E}]")
+        new = lambda cols: torch.empty(total_rows, cols, dtype=torch.float32, device=dev)  # noqa: E731
+        self.x, self.out, self._qkv, self._comb = torch.zeros(total_rows, E, dtype=torch.float32, device=dev), new(E), new(W), new(E)
+        a = make_paged_attn(cache, cu_new, base_len, self._comb, self.out, num_heads, max_new, max_len, 1.0,
+                            block_mode=block_mode, window=window)
+        self._ws = paged_attn_workspace(a)
+        self._keep = [w_qkv, w_proj, cache, cu_new, base_len, q_gain, k_gain, rope_cos, rope_sin]
+        d = self.desc = L.PagedStepDesc()
+        d.cache, d.batch, d.num_heads, d.total_rows, d.max_new = cache.desc, cache.batch, num_heads, total_rows, max_new
+        d.max_len, d.block_mode, d.window, d.precision = max_len, int(block_mode), window, precision
+        d.cu_new, d.base_len = cu_new.data_ptr(), base_len.data_ptr()
+        d.input, d.input_stride = self.x.data_ptr(), self.x.stride(0)
+        d.packed_qkv, d.packed_proj = w_qkv.buf.data_ptr(), w_proj.buf.data_ptr()
+        d.output, d.output_stride = self.out.data_ptr(), self.out.stride(0)
+        d.qkv_work, d.combined_work = self._qkv.data_ptr(), self._comb.data_ptr()
+        if self._ws is not None:
+            d.workspace, d.workspace_bytes = self._ws.data_ptr(), self._ws.numel()
+        d.q_gain, d.k_gain, d.eps = _vector(q_gain, hd, "q_gain"), _vector(k_gain, hd, "k_gain"), float(eps)
+        _rope(d, rope_cos, rope_sin, hd)
+
+    def run(self, stream=None) -> None:
+        L.check(L.load().fblt_paged_self_attention_step(C.byref(self.desc), _stream_ptr(stream)))
+
+
 # --------------------------------------------------------------------------- host-buffer sessions
 
 class Session:

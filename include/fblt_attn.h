@@ -677,6 +677,223 @@ typedef struct {
 int fblt_kv_self_attention_step(const fblt_kv_step_desc *desc, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* paged KV cache in 8 bits                                                  */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * What an 8-bit cache row holds. For each (position, kv head) the head_dim values x of K (and of V) are stored as
+ * codes and ONE power-of-two exponent e: value = code * 2^e, with e the least integer for which
+ * max|x| <= Qmax * 2^e and code = x * 2^-e rounded to nearest even.
+ *   FBLT_KV_E4M3: float8 e4m3fn codes, Qmax = 448, -117 <= e <= 119
+ *   FBLT_KV_INT8: two's complement bytes, Qmax = 127, -126 <= e <= 121
+ * (e is clamped to those bounds; a code that would pass Qmax then is Qmax.) With a power of two as the scale the
+ * quotient x * 2^-e is exact, so a row has one quantised form whoever computes it, every stored value is a bf16
+ * number, and reading it back is exact. A NaN is stored as 0 and an infinity as +-Qmax * 2^e with e from the finite
+ * values; both raise FBLT_PAGED_NONFINITE. The library never writes the e4m3 codes 0x7f / 0xff (NaN); a cache that
+ * holds them is read as +-480 * 2^e.
+ */
+typedef enum { FBLT_KV_E4M3 = 0, FBLT_KV_INT8 = 1 } fblt_kv_format;
+
+/* Bits of fblt_paged_cache.status, OR'ed in by the kernels (never cleared by the library). */
+enum {
+    FBLT_PAGED_BAD_PAGE = 1,     /* a position lay beyond max_pages, or its page id outside [0, num_pages): append left
+                                  * the row out, read wrote zeros, attention did not see the key */
+    FBLT_PAGED_NONFINITE = 2,    /* append met an infinity or a NaN */
+    FBLT_PAGED_BAD_POSITION = 4, /* a position outside the rotary tables: the row was left unrotated */
+    FBLT_PAGED_BAD_LENGTH = 8    /* base_len[b] or start[b] negative, cu_* decreasing or outside [0, total], positions
+                                  * past 2^31 - 1, or more rows than max_new: those rows were not written (read and
+                                  * attention: not computed) */
+};
+
+/*
+ * The pages. Page p of kv head h holds page_size consecutive positions of one sequence:
+ *   codes [num_pages, num_kv_heads, page_size, head_dim] bytes, exponents [num_pages, num_kv_heads, page_size] int8.
+ * Position j of sequence b lives in page page_table[b * page_table_stride + j / page_size], slot j % page_size.
+ * A page may appear in the tables of several sequences (a shared prefix) as long as nobody appends to it; entries
+ * beyond a sequence's last page are not read. Page ids are checked by the kernels (see the status bits).
+ */
+typedef struct {
+    int32_t format; /* fblt_kv_format */
+    int32_t num_kv_heads;
+    int32_t head_dim;  /* 32, 64 or 128 */
+    int32_t page_size; /* a multiple of 16, 16 .. 1024 */
+    int32_t num_pages;
+    int32_t max_pages; /* entries of a page table row that may be read */
+    uint8_t *k_codes;  /* device, 16-byte aligned */
+    uint8_t *v_codes;
+    int8_t *k_exp; /* device, 16-byte aligned */
+    int8_t *v_exp;
+    const int32_t *page_table; /* device [batch, page_table_stride] */
+    int64_t page_table_stride;
+    int32_t *status; /* optional device word */
+} fblt_paged_cache;
+
+/*
+ * Per-head RMS norm of queries and keys with the rotary embedding in the same pass (no counterpart in the reference,
+ * whose heads are not normalised; it takes the place of the 2 x heads blt_rope_apply_packed launches of
+ * models/attention.c:73-89 for models that have both):
+ *   y_i = x_i * gain_i / sqrt(mean_j x_j^2 + eps), then every pair (y_2i, y_2i+1) rotated by the tables' row pos[r].
+ * q is [rows, num_heads * head_dim], k [rows, num_kv_heads * head_dim] with their own row strides (a packed
+ * projection is read in place); q_out / k_out may be the inputs themselves. q or k may be NULL (then so is its output).
+ * q_gain / k_gain [head_dim] NULL: that one is not normalised. rope tables NULL: not rotated; [rope_len, head_dim / 2]
+ * otherwise, pos device int32 [rows]; a row whose position lies outside [0, rope_len) is left unrotated and raises
+ * FBLT_PAGED_BAD_POSITION in *status (optional). All sums in fp32; mean_j x_j^2 must be finite. head_dim 32, 64
+ * or 128; strides multiples of 4, buffers 16-byte aligned, an output either equals its input (same stride) or does
+ * not overlap any input.
+ */
+typedef struct {
+    int64_t rows;
+    int32_t num_heads, num_kv_heads, head_dim;
+    int32_t rope_len;
+    const float *q;
+    int64_t q_stride;
+    const float *k;
+    int64_t k_stride;
+    float *q_out;
+    int64_t q_out_stride;
+    float *k_out;
+    int64_t k_out_stride;
+    const float *q_gain;
+    const float *k_gain;
+    float eps;
+    int32_t reserved;
+    const float *rope_cos;
+    const float *rope_sin;
+    const int32_t *pos;
+    int32_t *status;
+} fblt_qk_norm_rope_desc;
+
+int fblt_qk_norm_rope(const fblt_qk_norm_rope_desc *desc, void *stream);
+
+/*
+ * Writes the new rows of every sequence into its pages. Packed row cu_new[b] + i (i < cu_new[b+1] - cu_new[b], which
+ * may be 0) belongs to sequence b at position base_len[b] + i. K rows are normalised (k_gain) and rotated (rope
+ * tables) as in fblt_qk_norm_rope when those are given, then quantised; V rows are quantised as they are. With q the
+ * query rows are normalised and rotated in the same launch and written to q_out (which may be q). Slots of other
+ * positions are left as they are; base_len is not modified. All the rows of one call must have distinct slots.
+ * The write-through of infer/kv_cache.c:347-366 for this cache.
+ */
+typedef struct {
+    fblt_paged_cache cache;
+    int32_t batch;
+    int32_t num_heads; /* query heads (0 without q) */
+    int32_t total_rows; /* host copy of cu_new[batch] */
+    int32_t rope_len;
+    const int32_t *cu_new;   /* device [batch + 1] */
+    const int32_t *base_len; /* device [batch] */
+    const float *k;
+    int64_t k_stride;
+    const float *v;
+    int64_t v_stride;
+    const float *q; /* optional */
+    int64_t q_stride;
+    float *q_out;
+    int64_t q_out_stride;
+    const float *q_gain;
+    const float *k_gain;
+    float eps;
+    int32_t reserved;
+    const float *rope_cos;
+    const float *rope_sin;
+} fblt_paged_append_desc;
+
+int fblt_paged_append(const fblt_paged_append_desc *desc, void *stream);
+
+/*
+ * Reads positions start[b] .. start[b] + cu_rows[b+1] - cu_rows[b] of every sequence (start NULL: 0) back into packed
+ * rows [total_rows, num_kv_heads * head_dim] of fp32 or bf16; both are exact. k_out or v_out may be NULL.
+ */
+enum { FBLT_PAGED_OUT_FP32 = 0, FBLT_PAGED_OUT_BF16 = 1 };
+typedef struct {
+    fblt_paged_cache cache;
+    int32_t batch;
+    int32_t total_rows; /* host copy of cu_rows[batch] */
+    int32_t out_type;
+    int32_t reserved;
+    const int32_t *cu_rows; /* device [batch + 1] */
+    const int32_t *start;   /* device [batch] or NULL */
+    void *k_out;
+    int64_t k_out_stride; /* elements; multiples of 8 (bf16) or 4 (fp32) */
+    void *v_out;
+    int64_t v_out_stride;
+} fblt_paged_read_desc;
+
+int fblt_paged_read(const fblt_paged_read_desc *desc, void *stream);
+
+/*
+ * Attention of a chunk of new rows over the paged cache, which already holds them (fblt_paged_append before): one
+ * token per sequence, a drafted block, or thousands of prompt rows. Packed row cu_new[b] + i is the query at position
+ * p = base_len[b] + i; num_heads is a multiple of cache.num_kv_heads, query head h reads kv head
+ * h / (num_heads / num_kv_heads). Visible keys, as in fblt_decode_desc (infer/kv_cache.c:229-236):
+ *   block_mode == 0: j <= p && (window == 0 || p - j < window)
+ *   block_mode == 1: every key of the sequence, j < base_len[b] + new rows (window is ignored)
+ * Scores that are not finite weigh 0 and a row without any key gives zeros (ops/vecmath_cpu.c:16-53). Products carry
+ * at least 22 bits of q and of the probabilities and all of the cache's; sums are fp32. The result does not depend on
+ * how a prompt was cut into chunks beyond fp32 rounding.
+ * max_new and max_len are host-known bounds of the new rows and of base_len[b] + new rows. splits: pieces the key range
+ * of a (sequence, kv head) is cut into, merged by a second launch; 0 = choose. Workspace: fblt_paged_attn_workspace()
+ * bytes, 16-byte aligned, not shared by calls that may overlap. The call only enqueues launches.
+ */
+typedef struct {
+    fblt_paged_cache cache;
+    int32_t batch;
+    int32_t num_heads;
+    int32_t total_rows; /* host copy of cu_new[batch] */
+    int32_t max_new;
+    int32_t max_len;
+    int32_t block_mode;
+    int32_t window;
+    int32_t splits;
+    const int32_t *cu_new;   /* device [batch + 1] */
+    const int32_t *base_len; /* device [batch] */
+    const float *q;          /* device [total_rows, num_heads * head_dim] */
+    int64_t q_stride;
+    float *out;
+    int64_t out_stride;
+    float scale;
+    int32_t reserved;
+} fblt_paged_attn_desc;
+
+size_t fblt_paged_attn_workspace(const fblt_paged_attn_desc *desc);
+int fblt_paged_attn(const fblt_paged_attn_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * The self-attention part of a step over the paged cache: fblt_kv_self_attention_step for this cache, with any number
+ * of new rows per sequence. qkv = input * weight_qkv ([E, (num_heads + 2 num_kv_heads) * head_dim], q | k | v columns,
+ * E = num_heads * head_dim, packed by fblt_matmul_pack_weights); q, k normalised (gains) and rotated (tables); K / V
+ * quantised into the pages; attention with scale 1 / sqrt(head_dim); output = combined * weight_proj ([E, E]). Does
+ * not advance base_len. Only enqueues launches, and lengths and pages are read on the device, so that a loop of
+ * steps can be captured in a CUDA graph and replayed while the caches grow (max_len then bounds every replay).
+ * The input, the projections and the scratch are as in fblt_kv_step_desc. Without enough workspace the key range
+ * is not split.
+ */
+typedef struct {
+    fblt_paged_cache cache;
+    int32_t batch, num_heads, total_rows, max_new;
+    int32_t max_len, block_mode, window, precision;
+    const int32_t *cu_new;
+    const int32_t *base_len;
+    const float *input; /* [total_rows, E] */
+    int64_t input_stride;
+    const void *packed_qkv;
+    const void *packed_proj;
+    float *output;
+    int64_t output_stride;
+    float *qkv_work;      /* [total_rows, (num_heads + 2 num_kv_heads) * head_dim] */
+    float *combined_work; /* [total_rows, E] */
+    void *workspace;
+    size_t workspace_bytes;
+    const float *q_gain;
+    const float *k_gain;
+    float eps;
+    int32_t rope_len;
+    const float *rope_cos;
+    const float *rope_sin;
+} fblt_paged_step_desc;
+
+int fblt_paged_self_attention_step(const fblt_paged_step_desc *desc, void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* host-buffer sessions (what a host-side caller with no device memory uses) */
 /* ------------------------------------------------------------------------ */
 
@@ -810,7 +1027,9 @@ void fblt_gather_destroy(fblt_gather *g);
  * process ends ("[fblt] N kernel launches"). */
 uint64_t fblt_launch_count(void);
 /* sizeof of {fblt_head_args, fblt_patch_info, fblt_mask_desc, fblt_attn_desc,
- * fblt_decode_desc, fblt_mha_desc, fblt_cross_desc, fblt_kv_step_desc}, for bindings that re-declare the structs. Returns the count. */
+ * fblt_decode_desc, fblt_mha_desc, fblt_cross_desc, fblt_kv_step_desc, fblt_paged_cache, fblt_qk_norm_rope_desc,
+ * fblt_paged_append_desc, fblt_paged_read_desc, fblt_paged_attn_desc, fblt_paged_step_desc}, for bindings that
+ * re-declare the structs. Returns the count. */
 size_t fblt_abi_sizes(size_t *out, size_t cap);
 
 #ifdef __cplusplus
