@@ -1,63 +1,468 @@
-// Attention of new query rows over the 8-bit paged KV cache (fblt_paged_attn).
+// Attention of new query rows over the 8-bit paged KV cache (fblt_paged_attn): the streaming kernel for few rows per
+// (sequence, kv head) -- one token, a drafted block, with grouped heads up to 64 rows -- the merge of a split key
+// range, and the dispatch.
+//
+// out = sum_k p_k v_k / sum_k p_k, p_k = 2^(s_k - m), s_k = scale log2(e) q . k, in one pass over the keys with the
+// running maximum m. A cache row is used by at most G * n_new query rows, so the bytes of the cache bound this: the
+// stream has to be read at HBM speed and everything else has to fit beside it.
+//
+//   * CTA = (sequence, kv head, key range, tile of query rows); the rows of one kv head are its G query heads of every
+//     new token, so grouped heads and drafted blocks read a key once.
+//   * A producer warp copies stages of 64 keys (four groups of 16, each inside one page) into a ring with untiled
+//     bulk copies; group i lies 32 bytes further round the banks than group i - 1.
+//   * Four consumer warps multiply with mma.sync m16n8k16 in fp16: codes ARE halves (an 8-bit code has at most 8
+//     significant bits), and the 16 rows of the A operand are 8 query rows in two planes, q = hi + lo with 22 bits
+//     in all, so q . code is fp32 class in ONE instruction and hi + lo are added in registers. Probabilities go back
+//     the same way for P V. The exponents of K multiply scores, those of V probabilities: per (row, key), not per value.
+//     tcgen05 would need 128 rows of A; 8 .. 64 exist.
+//   * Both products see keys and head_dim in an order of our own choosing (a sum has none): lane t of a quad takes 16
+//     neighbouring codes of a K row, lane g 1/8 of a V row, and the 16 keys of one product are 4 of each group, so
+//     that with the 32-byte skew V's column-wise reads touch every bank once.
 #include "paged.cuh"
+#include "tc5.cuh"
 
 namespace fblt {
 
 struct PagedAttnParams {
     PagedView pv;
-    int batch, H, G, total, max_new, block_mode, window;
+    int batch, H, G, total, max_new, block_mode, window, splits, row_tiles;
     const int32_t *cu, *base;
     const float *q;
     int64_t qs;
     float *out;
     int64_t os;
+    float *ws;
     float qscale; // scale * log2(e)
 };
 
-// One warp per (row, query head): keys one after the other, lanes over head_dim.
-template <int HD, int FMT>
-__global__ void __launch_bounds__(128) paged_row_kernel(const PagedAttnParams p) {
-    constexpr int E = HD / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = blockIdx.z, h = blockIdx.y, i = blockIdx.x * 4 + warp;
+__device__ unsigned int g_paged_error; // 0 = ok; otherwise (code << 24) | blockIdx.x of the first CTA that gave up
+
+constexpr int kPsThreads = 160, kPsStages = 4, kPsKeys = 64;
+// A row's weights times the scales of V, p 2^ev, are put into halves in units of 2^(R - kPsHead), R within four of the
+// largest exponent that p 2^ev has had (R follows the row's maximum when that moves): at most 2^(kPsHead + 5), and what
+// is 2^-24 of the largest still has 11 bits, however unequal the rows of V are.
+constexpr int kPsHead = 10, kPsNoUnit = -(1 << 20);
+
+template <int HD>
+struct PsShape {
+    static constexpr int kGroup = 16 * HD;         // bytes of 16 keys
+    static constexpr int kPitch = kGroup + 32;     // see the bank skew above
+    static constexpr int kOffV = 4 * kPitch, kOffE = 8 * kPitch;
+    static constexpr int kStage = 8 * kPitch + 128; // K groups, V groups, 64 exponents each
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// x, y -> (hi, lo) planes of two halves each: 22 bits of a value of ordinary size
+__device__ __forceinline__ void split_half2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+__device__ __forceinline__ int byte_exp(uint32_t w, int i, int lo, int hi) { // signed byte i, clamped to the format's range
+    return min(max((int)(int8_t)(w >> (8 * i)), lo), hi);
+}
+
+// Rows [rt * RT, ..) of kv head `kvh`'s G * n rows; row r is head r % G of token r / G.
+struct RowRange {
+    int lo, hi; // keys the tile's rows see between them
+};
+__device__ __forceinline__ RowRange tile_range(const PagedAttnParams &p, int base, int n, int row0, int rows) {
+    RowRange r;
+    const int i0 = row0 / p.G, i1 = min(n - 1, (row0 + rows - 1) / p.G);
+    r.hi = p.block_mode ? base + n : base + i1 + 1;
+    r.lo = !p.block_mode && p.window > 0 ? max(0, base + i0 - p.window + 1) : 0;
+    return r;
+}
+
+template <int HD, int FMT, int RB, int WR>
+__global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAttnParams p) {
+    using F = KvFormat<FMT>;
+    using S = PsShape<HD>;
+    constexpr int WK = 4 / WR, RT = 8 * RB * WR, KS = HD / 16, NB = HD / 8, PR = HD + 4;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t *ring = smem;
+    uint4 *sq = reinterpret_cast<uint4 *>(smem + kPsStages * S::kStage); // [RB * WR][KS][32] A fragments
+    __shared__ uint64_t full[kPsStages], empty[kPsStages];
+    __shared__ uint32_t vmask[kPsStages];
+    __shared__ float crow[RT], sm[WK * RT], sl[WK * RT];
+    __shared__ int s_abort;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int kvh = blockIdx.x, split = blockIdx.y, b = blockIdx.z / p.row_tiles, rt = blockIdx.z - b * p.row_tiles;
     int r0, n, base;
     if (!paged_seq(p.pv, p.cu, p.base, p.total, b, r0, n, base)) return;
-    if (n > p.max_new && i == 0 && h == 0 && lane == 0) p.pv.raise(FBLT_PAGED_BAD_LENGTH);
-    if (i >= n) return;
-    const int pos = base + i, kvh = h / p.G;
-    const int hi = p.block_mode ? base + n : pos + 1;
-    const int lo = !p.block_mode && p.window > 0 ? max(0, pos - p.window + 1) : 0;
-    float q[E], acc[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        q[e] = p.q[(int64_t)(r0 + i) * p.qs + h * HD + lane * E + e] * p.qscale;
-        acc[e] = 0.0f;
+    if (n > p.max_new) {
+        if (tid == 0) p.pv.raise(FBLT_PAGED_BAD_LENGTH);
     }
-    for (int j = lo; j < hi; ++j) {
-        const int pi = j / p.pv.page_size, page = p.pv.page(b, pi);
-        if (page < 0) {
-            if (lane == 0) p.pv.raise(FBLT_PAGED_BAD_PAGE);
-            continue;
+    const int rows = min(n, p.max_new) * p.G, row0 = rt * RT;
+    if (row0 >= rows) return;
+    const RowRange rr = tile_range(p, base, n, row0, min(RT, rows - row0));
+    // this split's stages
+    const int g0 = rr.lo >> 4, groups = ((rr.hi + 15) >> 4) - g0;
+    const int stages = (groups + 3) >> 2, per = (stages + p.splits - 1) / p.splits;
+    const int st0 = min(stages, split * per), nst = min(stages, st0 + per) - st0;
+    const int kb0 = (g0 + st0 * 4) * 16;
+
+    if (tid == 0) {
+        for (int i = 0; i < kPsStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 4);
         }
-        const int64_t at = p.pv.row(page, kvh, j - pi * p.pv.page_size);
-        const float ks = kv_scale<FMT>(p.pv.ke[at]), vs = kv_scale<FMT>(p.pv.ve[at]);
-        float s = 0.0f, v[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int64_t c = at * HD + lane * E + e;
-            s += q[e] * (kv_values<FMT>(p.pv.kc[c], 1.0f).x * ks);
-            v[e] = kv_values<FMT>(p.pv.vc[c], 1.0f).x * vs;
-        }
-        s = warp_sum(s);
-        if (!finite_f(s)) continue;
-        const float mn = fmaxf(m, s), c = exp2f(m - mn), w = exp2f(s - mn);
-        m = mn;
-        l = l * c + w;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * c + w * v[e];
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncthreads();
+
+    if (warp == 4) {
+        // ---- producer: lane = (group, K / V / K exponents / V exponents)
+        const int gi = (lane >> 2) & 3, what = lane & 3, kvlen = what < 2 ? S::kGroup : 16;
+        for (int st = 0; st < nst; ++st) {
+            const int slot = st % kPsStages, key = kb0 + st * kPsKeys + gi * 16;
+            int page = -1, off = 0;
+            if (lane < 16 && key < rr.hi) {
+                const int pi = key / p.pv.page_size;
+                off = key - pi * p.pv.page_size;
+                page = p.pv.page(b, pi);
+                if (page < 0 && what == 0) p.pv.raise(FBLT_PAGED_BAD_PAGE);
+            }
+            const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
+            if (st >= kPsStages) {
+                bool good = true;
+                if (lane == 0) good = mbar_wait_abort(&empty[slot], ((st / kPsStages) - 1) & 1, (const volatile int *)&s_abort);
+                if (!__shfl_sync(0xffffffffu, good, 0)) {
+                    if (lane == 0) {
+                        *(volatile int *)&s_abort = 1;
+                        atomicCAS(&g_paged_error, 0u, (0x41u << 24) | (blockIdx.x & 0xffffffu));
+                        // the copies in flight land before the CTA goes (bounded, like every wait)
+                        for (int j = max(0, st - kPsStages); j < st; ++j) mbar_wait(&full[j % kPsStages], (j / kPsStages) & 1);
+                    }
+                    break;
+                }
+            }
+            if (lane == 0) {
+                vmask[slot] = (ok & 1) | ((ok >> 3) & 2) | ((ok >> 6) & 4) | ((ok >> 9) & 8);
+                mbar_expect_tx(&full[slot], (__popc(ok) / 4) * (2 * S::kGroup + 32));
+            }
+            __syncwarp();
+            if (page >= 0) {
+                const int64_t at = p.pv.row(page, kvh, off);
+                const void *src = what == 0   ? (const void *)(p.pv.kc + at * HD)
+                                  : what == 1 ? (const void *)(p.pv.vc + at * HD)
+                                  : what == 2 ? (const void *)(p.pv.ke + at)
+                                              : (const void *)(p.pv.ve + at);
+                uint8_t *dst = ring + slot * S::kStage +
+                               (what == 0 ? gi * S::kPitch : what == 1 ? S::kOffV + gi * S::kPitch : S::kOffE + (what - 2) * 64 + gi * 16);
+                bulk_load(dst, src, kvlen, &full[slot]);
+            }
+        }
+    } else {
+        // ---- consumers
+        const int g = lane >> 2, t = lane & 3, wr = warp / WK, wk = warp % WK;
+        // query fragments: a warp per block of 8 rows; row g's values at this lane's head_dim positions
+        for (int rb = warp; rb < RB * WR; rb += 4) {
+            const int r = row0 + rb * 8 + g;
+            float4 x[KS];
+            float a = 0.0f;
+            const bool live = r < rows;
+            const int i = live ? r / p.G : 0;
+            const float *src = p.q + (int64_t)(r0 + i) * p.qs + (int64_t)(kvh * p.G + (r - i * p.G)) * HD;
 #pragma unroll
-    for (int e = 0; e < E; ++e) p.out[(int64_t)(r0 + i) * p.os + h * HD + lane * E + e] = l > 0.0f ? acc[e] / l : 0.0f;
+            for (int s = 0; s < KS; ++s) {
+                const int d = HD == 32 ? 8 * t + 4 * s : 64 * (s >> 2) + 16 * t + 4 * (s & 3);
+                x[s] = live ? *reinterpret_cast<const float4 *>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float v[4] = {x[s].x, x[s].y, x[s].z, x[s].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a = finite_f(v[e]) ? fmaxf(a, fabsf(v[e])) : a;
+            }
+            a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+            a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+            // q * 2^e with its largest value in [2^13, 2^14): halves keep the row's small values too
+            const int e = min(13 - ((__float_as_int(a) >> 23) - 127), 126);
+            const float up = exp2_int(e);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                uint4 f;
+                split_half2(x[s].x * up, x[s].y * up, f.x, f.y);
+                split_half2(x[s].z * up, x[s].w * up, f.z, f.w);
+                sq[(rb * KS + s) * 32 + lane] = f;
+            }
+            if (t == 0) crow[rb * 8 + g] = p.qscale * exp2_int(-e);
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+
+        float m[RB], l[RB], c[RB], o[RB][NB][4];
+        int lo[RB], span[RB], R[RB]; // o holds sums of p v in units of 2^R
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const int ri = (wr * RB + rb) * 8 + g, r = row0 + ri, pos = base + r / p.G;
+            const int hi = r >= rows ? 0 : p.block_mode ? base + n : pos + 1;
+            lo[rb] = r >= rows || p.block_mode || p.window <= 0 ? 0 : max(0, pos - p.window + 1);
+            span[rb] = hi - lo[rb];
+            m[rb] = -INFINITY;
+            l[rb] = 0.0f;
+            R[rb] = kPsNoUnit;
+            c[rb] = crow[ri];
+#pragma unroll
+            for (int j = 0; j < NB; ++j) o[rb][j][0] = o[rb][j][1] = o[rb][j][2] = o[rb][j][3] = 0.0f;
+        }
+        const uint4 *myq = sq + wr * RB * KS * 32 + lane;
+        for (int st = 0; st < nst; ++st) {
+            const int slot = st % kPsStages;
+            if (!mbar_wait_abort(&full[slot], (st / kPsStages) & 1, (const volatile int *)&s_abort)) {
+                *(volatile int *)&s_abort = 1;
+                if (lane == 0) atomicCAS(&g_paged_error, 0u, (0x42u << 24) | (blockIdx.x & 0xffffffu));
+                break;
+            }
+            const uint8_t *stage = ring + slot * S::kStage;
+            const bool there = (vmask[slot] >> t) & 1; // this lane's scores and V rows are keys of group t
+#pragma unroll 1
+            for (int uu = 0; uu < 4 / WK; ++uu) {
+                const int u = wk * (4 / WK) + uu;
+                // ---- S: K rows of this lane are key 4u + (g & 1) (+ 2) of group g / 2
+                float s[RB][2][4];
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int nb = 0; nb < 2; ++nb) s[rb][nb][0] = s[rb][nb][1] = s[rb][nb][2] = s[rb][nb][3] = 0.0f;
+                const uint8_t *krow = stage + (g >> 1) * S::kPitch + (4 * u + (g & 1)) * HD;
+#pragma unroll
+                for (int i = 0; i < (HD + 63) / 64; ++i) {
+                    uint32_t kw[2][4];
+#pragma unroll
+                    for (int nb = 0; nb < 2; ++nb) {
+                        if (HD == 32) {
+                            const uint2 v = *reinterpret_cast<const uint2 *>(krow + nb * 2 * HD + 8 * t);
+                            kw[nb][0] = v.x, kw[nb][1] = v.y;
+                        } else {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(krow + nb * 2 * HD + 64 * i + 16 * t);
+                            kw[nb][0] = v.x, kw[nb][1] = v.y, kw[nb][2] = v.z, kw[nb][3] = v.w;
+                        }
+                    }
+#pragma unroll
+                    for (int w = 0; w < (HD == 32 ? 2 : 4); ++w) {
+                        uint32_t b0[2], b1[2];
+                        F::halves(kw[0][w], b0[0], b1[0]);
+                        F::halves(kw[1][w], b0[1], b1[1]);
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) {
+                            const uint4 a = myq[(rb * KS + 4 * i + w) * 32];
+                            mma_f16(s[rb][0], a, b0[0], b1[0]);
+                            mma_f16(s[rb][1], a, b0[1], b1[1]);
+                        }
+                    }
+                }
+                // ---- softmax: this lane has row g of every block and keys 4u .. 4u + 3 of group t
+                const uint32_t ke = *reinterpret_cast<const uint32_t *>(stage + S::kOffE + t * 16 + 4 * u);
+                const uint32_t ve = *reinterpret_cast<const uint32_t *>(stage + S::kOffE + 64 + t * 16 + 4 * u);
+                const int key = kb0 + st * kPsKeys + t * 16 + 4 * u;
+                float ks[4];
+                int ev[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    ks[j] = exp2_int(byte_exp(ke, j, F::kEmin, F::kEmax) + F::kShift);
+                    ev[j] = byte_exp(ve, j, F::kEmin, F::kEmax);
+                }
+                float mn[RB];
+                bool moved = false;
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float &x = s[rb][j >> 1][j & 1];
+                        x = (x + s[rb][j >> 1][2 + (j & 1)]) * ks[j] * c[rb];
+                        const bool ok = there && (unsigned)(key + j - lo[rb]) < (unsigned)span[rb] && finite_f(x);
+                        x = ok ? x : -INFINITY;
+                        mx = fmaxf(mx, x);
+                    }
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    mn[rb] = fmaxf(m[rb], mx);
+                    moved |= mn[rb] > m[rb];
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        // o's unit follows the maximum down, so its values shrink by less than 2
+                        const float d = m[rb] == -INFINITY ? 0.0f : fmaxf(m[rb] - mn[rb], -4096.0f), whole = floorf(d);
+                        const float f = t5_ex2(d - whole);
+                        l[rb] *= t5_ex2(d);
+                        R[rb] += (int)whole;
+                        m[rb] = mn[rb];
+#pragma unroll
+                        for (int j = 0; j < NB; ++j)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) o[rb][j][k] *= f;
+                    }
+                }
+                int Rn[RB];
+                bool raise = false;
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    const float mref = m[rb] == -INFINITY ? 0.0f : m[rb];
+                    int top = kPsNoUnit;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float &x = s[rb][j >> 1][j & 1];
+                        x = t5_ex2(x - mref);
+                        l[rb] += x;
+                        if (x > 0.0f) top = max(top, (__float_as_int(x) >> 23) - 127 + ev[j]);
+                    }
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    Rn[rb] = top > R[rb] + 4 ? top : R[rb];
+                    raise |= Rn[rb] != R[rb];
+                }
+                if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        const float f = R[rb] - Rn[rb] < -126 ? 0.0f : exp2_int(R[rb] - Rn[rb]);
+                        R[rb] = Rn[rb];
+#pragma unroll
+                        for (int j = 0; j < NB; ++j)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) o[rb][j][k] *= f;
+                    }
+                }
+                uint4 pa[RB];
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    float w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float x = s[rb][j >> 1][j & 1];
+                        w[j] = x > 0.0f ? x * exp2_int(max(ev[j] - R[rb] + kPsHead, -126)) : 0.0f;
+                    }
+                    split_half2(w[0], w[1], pa[rb].x, pa[rb].y);
+                    split_half2(w[2], w[3], pa[rb].z, pa[rb].w);
+                }
+                // ---- O += P V: columns g * HD / 8 .. of keys 4u .. 4u + 3 of group t
+                const uint8_t *vrow = stage + S::kOffV + t * S::kPitch + 4 * u * HD + g * NB;
+                uint32_t vw[4][NB / 4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (HD == 32) {
+                        vw[j][0] = *reinterpret_cast<const uint32_t *>(vrow + j * HD);
+                    } else if (HD == 64) {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(vrow + j * HD);
+                        vw[j][0] = v.x, vw[j][NB / 4 - 1] = v.y;
+                    } else {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(vrow + j * HD);
+                        vw[j][0] = v.x, vw[j][1 % (NB / 4)] = v.y, vw[j][2 % (NB / 4)] = v.z, vw[j][3 % (NB / 4)] = v.w;
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < NB / 4; ++w) {
+                    uint32_t b0[4], b1[4];
+                    F::halves(__byte_perm(vw[0][w], vw[1][w], 0x5140), b0[0], b0[1]);
+                    F::halves(__byte_perm(vw[0][w], vw[1][w], 0x7362), b0[2], b0[3]);
+                    F::halves(__byte_perm(vw[2][w], vw[3][w], 0x5140), b1[0], b1[1]);
+                    F::halves(__byte_perm(vw[2][w], vw[3][w], 0x7362), b1[2], b1[3]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) mma_f16(o[rb][4 * w + j], pa[rb], b0[j], b1[j]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[slot]);
+        }
+        // ---- the warps' shares of the keys meet in shared memory (every copy has landed: the ring is free)
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        float *part = reinterpret_cast<float *>(smem);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const int row = wk * RT + (wr * RB + rb) * 8 + g;
+            const float unit = R[rb] < -126 ? 0.0f : exp2_int(R[rb]);
+            l[rb] += __shfl_xor_sync(0xffffffffu, l[rb], 1);
+            l[rb] += __shfl_xor_sync(0xffffffffu, l[rb], 2);
+            if (t == 0) {
+                sm[row] = m[rb];
+                sl[row] = l[rb];
+            }
+            constexpr float kDown = (float)(1 << F::kShift) / (float)(1 << kPsHead);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < NB; j += 4) {
+                    float4 v;
+                    v.x = (o[rb][j][h] + o[rb][j][2 + h]) * kDown * unit;
+                    v.y = (o[rb][j + 1][h] + o[rb][j + 1][2 + h]) * kDown * unit;
+                    v.z = (o[rb][j + 2][h] + o[rb][j + 2][2 + h]) * kDown * unit;
+                    v.w = (o[rb][j + 3][h] + o[rb][j + 3][2 + h]) * kDown * unit;
+                    *reinterpret_cast<float4 *>(part + row * PR + (2 * t + h) * NB + j) = v;
+                }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (*(volatile int *)&s_abort) return;
+        for (int it = tid; it < RT * (HD / 4); it += 128) {
+            const int ri = it / (HD / 4), d = (it - ri * (HD / 4)) * 4, r = row0 + ri;
+            if (r >= rows) continue;
+            float M = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < WK; ++k) M = fmaxf(M, sm[k * RT + ri]);
+            const float mref = M == -INFINITY ? 0.0f : M;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            float L = 0.0f;
+#pragma unroll
+            for (int k = 0; k < WK; ++k) {
+                const float f = t5_ex2(sm[k * RT + ri] - mref);
+                const float4 v = *reinterpret_cast<const float4 *>(part + (k * RT + ri) * PR + d);
+                L += sl[k * RT + ri] * f;
+                a.x += v.x * f, a.y += v.y * f, a.z += v.z * f, a.w += v.w * f;
+            }
+            const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+            a = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+            const int i = r / p.G, head = kvh * p.G + (r - i * p.G);
+            if (p.splits > 1) {
+                float *w = p.ws + (((int64_t)(r0 + i) * p.H + head) * p.splits + split) * PR;
+                *reinterpret_cast<float4 *>(w + d) = a;
+                if (d == 0) *reinterpret_cast<float2 *>(w + HD) = make_float2(M, L);
+            } else {
+                *reinterpret_cast<float4 *>(p.out + (int64_t)(r0 + i) * p.os + (int64_t)head * HD + d) = a;
+            }
+        }
+    }
+}
+
+// Merge of a split key range: HD / 4 lanes per (packed row, head), o = sum_s L_s 2^(m_s - M) o_s / sum_s L_s 2^(m_s - M).
+// Every piece of a live row was written by the launch before, an empty one with L = 0.
+template <int HD>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams p) {
+    constexpr int LPH = HD / 4, PR = HD + 4;
+    const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
+    const int lane = threadIdx.x % LPH;
+    if (unit >= (int64_t)p.total * p.H) return;
+    const int r = (int)(unit / p.H), head = (int)(unit - (int64_t)r * p.H);
+    int lo = 0, hi = p.batch; // the last sequence that starts at or before r
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(p.cu + mid) <= r) lo = mid;
+        else hi = mid;
+    }
+    int r0, n, base;
+    if (!paged_seq(p.pv, p.cu, p.base, p.total, lo, r0, n, base) || r < r0 || r >= r0 + min(n, p.max_new)) return;
+    const float *w = p.ws + unit * p.splits * PR;
+    float M = -INFINITY, L = 0.0f;
+    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, w[s * PR + HD]);
+    const float mref = M == -INFINITY ? 0.0f : M;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.splits; ++s) {
+        const float2 ml = *reinterpret_cast<const float2 *>(w + s * PR + HD);
+        const float f = t5_ex2(ml.x - mref) * ml.y;
+        const float4 v = *reinterpret_cast<const float4 *>(w + s * PR + lane * 4);
+        L += f;
+        a.x += v.x * f, a.y += v.y * f, a.z += v.z * f, a.w += v.w * f;
+    }
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    *reinterpret_cast<float4 *>(p.out + (int64_t)r * p.os + (int64_t)head * HD + lane * 4) =
+        make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
 }
 
 int paged_attn_check(const fblt_paged_attn_desc *d) {
@@ -82,29 +487,88 @@ int paged_attn_check(const fblt_paged_attn_desc *d) {
     return FBLT_OK;
 }
 
-template <int HD, int FMT>
-static int launch_paged_row(const PagedAttnParams &p, cudaStream_t s) {
-    const dim3 grid((unsigned)((p.max_new + 3) / 4), (unsigned)p.H, (unsigned)p.batch);
-    paged_row_kernel<HD, FMT><<<grid, 128, 0, s>>>(p);
+// ---- plan: tile of rows and pieces of the key range --------------------------------------------------------------
+
+struct PagedPlan {
+    int rb, wr, row_tiles, splits;
+    size_t need;
+};
+
+static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
+    PagedPlan pl;
+    const int64_t rows = (int64_t)d->max_new * (d->num_heads / d->cache.num_kv_heads);
+    pl.rb = rows <= 8 ? 1 : 2;
+    pl.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    const int rt = 8 * pl.rb * pl.wr;
+    pl.row_tiles = (int)((rows + rt - 1) / rt);
+    int64_t s = d->splits;
+    if (s == 0) {
+        const int64_t ctas = (int64_t)d->batch * d->cache.num_kv_heads * pl.row_tiles, target = 148 * 4;
+        s = ctas >= target ? 1 : target / ctas;
+        const int64_t cap = d->max_len / (4 * kPsKeys); // a piece is worth at least four stages
+        if (s > cap) s = cap;
+    }
+    pl.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+    pl.need = pl.splits > 1 ? (size_t)d->total_rows * d->num_heads * pl.splits * (d->cache.head_dim + 4) * sizeof(float) : 0;
+    return pl;
+}
+
+template <int HD, int FMT, int RB, int WR>
+static int launch_stream_t(const PagedAttnParams &p, cudaStream_t s) {
+    constexpr int smem = kPsStages * PsShape<HD>::kStage + RB * WR * (HD / 16) * 512;
+    static_assert(4 / WR * 8 * RB * WR * (HD + 4) * 4 <= smem, "the merge area fits the ring");
+    FBLT_CUDA_TRY(cudaFuncSetAttribute(paged_stream_kernel<HD, FMT, RB, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const dim3 grid((unsigned)p.pv.kvh, (unsigned)p.splits, (unsigned)(p.batch * p.row_tiles));
+    paged_stream_kernel<HD, FMT, RB, WR><<<grid, kPsThreads, smem, s>>>(p);
     count_launch();
-    return check_launch("paged_row_kernel");
+    return check_launch("paged_stream_kernel");
+}
+
+template <int HD>
+static int launch_paged(const PagedAttnParams &p, const PagedPlan &pl, bool e4, cudaStream_t s) {
+    int st;
+#define FBLT_PS(RB, WR) (e4 ? launch_stream_t<HD, FBLT_KV_E4M3, RB, WR>(p, s) : launch_stream_t<HD, FBLT_KV_INT8, RB, WR>(p, s))
+    if (pl.rb == 1) st = FBLT_PS(1, 1);
+    else if (pl.wr == 1) st = FBLT_PS(2, 1);
+    else if (pl.wr == 2) st = FBLT_PS(2, 2);
+    else st = FBLT_PS(2, 4);
+#undef FBLT_PS
+    if (st != FBLT_OK || p.splits <= 1) return st;
+    const int64_t units = (int64_t)p.total * p.H, per = 256 / (HD / 4);
+    paged_merge_kernel<HD><<<(unsigned)((units + per - 1) / per), 256, 0, s>>>(p);
+    count_launch();
+    return check_launch("paged_merge_kernel");
+}
+
+int paged_take_error() {
+    unsigned int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_paged_error, sizeof(v)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(g_paged_error, &zero, sizeof(zero));
+    return (int)v;
 }
 
 } // namespace fblt
 
 extern "C" size_t fblt_paged_attn_workspace(const fblt_paged_attn_desc *d) {
-    if (fblt::paged_attn_check(d) != FBLT_OK) return 0;
-    return 0;
+    if (fblt::paged_attn_check(d) != FBLT_OK || d->batch == 0 || d->total_rows == 0 || d->max_new == 0) return 0;
+    return fblt::paged_plan(d).need;
 }
 
 extern "C" int fblt_paged_attn(const fblt_paged_attn_desc *d, void *workspace, size_t workspace_bytes, void *stream) {
     fblt::NvtxRange nvtx_range("fblt_paged_attn");
     using namespace fblt;
-    (void)workspace;
-    (void)workspace_bytes;
     int st = paged_attn_check(d);
     if (st != FBLT_OK) return st;
     if (d->batch == 0 || d->total_rows == 0 || d->max_new == 0) return FBLT_OK;
+    const PagedPlan pl = paged_plan(d);
+    if (pl.need > 0) {
+        if (!workspace || workspace_bytes < pl.need)
+            return fail(FBLT_ERR_WORKSPACE, "paged_attn: %zu bytes of workspace needed (fblt_paged_attn_workspace), got %zu", pl.need,
+                        workspace_bytes);
+        if ((uintptr_t)workspace & 15) return fail(FBLT_ERR_ARG, "paged_attn: workspace must be 16-byte aligned");
+    }
+    if ((int64_t)d->batch * pl.row_tiles > 65535)
+        return fail(FBLT_ERR_LIMIT, "paged_attn: batch * row tiles (%d) exceed 65535 per launch", pl.row_tiles);
     PagedAttnParams p;
     memset(&p, 0, sizeof(p));
     p.pv = paged_view(d->cache);
@@ -115,18 +579,21 @@ extern "C" int fblt_paged_attn(const fblt_paged_attn_desc *d, void *workspace, s
     p.max_new = d->max_new;
     p.block_mode = d->block_mode ? 1 : 0;
     p.window = d->window;
+    p.splits = pl.splits;
+    p.row_tiles = pl.row_tiles;
     p.cu = d->cu_new;
     p.base = d->base_len;
     p.q = d->q;
     p.qs = d->q_stride;
     p.out = d->out;
     p.os = d->out_stride;
+    p.ws = (float *)workspace;
     p.qscale = d->scale * kLog2e;
     cudaStream_t s = (cudaStream_t)stream;
     const bool e4 = d->cache.format == FBLT_KV_E4M3;
     switch (d->cache.head_dim) {
-    case 32: return e4 ? launch_paged_row<32, FBLT_KV_E4M3>(p, s) : launch_paged_row<32, FBLT_KV_INT8>(p, s);
-    case 64: return e4 ? launch_paged_row<64, FBLT_KV_E4M3>(p, s) : launch_paged_row<64, FBLT_KV_INT8>(p, s);
-    default: return e4 ? launch_paged_row<128, FBLT_KV_E4M3>(p, s) : launch_paged_row<128, FBLT_KV_INT8>(p, s);
+    case 32: return launch_paged<32>(p, pl, e4, s);
+    case 64: return launch_paged<64>(p, pl, e4, s);
+    default: return launch_paged<128>(p, pl, e4, s);
     }
 }

@@ -399,6 +399,7 @@ int gemm5_take_error(); // gemm5_kernel.cu
 int gemm5_take_error_on(cudaStream_t s);
 int unit5_take_error(); // unit5_kernel.cu
 int unit5_take_error_on(cudaStream_t s);
+int paged_take_error(); // paged_attn.cu
 
 // The same report for a caller that has just synchronised its own streams: reads (and, when set,
 // clears) the two error words in order with `s` and waits for `s` only -- other streams of the
@@ -471,5 +472,6 @@ extern "C" int fblt_tcgen05_error(void) {
     if (v) cudaMemcpyToSymbol(fblt::g_t5_error, &zero, sizeof(zero));
     const int g = fblt::gemm5_take_error();
     const int u5 = fblt::unit5_take_error();
-    return v ? (int)v : (u5 ? u5 : g);
+    const int pg = fblt::paged_take_error();
+    return v ? (int)v : (u5 ? u5 : (pg ? pg : g));
 }

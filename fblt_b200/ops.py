@@ -534,6 +534,8 @@ def dv_commit(logits: torch.Tensor, width: int, x: torch.Tensor, l: torch.Tensor
 
 
 # --------------------------------------------------------------------------- paged 8-bit KV cache
+# The make_* functions check their tensors and fill a descriptor that keeps them alive (`keep`); it is made once for a
+# program's buffers and launched as often as it likes.
 
 _KV_FORMATS = {"e4m3": L.KV_E4M3, "int8": L.KV_INT8}
 
@@ -644,6 +646,7 @@ def make_qk_norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], pos:
         d.pos = _table(pos, rows, "pos").data_ptr()
     if status is not None:
         d.status = _table(status, 1, "status").data_ptr()
+    d.keep = [q, k, pos, q_out, k_out, q_gain, k_gain, rope_cos, rope_sin, status]
     return d
 
 
@@ -671,6 +674,7 @@ def make_paged_append(cache: PagedKvCache, cu_new: torch.Tensor, base_len: torch
         raise ValueError("q, q_out, k and v have one row count")
     d.q_gain, d.k_gain = _vector(q_gain, hd, "q_gain"), _vector(k_gain, hd, "k_gain")
     _rope(d, rope_cos, rope_sin, hd)
+    d.keep = [cache, cu_new, base_len, k, v, q, q_out, q_gain, k_gain, rope_cos, rope_sin]
     return d
 
 
@@ -693,6 +697,7 @@ def make_paged_read(cache: PagedKvCache, cu_rows: torch.Tensor, k_out: Optional[
         if t is not None:
             setattr(d, name, _rows(t, cache.num_kv_heads * cache.head_dim, name, (torch.float32, torch.bfloat16)).data_ptr())
             setattr(d, name + "_stride", t.stride(0))
+    d.keep = [cache, cu_rows, k_out, v_out, start]
     return d
 
 
@@ -715,6 +720,7 @@ def make_paged_attn(cache: PagedKvCache, cu_new: torch.Tensor, base_len: torch.T
     if q.shape[0] != out.shape[0]:
         raise ValueError("q and out have one row count")
     d.scale = float(scale)
+    d.keep = [cache, cu_new, base_len, q, out]
     return d
 
 

@@ -452,6 +452,21 @@ def test_offsets_beyond_32_bits(cuda_lib):
         del c
 
 
+def test_workspace_is_checked(cuda_lib):
+    c = make_cache(90, "e4m3", [4000], 1, 64, 16)
+    fill_cache(c, 91, [4000])
+    q, out = randn(gen(1), 1, 64), torch.empty(1, 64, device="cuda")
+    d = ops.make_paged_attn(c, cu([1]), i32([3999]), q, out, 1, 1, 4000, 0.125, splits=4)
+    ws = ops.paged_attn_workspace(d)
+    assert ws is not None
+    for w in (None, ws[:-16], torch.empty(ws.numel() + 16, dtype=torch.uint8, device="cuda")[8:]):
+        with pytest.raises(L.FbltError):
+            ops.paged_attn(d, w)
+    ops.paged_attn(d, ws)
+    torch.cuda.synchronize()
+    check_attention(c, q, out, [1], [3999], 1)
+
+
 def test_more_new_rows_than_announced(cuda_lib):
     """Rows past max_new are left out and reported; the others are right."""
     c = make_cache(92, "int8", [40, 300], 2, 64, 16)
@@ -460,9 +475,9 @@ def test_more_new_rows_than_announced(cuda_lib):
         new, base = [2, max_new + 70], [38, 300 - max_new - 70]
         q, out = attend(c, new, base, 2, 94, max_new=max_new)
         assert c.status_bits() == L.PAGED_BAD_LENGTH
-        whole = torch.full_like(out, math.nan)
+        assert bool(torch.isnan(out[2 + max_new:]).all())
         _, whole = attend(c, new, base, 2, 94)
-        assert torch.equal(out[:2], whole[:2])
+        check_attention(c, q, torch.cat([out[:2 + max_new], whole[2 + max_new:]]), new, base, 2)
         assert c.status_bits() == 0
 
 
