@@ -56,6 +56,13 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
+// 16 bytes global -> shared, bypassing L1
+__device__ __forceinline__ void cp_async_16(void *smem_dst, const void *gmem_src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem_dst)), "l"(gmem_src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 // x, y -> (hi, lo) planes of two halves each: 22 bits of a value of ordinary size
 __device__ __forceinline__ void split_half2(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -111,7 +118,7 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
 
     if (tid == 0) {
         for (int i = 0; i < kPsStages; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], 33);
             mbar_init(&empty[i], 4);
         }
         s_abort = 0;
@@ -120,16 +127,16 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
     __syncthreads();
 
     if (warp == 4) {
-        // ---- producer: lane = (group, K / V / K exponents / V exponents)
-        const int gi = (lane >> 2) & 3, what = lane & 3, kvlen = what < 2 ? S::kGroup : 16;
+        // ---- producer: 16 bytes a lane and copy; lanes 0 .. 3 look the groups' pages up
         for (int st = 0; st < nst; ++st) {
-            const int slot = st % kPsStages, key = kb0 + st * kPsKeys + gi * 16;
-            int page = -1, off = 0;
-            if (lane < 16 && key < rr.hi) {
+            const int slot = st % kPsStages, key = kb0 + st * kPsKeys + lane * 16;
+            int page = -1;
+            int64_t at = 0;
+            if (lane < 4 && key < rr.hi) {
                 const int pi = key / p.pv.page_size;
-                off = key - pi * p.pv.page_size;
                 page = p.pv.page(b, pi);
-                if (page < 0 && what == 0) p.pv.raise(FBLT_PAGED_BAD_PAGE);
+                if (page < 0) p.pv.raise(FBLT_PAGED_BAD_PAGE);
+                else at = p.pv.row(page, kvh, key - pi * p.pv.page_size);
             }
             const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
             if (st >= kPsStages) {
@@ -139,28 +146,31 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
                     if (lane == 0) {
                         *(volatile int *)&s_abort = 1;
                         atomicCAS(&g_paged_error, 0u, (0x41u << 24) | (blockIdx.x & 0xffffffu));
-                        // the copies in flight land before the CTA goes (bounded, like every wait)
-                        for (int j = max(0, st - kPsStages); j < st; ++j) mbar_wait(&full[j % kPsStages], (j / kPsStages) & 1);
                     }
                     break;
                 }
             }
-            if (lane == 0) {
-                vmask[slot] = (ok & 1) | ((ok >> 3) & 2) | ((ok >> 6) & 4) | ((ok >> 9) & 8);
-                mbar_expect_tx(&full[slot], (__popc(ok) / 4) * (2 * S::kGroup + 32));
+            uint8_t *stage = ring + slot * S::kStage;
+#pragma unroll
+            for (int gi = 0; gi < 4; ++gi) {
+                const int64_t row = __shfl_sync(0xffffffffu, at, gi);
+                if (!((ok >> gi) & 1)) continue;
+                const uint8_t *ksrc = p.pv.kc + row * HD + lane * 16, *vsrc = p.pv.vc + row * HD + lane * 16;
+                uint8_t *kdst = stage + gi * S::kPitch + lane * 16;
+#pragma unroll
+                for (int c = 0; c < S::kGroup; c += 512) {
+                    cp_async_16(kdst + c, ksrc + c);
+                    cp_async_16(kdst + S::kOffV + c, vsrc + c);
+                }
+                if (lane < 2) cp_async_16(stage + S::kOffE + lane * 64 + gi * 16, (lane ? p.pv.ve : p.pv.ke) + row);
             }
-            __syncwarp();
-            if (page >= 0) {
-                const int64_t at = p.pv.row(page, kvh, off);
-                const void *src = what == 0   ? (const void *)(p.pv.kc + at * HD)
-                                  : what == 1 ? (const void *)(p.pv.vc + at * HD)
-                                  : what == 2 ? (const void *)(p.pv.ke + at)
-                                              : (const void *)(p.pv.ve + at);
-                uint8_t *dst = ring + slot * S::kStage +
-                               (what == 0 ? gi * S::kPitch : what == 1 ? S::kOffV + gi * S::kPitch : S::kOffE + (what - 2) * 64 + gi * 16);
-                bulk_load(dst, src, kvlen, &full[slot]);
+            cp_async_arrive(&full[slot]); // one arrival a lane, when its copies have landed
+            if (lane == 0) {
+                vmask[slot] = ok;
+                mbar_arrive(&full[slot]);
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory"); // nothing is in flight when the CTA goes
     } else {
         // ---- consumers
         const int g = lane >> 2, t = lane & 3, wr = warp / WK, wk = warp % WK;
