@@ -78,23 +78,19 @@ struct KvFormat;
 template <>
 struct KvFormat<FBLT_KV_E4M3> {
     static constexpr int kEmin = -117, kEmax = 119, kQmax = 448;
-    // The byte's fields moved into a half's (bias 15) give code * 2^-8, subnormal codes included: half subnormals
-    // are fixed point like e4m3's. value = half * 2^(e + kShift).
-    static constexpr int kShift = 8;
+    // value = half * 2^(e + kShift)
+    static constexpr int kShift = 0;
     // least e with a <= 448 * 2^e, from the bits of a = 1.m * 2^x: x - 8, one more where the significand passes 1.75
     static __device__ __forceinline__ int exponent(float a) {
         const int b = __float_as_int(a);
         const int e = (b >> 23) - 127 - 8 + ((b & 0x7fffff) > 0x600000 ? 1 : 0);
         return min(max(e, kEmin), kEmax);
     }
-    // two bytes at the upper halves of their 16-bit lanes -> two halves
-    static __device__ __forceinline__ uint32_t widen(uint32_t x) {
-        return (x & 0x80008000u) | ((x >> 1) & 0x7fff7fffu & 0x3f803f80u);
-    }
     // four codes (one word) -> halves of codes 0, 1 and of codes 2, 3
     static __device__ __forceinline__ void halves(uint32_t w, uint32_t &h01, uint32_t &h23) {
-        h01 = widen(__byte_perm(w, 0, 0x1404));
-        h23 = widen(__byte_perm(w, 0, 0x3424));
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(h01), "=r"(h23)
+            : "r"(w));
     }
     // four scaled finite values -> one word of codes
     static __device__ __forceinline__ uint32_t codes(float a, float b, float c, float d) {

@@ -37,7 +37,7 @@ struct PagedAttnParams {
 
 __device__ unsigned int g_paged_error; // 0 = ok; otherwise (code << 24) | blockIdx.x of the first CTA that gave up
 
-constexpr int kPsThreads = 160, kPsStages = 4, kPsKeys = 64;
+constexpr int kPsThreads = 160;
 // A row's weights times the scales of V, p 2^ev, are put into halves in units of 2^(R - kPsHead), R within four of the
 // largest exponent that p 2^ev has had (R follows the row's maximum when that moves): at most 2^(kPsHead + 5), and what
 // is 2^-24 of the largest still has 11 bits, however unequal the rows of V are.
@@ -45,10 +45,13 @@ constexpr int kPsHead = 10, kPsNoUnit = -(1 << 20);
 
 template <int HD>
 struct PsShape {
-    static constexpr int kGroup = 16 * HD;         // bytes of 16 keys
-    static constexpr int kPitch = kGroup + 32;     // see the bank skew above
+    static constexpr int kKeys = HD == 128 ? 32 : 64;   // keys of a stage
+    static constexpr int kPer = kKeys / 4;              // keys of a group
+    static constexpr int kGroup = kPer * HD;            // their bytes
+    static constexpr int kPitch = kGroup + 32;          // see the bank skew above
     static constexpr int kOffV = 4 * kPitch, kOffE = 8 * kPitch;
-    static constexpr int kStage = 8 * kPitch + 128; // K groups, V groups, 64 exponents each
+    static constexpr int kStage = 8 * kPitch + 2 * kKeys + (HD == 128 ? 64 : 0); // K groups, V groups, exponents
+    static constexpr int kStages = 8;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
@@ -60,6 +63,9 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t 
 __device__ __forceinline__ void cp_async_16(void *smem_dst, const void *gmem_src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem_dst)), "l"(gmem_src) : "memory");
 }
+__device__ __forceinline__ void cp_async_8(void *smem_dst, const void *gmem_src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(smem_dst)), "l"(gmem_src) : "memory");
+}
 __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -70,9 +76,6 @@ __device__ __forceinline__ void split_half2(float x, float y, uint32_t &hi, uint
     const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
-}
-__device__ __forceinline__ int byte_exp(uint32_t w, int i, int lo, int hi) { // signed byte i, clamped to the format's range
-    return min(max((int)(int8_t)(w >> (8 * i)), lo), hi);
 }
 
 // Rows [rt * RT, ..) of kv head `kvh`'s G * n rows; row r is head r % G of token r / G.
@@ -91,13 +94,15 @@ template <int HD, int FMT, int RB, int WR>
 __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAttnParams p) {
     using F = KvFormat<FMT>;
     using S = PsShape<HD>;
-    constexpr int WK = 4 / WR, RT = 8 * RB * WR, KS = HD / 16, NB = HD / 8, PR = HD + 4;
+    constexpr int WK = 4 / WR, RT = 8 * RB * WR, KS = HD / 16, NB = HD / 8, PR = HD + 4, NS = S::kStages;
+    constexpr int U = RB * HD >= 256 ? 1 : 2; // products of 16 keys that go through the softmax together
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem;
-    uint4 *sq = reinterpret_cast<uint4 *>(smem + kPsStages * S::kStage); // [RB * WR][KS][32] A fragments
-    __shared__ uint64_t full[kPsStages], empty[kPsStages];
-    __shared__ uint32_t vmask[kPsStages];
+    uint4 *sq = reinterpret_cast<uint4 *>(smem + NS * S::kStage); // [RB * WR][KS][32] A fragments
+    __shared__ uint64_t full[NS], empty[NS];
+    __shared__ uint32_t vmask[NS];
     __shared__ float crow[RT], sm[WK * RT], sl[WK * RT];
+    __shared__ __align__(16) float scale[4][2][S::kKeys]; // a warp's own: the stage's scales of K and of V
     __shared__ int s_abort;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -110,16 +115,15 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
     const int rows = min(n, p.max_new) * p.G, row0 = rt * RT;
     if (row0 >= rows) return;
     const RowRange rr = tile_range(p, base, n, row0, min(RT, rows - row0));
-    // this split's stages
-    const int g0 = rr.lo >> 4, groups = ((rr.hi + 15) >> 4) - g0;
-    const int stages = (groups + 3) >> 2, per = (stages + p.splits - 1) / p.splits;
+    // this split's stages (a stage starts at a multiple of 16, a page too)
+    const int first = rr.lo & ~15, stages = (rr.hi - first + S::kKeys - 1) / S::kKeys, per = (stages + p.splits - 1) / p.splits;
     const int st0 = min(stages, split * per), nst = min(stages, st0 + per) - st0;
-    const int kb0 = (g0 + st0 * 4) * 16;
+    const int kb0 = first + st0 * S::kKeys;
 
     if (tid == 0) {
-        for (int i = 0; i < kPsStages; ++i) {
+        for (int i = 0; i < NS; ++i) {
             mbar_init(&full[i], 33);
-            mbar_init(&empty[i], 4);
+            mbar_init(&empty[i], WR);
         }
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -127,21 +131,27 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
     __syncthreads();
 
     if (warp == 4) {
-        // ---- producer: 16 bytes a lane and copy; lanes 0 .. 3 look the groups' pages up
+        // ---- producer: 16 bytes a lane and copy; pages are looked up eight stages (a lane per group) at a time, one
+        // look-up ahead
+        auto look = [&](int st) -> int64_t {
+            const int key = kb0 + (st + (lane >> 2)) * S::kKeys + (lane & 3) * S::kPer;
+            if (st + (lane >> 2) >= nst || key >= rr.hi) return -1;
+            const int pi = key / p.pv.page_size, page = p.pv.page(b, pi);
+            if (page < 0) p.pv.raise(FBLT_PAGED_BAD_PAGE);
+            return page < 0 ? -1 : p.pv.row(page, kvh, key - pi * p.pv.page_size);
+        };
+        int64_t now = -1, next = look(0);
         for (int st = 0; st < nst; ++st) {
-            const int slot = st % kPsStages, key = kb0 + st * kPsKeys + lane * 16;
-            int page = -1;
-            int64_t at = 0;
-            if (lane < 4 && key < rr.hi) {
-                const int pi = key / p.pv.page_size;
-                page = p.pv.page(b, pi);
-                if (page < 0) p.pv.raise(FBLT_PAGED_BAD_PAGE);
-                else at = p.pv.row(page, kvh, key - pi * p.pv.page_size);
+            const int slot = st % NS;
+            if ((st & 7) == 0) {
+                now = next;
+                next = look(st + 8);
             }
-            const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
-            if (st >= kPsStages) {
+            const int64_t at = __shfl_sync(0xffffffffu, now, (st & 7) * 4 + (lane & 3));
+            const uint32_t ok = __ballot_sync(0xffffffffu, at >= 0) & 15;
+            if (st >= NS) {
                 bool good = true;
-                if (lane == 0) good = mbar_wait_abort(&empty[slot], ((st / kPsStages) - 1) & 1, (const volatile int *)&s_abort);
+                if (lane == 0) good = mbar_wait_abort(&empty[slot], ((st / NS) - 1) & 1, (const volatile int *)&s_abort);
                 if (!__shfl_sync(0xffffffffu, good, 0)) {
                     if (lane == 0) {
                         *(volatile int *)&s_abort = 1;
@@ -162,7 +172,9 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
                     cp_async_16(kdst + c, ksrc + c);
                     cp_async_16(kdst + S::kOffV + c, vsrc + c);
                 }
-                if (lane < 2) cp_async_16(stage + S::kOffE + lane * 64 + gi * 16, (lane ? p.pv.ve : p.pv.ke) + row);
+                if (lane < S::kPer / 4) // K's exponents, then V's, eight at a time
+                    cp_async_8(stage + S::kOffE + (lane & 1) * S::kKeys + gi * S::kPer + (lane >> 1) * 8,
+                               ((lane & 1) ? p.pv.ve : p.pv.ke) + row + (lane >> 1) * 8);
             }
             cp_async_arrive(&full[slot]); // one arrival a lane, when its copies have landed
             if (lane == 0) {
@@ -210,9 +222,10 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
         int lo[RB], span[RB], R[RB]; // o holds sums of p v in units of 2^R
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            const int ri = (wr * RB + rb) * 8 + g, r = row0 + ri, pos = base + r / p.G;
-            const int hi = r >= rows ? 0 : p.block_mode ? base + n : pos + 1;
-            lo[rb] = r >= rows || p.block_mode || p.window <= 0 ? 0 : max(0, pos - p.window + 1);
+            // a row past the last one has zeros for a query and sees what the last one sees; it is not written
+            const int ri = (wr * RB + rb) * 8 + g, pos = base + min(row0 + ri, rows - 1) / p.G;
+            const int hi = p.block_mode ? base + n : pos + 1;
+            lo[rb] = p.block_mode || p.window <= 0 ? 0 : max(0, pos - p.window + 1);
             span[rb] = hi - lo[rb];
             m[rb] = -INFINITY;
             l[rb] = 0.0f;
@@ -222,88 +235,145 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
             for (int j = 0; j < NB; ++j) o[rb][j][0] = o[rb][j][1] = o[rb][j][2] = o[rb][j][3] = 0.0f;
         }
         const uint4 *myq = sq + wr * RB * KS * 32 + lane;
-        for (int st = 0; st < nst; ++st) {
-            const int slot = st % kPsStages;
-            if (!mbar_wait_abort(&full[slot], (st / kPsStages) & 1, (const volatile int *)&s_abort)) {
+        float(&kscale)[S::kKeys] = scale[warp][0], (&vscale)[S::kKeys] = scale[warp][1];
+        for (int st = wk; st < nst; st += WK) { // a stage belongs to the WR warps of one key share
+            const int slot = st % NS;
+            if (!mbar_wait_abort(&full[slot], (st / NS) & 1, (const volatile int *)&s_abort)) {
                 *(volatile int *)&s_abort = 1;
                 if (lane == 0) atomicCAS(&g_paged_error, 0u, (0x42u << 24) | (blockIdx.x & 0xffffffu));
                 break;
             }
             const uint8_t *stage = ring + slot * S::kStage;
-            const bool there = (vmask[slot] >> t) & 1; // this lane's scores and V rows are keys of group t
+            const int kb = kb0 + st * S::kKeys;
+            const uint32_t here = vmask[slot];
+            const bool there = (here >> t) & 1; // this lane's scores and V rows are keys of group t
+            // every key of the stage is there and every row of the warp sees it
+            const bool whole = __all_sync(0xffffffffu, here == 15 && kb >= lo[0] && kb + S::kKeys <= lo[0] + span[0] &&
+                                                           (RB == 1 || (kb >= lo[RB - 1] && kb + S::kKeys <= lo[RB - 1] + span[RB - 1])));
+            // Slots that hold no visible key may hold any bytes, NaN codes too, and zero times those is no zero: their V
+            // rows are cleared (every warp of the share clears them before it reads, so no one sees them).
+            if (here != 15 || kb < rr.lo || kb + S::kKeys > rr.hi) {
+                for (int i = lane; i < S::kKeys * (HD / 16); i += 32) {
+                    const int k = i / (HD / 16), grp = k / S::kPer;
+                    if (kb + k < rr.lo || kb + k >= rr.hi || !((here >> grp) & 1))
+                        *reinterpret_cast<uint4 *>(ring + slot * S::kStage + S::kOffV + grp * S::kPitch + (k % S::kPer) * HD + (i % (HD / 16)) * 16) =
+                            make_uint4(0, 0, 0, 0);
+                }
+            }
+            // ---- scales of the stage's keys; V's relative to the largest, 2^et
+            int et = kPsNoUnit;
+            {
+                constexpr int KL = S::kKeys / 32; // keys of a lane
+                int e[KL];
+#pragma unroll
+                for (int i = 0; i < KL; ++i) {
+                    const int k = lane * KL + i;
+                    kscale[k] = exp2_int(min(max((int)(int8_t)stage[S::kOffE + k], F::kEmin), F::kEmax) + F::kShift);
+                    e[i] = min(max((int)(int8_t)stage[S::kOffE + S::kKeys + k], F::kEmin), F::kEmax);
+                    if (kb + k >= rr.lo && kb + k < rr.hi && ((here >> (k / S::kPer)) & 1)) et = max(et, e[i]);
+                }
+                et = __reduce_max_sync(0xffffffffu, et);
+#pragma unroll
+                for (int i = 0; i < KL; ++i) vscale[lane * KL + i] = exp2_int(min(max(e[i] - et, -126), 0));
+            }
+            __syncwarp();
 #pragma unroll 1
-            for (int uu = 0; uu < 4 / WK; ++uu) {
-                const int u = wk * (4 / WK) + uu;
-                // ---- S: K rows of this lane are key 4u + (g & 1) (+ 2) of group g / 2
-                float s[RB][2][4];
+            for (int u0 = 0; u0 < S::kPer / 4; u0 += U) {
+                // ---- S: K rows of this lane are keys 4u + (g & 1) and 4u + (g & 1) + 2 of group g / 2
+                float s[RB][U][2][4];
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-                    for (int nb = 0; nb < 2; ++nb) s[rb][nb][0] = s[rb][nb][1] = s[rb][nb][2] = s[rb][nb][3] = 0.0f;
-                const uint8_t *krow = stage + (g >> 1) * S::kPitch + (4 * u + (g & 1)) * HD;
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int nb = 0; nb < 2; ++nb) s[rb][u][nb][0] = s[rb][u][nb][1] = s[rb][u][nb][2] = s[rb][u][nb][3] = 0.0f;
+                const uint8_t *krow = stage + (g >> 1) * S::kPitch + (4 * u0 + (g & 1)) * HD;
 #pragma unroll
                 for (int i = 0; i < (HD + 63) / 64; ++i) {
-                    uint32_t kw[2][4];
+                    constexpr int KW = HD == 32 ? 2 : 4;
+                    uint32_t kw[U][2][KW];
 #pragma unroll
-                    for (int nb = 0; nb < 2; ++nb) {
-                        if (HD == 32) {
-                            const uint2 v = *reinterpret_cast<const uint2 *>(krow + nb * 2 * HD + 8 * t);
-                            kw[nb][0] = v.x, kw[nb][1] = v.y;
-                        } else {
-                            const uint4 v = *reinterpret_cast<const uint4 *>(krow + nb * 2 * HD + 64 * i + 16 * t);
-                            kw[nb][0] = v.x, kw[nb][1] = v.y, kw[nb][2] = v.z, kw[nb][3] = v.w;
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int nb = 0; nb < 2; ++nb) {
+                            const uint8_t *src = krow + (4 * u + 2 * nb) * HD;
+                            if (HD == 32) {
+                                const uint2 v = *reinterpret_cast<const uint2 *>(src + 8 * t);
+                                kw[u][nb][0] = v.x, kw[u][nb][1] = v.y;
+                            } else {
+                                const uint4 v = *reinterpret_cast<const uint4 *>(src + 64 * i + 16 * t);
+                                kw[u][nb][0] = v.x, kw[u][nb][1] = v.y, kw[u][nb][KW - 2] = v.z, kw[u][nb][KW - 1] = v.w;
+                            }
                         }
-                    }
 #pragma unroll
-                    for (int w = 0; w < (HD == 32 ? 2 : 4); ++w) {
-                        uint32_t b0[2], b1[2];
-                        F::halves(kw[0][w], b0[0], b1[0]);
-                        F::halves(kw[1][w], b0[1], b1[1]);
+                    for (int w = 0; w < KW; ++w) {
+                        uint4 a[RB];
 #pragma unroll
-                        for (int rb = 0; rb < RB; ++rb) {
-                            const uint4 a = myq[(rb * KS + 4 * i + w) * 32];
-                            mma_f16(s[rb][0], a, b0[0], b1[0]);
-                            mma_f16(s[rb][1], a, b0[1], b1[1]);
-                        }
+                        for (int rb = 0; rb < RB; ++rb) a[rb] = myq[(rb * KS + 4 * i + w) * 32];
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int nb = 0; nb < 2; ++nb) {
+                                uint32_t b0, b1;
+                                F::halves(kw[u][nb][w], b0, b1);
+#pragma unroll
+                                for (int rb = 0; rb < RB; ++rb) mma_f16(s[rb][u][nb], a[rb], b0, b1);
+                            }
                     }
                 }
                 // ---- softmax: this lane has row g of every block and keys 4u .. 4u + 3 of group t
-                const uint32_t ke = *reinterpret_cast<const uint32_t *>(stage + S::kOffE + t * 16 + 4 * u);
-                const uint32_t ve = *reinterpret_cast<const uint32_t *>(stage + S::kOffE + 64 + t * 16 + 4 * u);
-                const int key = kb0 + st * kPsKeys + t * 16 + 4 * u;
-                float ks[4];
-                int ev[4];
+                const int kl = t * S::kPer + 4 * u0; // key within the stage
+                float2 x[RB][U][2];
+                float mn[RB], odd = 0.0f; // odd: NaN once a score is not finite
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    ks[j] = exp2_int(byte_exp(ke, j, F::kEmin, F::kEmax) + F::kShift);
-                    ev[j] = byte_exp(ve, j, F::kEmin, F::kEmax);
+                for (int rb = 0; rb < RB; ++rb) mn[rb] = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float4 ks = *reinterpret_cast<const float4 *>(&kscale[kl + 4 * u]);
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                        for (int nb = 0; nb < 2; ++nb) {
+                            const float(&v)[4] = s[rb][u][nb];
+                            float2 y = __fadd2_rn(make_float2(v[0], v[1]), make_float2(v[2], v[3]));
+                            y = __fmul2_rn(__fmul2_rn(y, nb ? make_float2(ks.z, ks.w) : make_float2(ks.x, ks.y)), make_float2(c[rb], c[rb]));
+                            x[rb][u][nb] = y;
+                            odd = fmaf(y.x, 0.0f, fmaf(y.y, 0.0f, odd));
+                            mn[rb] = fmaxf(mn[rb], fmaxf(y.x, y.y));
+                        }
                 }
-                float mn[RB];
+                if (!whole || __any_sync(0xffffffffu, odd != 0.0f)) {
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        mn[rb] = -INFINITY;
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int nb = 0; nb < 2; ++nb) {
+                                float2 &y = x[rb][u][nb];
+                                const int k = kb + kl + 4 * u + 2 * nb - lo[rb];
+                                y.x = there && (unsigned)k < (unsigned)span[rb] && finite_f(y.x) ? y.x : -INFINITY;
+                                y.y = there && (unsigned)(k + 1) < (unsigned)span[rb] && finite_f(y.y) ? y.y : -INFINITY;
+                                mn[rb] = fmaxf(mn[rb], fmaxf(y.x, y.y));
+                            }
+                    }
+                }
                 bool moved = false;
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float &x = s[rb][j >> 1][j & 1];
-                        x = (x + s[rb][j >> 1][2 + (j & 1)]) * ks[j] * c[rb];
-                        const bool ok = there && (unsigned)(key + j - lo[rb]) < (unsigned)span[rb] && finite_f(x);
-                        x = ok ? x : -INFINITY;
-                        mx = fmaxf(mx, x);
-                    }
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    mn[rb] = fmaxf(m[rb], mx);
+                    mn[rb] = fmaxf(mn[rb], __shfl_xor_sync(0xffffffffu, mn[rb], 1));
+                    mn[rb] = fmaxf(mn[rb], __shfl_xor_sync(0xffffffffu, mn[rb], 2));
+                    mn[rb] = fmaxf(mn[rb], m[rb]);
                     moved |= mn[rb] > m[rb];
                 }
                 if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb) {
                         // o's unit follows the maximum down, so its values shrink by less than 2
-                        const float d = m[rb] == -INFINITY ? 0.0f : fmaxf(m[rb] - mn[rb], -4096.0f), whole = floorf(d);
-                        const float f = t5_ex2(d - whole);
+                        const float d = m[rb] == -INFINITY ? 0.0f : fmaxf(m[rb] - mn[rb], -4096.0f), down = floorf(d);
+                        const float f = t5_ex2(d - down);
                         l[rb] *= t5_ex2(d);
-                        R[rb] += (int)whole;
+                        R[rb] += (int)down;
                         m[rb] = mn[rb];
 #pragma unroll
                         for (int j = 0; j < NB; ++j)
@@ -311,73 +381,84 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
                             for (int k = 0; k < 4; ++k) o[rb][j][k] *= f;
                     }
                 }
-                int Rn[RB];
-                bool raise = false;
+                float top[RB]; // the largest p 2^(ev - et)
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    const float mref = m[rb] == -INFINITY ? 0.0f : m[rb];
-                    int top = kPsNoUnit;
+                    const float mref = m[rb] == -INFINITY ? 0.0f : -m[rb];
+                    float2 sum = make_float2(0.0f, 0.0f);
+                    top[rb] = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float &x = s[rb][j >> 1][j & 1];
-                        x = t5_ex2(x - mref);
-                        l[rb] += x;
-                        if (x > 0.0f) top = max(top, (__float_as_int(x) >> 23) - 127 + ev[j]);
+                    for (int u = 0; u < U; ++u) {
+                        const float4 vs = *reinterpret_cast<const float4 *>(&vscale[kl + 4 * u]);
+#pragma unroll
+                        for (int nb = 0; nb < 2; ++nb) {
+                            float2 &y = x[rb][u][nb];
+                            y = __fadd2_rn(y, make_float2(mref, mref));
+                            y = make_float2(t5_ex2(y.x), t5_ex2(y.y));
+                            sum = __fadd2_rn(sum, y);
+                            y = __fmul2_rn(y, nb ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y));
+                            top[rb] = fmaxf(top[rb], fmaxf(y.x, y.y));
+                        }
                     }
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    Rn[rb] = top > R[rb] + 4 ? top : R[rb];
-                    raise |= Rn[rb] != R[rb];
+                    l[rb] += sum.x + sum.y;
                 }
+                bool raise = false;
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) raise |= top[rb] > 0.0f && (__float_as_int(top[rb]) >> 23) - 127 + et > R[rb] + 4;
                 if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb) {
-                        const float f = R[rb] - Rn[rb] < -126 ? 0.0f : exp2_int(R[rb] - Rn[rb]);
-                        R[rb] = Rn[rb];
+                        float w = fmaxf(top[rb], __shfl_xor_sync(0xffffffffu, top[rb], 1));
+                        w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 2));
+                        const int Rn = w > 0.0f ? max(R[rb], (__float_as_int(w) >> 23) - 127 + et) : R[rb];
+                        const float f = R[rb] - Rn < -126 ? 0.0f : exp2_int(R[rb] - Rn);
+                        R[rb] = Rn;
 #pragma unroll
                         for (int j = 0; j < NB; ++j)
 #pragma unroll
                             for (int k = 0; k < 4; ++k) o[rb][j][k] *= f;
                     }
                 }
-                uint4 pa[RB];
+                uint4 pa[RB][U];
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    float w[4];
+                    // p 2^(ev - et) in units of 2^(R - kPsHead); a row without a weight has only zeros
+                    const float f = exp2_int(min(max(et - R[rb] + kPsHead, -126), 126));
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float x = s[rb][j >> 1][j & 1];
-                        w[j] = x > 0.0f ? x * exp2_int(max(ev[j] - R[rb] + kPsHead, -126)) : 0.0f;
+                    for (int u = 0; u < U; ++u) {
+                        split_half2(x[rb][u][0].x * f, x[rb][u][0].y * f, pa[rb][u].x, pa[rb][u].y);
+                        split_half2(x[rb][u][1].x * f, x[rb][u][1].y * f, pa[rb][u].z, pa[rb][u].w);
                     }
-                    split_half2(w[0], w[1], pa[rb].x, pa[rb].y);
-                    split_half2(w[2], w[3], pa[rb].z, pa[rb].w);
                 }
                 // ---- O += P V: columns g * HD / 8 .. of keys 4u .. 4u + 3 of group t
-                const uint8_t *vrow = stage + S::kOffV + t * S::kPitch + 4 * u * HD + g * NB;
-                uint32_t vw[4][NB / 4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (HD == 32) {
-                        vw[j][0] = *reinterpret_cast<const uint32_t *>(vrow + j * HD);
-                    } else if (HD == 64) {
-                        const uint2 v = *reinterpret_cast<const uint2 *>(vrow + j * HD);
-                        vw[j][0] = v.x, vw[j][NB / 4 - 1] = v.y;
-                    } else {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(vrow + j * HD);
-                        vw[j][0] = v.x, vw[j][1 % (NB / 4)] = v.y, vw[j][2 % (NB / 4)] = v.z, vw[j][3 % (NB / 4)] = v.w;
+                for (int u = 0; u < U; ++u) {
+                    const uint8_t *vrow = stage + S::kOffV + t * S::kPitch + 4 * (u0 + u) * HD + g * NB;
+                    uint32_t vw[4][NB / 4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (HD == 32) {
+                            vw[j][0] = *reinterpret_cast<const uint32_t *>(vrow + j * HD);
+                        } else if (HD == 64) {
+                            const uint2 v = *reinterpret_cast<const uint2 *>(vrow + j * HD);
+                            vw[j][0] = v.x, vw[j][NB / 4 - 1] = v.y;
+                        } else {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(vrow + j * HD);
+                            vw[j][0] = v.x, vw[j][1 % (NB / 4)] = v.y, vw[j][2 % (NB / 4)] = v.z, vw[j][3 % (NB / 4)] = v.w;
+                        }
                     }
-                }
 #pragma unroll
-                for (int w = 0; w < NB / 4; ++w) {
-                    uint32_t b0[4], b1[4];
-                    F::halves(__byte_perm(vw[0][w], vw[1][w], 0x5140), b0[0], b0[1]);
-                    F::halves(__byte_perm(vw[0][w], vw[1][w], 0x7362), b0[2], b0[3]);
-                    F::halves(__byte_perm(vw[2][w], vw[3][w], 0x5140), b1[0], b1[1]);
-                    F::halves(__byte_perm(vw[2][w], vw[3][w], 0x7362), b1[2], b1[3]);
+                    for (int w = 0; w < NB / 4; ++w) {
+                        uint32_t b0[4], b1[4];
+                        F::halves(__byte_perm(vw[0][w], vw[1][w], 0x5140), b0[0], b0[1]);
+                        F::halves(__byte_perm(vw[0][w], vw[1][w], 0x7362), b0[2], b0[3]);
+                        F::halves(__byte_perm(vw[2][w], vw[3][w], 0x5140), b1[0], b1[1]);
+                        F::halves(__byte_perm(vw[2][w], vw[3][w], 0x7362), b1[2], b1[3]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                        for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int rb = 0; rb < RB; ++rb) mma_f16(o[rb][4 * w + j], pa[rb], b0[j], b1[j]);
+                            for (int rb = 0; rb < RB; ++rb) mma_f16(o[rb][4 * w + j], pa[rb][u], b0[j], b1[j]);
+                    }
                 }
             }
             __syncwarp();
@@ -507,15 +588,17 @@ struct PagedPlan {
 static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
     PagedPlan pl;
     const int64_t rows = (int64_t)d->max_new * (d->num_heads / d->cache.num_kv_heads);
-    pl.rb = rows <= 8 ? 1 : 2;
-    pl.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    // Two blocks of 8 rows a warp while their output (64 registers a block at head_dim 128) leaves room for more than
+    // one CTA on an SM: at 128 one block (block of 8 rows x 4 heads over 64 caches: 557 us, two blocks 708 us).
+    pl.rb = rows <= 8 || d->cache.head_dim == 128 ? 1 : 2;
+    pl.wr = rows <= 8 * pl.rb ? 1 : rows <= 16 * pl.rb ? 2 : 4;
     const int rt = 8 * pl.rb * pl.wr;
     pl.row_tiles = (int)((rows + rt - 1) / rt);
     int64_t s = d->splits;
     if (s == 0) {
         const int64_t ctas = (int64_t)d->batch * d->cache.num_kv_heads * pl.row_tiles, target = 148 * 4;
         s = ctas >= target ? 1 : target / ctas;
-        const int64_t cap = d->max_len / (4 * kPsKeys); // a piece is worth at least four stages
+        const int64_t cap = d->max_len / 256; // a piece is worth a few stages
         if (s > cap) s = cap;
     }
     pl.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
@@ -525,7 +608,7 @@ static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
 
 template <int HD, int FMT, int RB, int WR>
 static int launch_stream_t(const PagedAttnParams &p, cudaStream_t s) {
-    constexpr int smem = kPsStages * PsShape<HD>::kStage + RB * WR * (HD / 16) * 512;
+    constexpr int smem = PsShape<HD>::kStages * PsShape<HD>::kStage + RB * WR * (HD / 16) * 512;
     static_assert(4 / WR * 8 * RB * WR * (HD + 4) * 4 <= smem, "the merge area fits the ring");
     FBLT_CUDA_TRY(cudaFuncSetAttribute(paged_stream_kernel<HD, FMT, RB, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const dim3 grid((unsigned)p.pv.kvh, (unsigned)p.splits, (unsigned)(p.batch * p.row_tiles));
@@ -538,10 +621,11 @@ template <int HD>
 static int launch_paged(const PagedAttnParams &p, const PagedPlan &pl, bool e4, cudaStream_t s) {
     int st;
 #define FBLT_PS(RB, WR) (e4 ? launch_stream_t<HD, FBLT_KV_E4M3, RB, WR>(p, s) : launch_stream_t<HD, FBLT_KV_INT8, RB, WR>(p, s))
-    if (pl.rb == 1) st = FBLT_PS(1, 1);
-    else if (pl.wr == 1) st = FBLT_PS(2, 1);
-    else if (pl.wr == 2) st = FBLT_PS(2, 2);
-    else st = FBLT_PS(2, 4);
+    constexpr int B = HD == 128 ? 1 : 2;
+    if (pl.rb == 1 && pl.wr == 1) st = FBLT_PS(1, 1);
+    else if (pl.wr == 1) st = FBLT_PS(B, 1);
+    else if (pl.wr == 2) st = FBLT_PS(B, 2);
+    else st = FBLT_PS(B, 4);
 #undef FBLT_PS
     if (st != FBLT_OK || p.splits <= 1) return st;
     const int64_t units = (int64_t)p.total * p.H, per = 256 / (HD / 4);

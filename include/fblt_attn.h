@@ -689,8 +689,9 @@ int fblt_kv_self_attention_step(const fblt_kv_step_desc *desc, void *stream);
  * (e is clamped to those bounds; a code that would pass Qmax then is Qmax.) With a power of two as the scale the
  * quotient x * 2^-e is exact, so a row has one quantised form whoever computes it, every stored value is a bf16
  * number, and reading it back is exact. A NaN is stored as 0 and an infinity as +-Qmax * 2^e with e from the finite
- * values; both raise FBLT_PAGED_NONFINITE. The library never writes the e4m3 codes 0x7f / 0xff (NaN); a cache that
- * holds them is read as +-480 * 2^e.
+ * values; both raise FBLT_PAGED_NONFINITE. The library never writes the e4m3 codes 0x7f / 0xff (NaN); what the rows of
+ * a sequence become whose visible positions hold them is not specified. Slots that no visible position has may hold
+ * any bytes.
  */
 typedef enum { FBLT_KV_E4M3 = 0, FBLT_KV_INT8 = 1 } fblt_kv_format;
 

@@ -281,7 +281,8 @@ def test_read_of_every_byte(cuda_lib):
         ops.paged_read(ops.make_paged_read(c, cu([21]), o, None, start=i32([11])))
         torch.cuda.synchronize()
         want = stored(c, 0, 32, "k")[11:].flatten(1)
-        big = want.abs() > 3.3e38  # -128 * 2^121 and 480 * 2^119 pass fp32's range; the library writes neither code
+        # -128 * 2^121 passes fp32's range and the e4m3 codes 0x7f / 0xff are NaN; the library writes none of them
+        big = (want.abs() > 3.3e38) | ((want.abs() == 480 * 2.0 ** torch.floor(torch.log2(want.abs() / 256))) & (fmt == "e4m3"))
         assert torch.equal(torch.where(big, 0.0, o.double().cpu()), torch.where(big, 0.0, want))
 
 
