@@ -14,7 +14,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libfblt_attn.so"
 SOURCES = ["status.cu", "head_l0.cu", "row_kernel.cu", "tile_kernel.cu", "tile5_kernel.cu", "unit5_kernel.cu", "gemm5_kernel.cu", "mha.cu", "decode_kernel.cu", "decisions.cu", "mask_dense.cu", "gather.cu",
-           "paged_cache.cu", "paged_attn.cu", "api.cu", "session.cu"]
+           "paged_cache.cu", "paged_attn.cu", "paged_chunk.cu", "api.cu", "session.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -140,4 +140,38 @@ __device__ __forceinline__ float kv_scale(int e) { // exponents outside the form
     return exp2_int(min(max(e, KvFormat<FMT>::kEmin), KvFormat<FMT>::kEmax) + KvFormat<FMT>::kShift);
 }
 
+// x, y -> (hi, lo) planes of two halves each: 22 bits of a value of ordinary size
+__device__ __forceinline__ void split_half2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// What the attention kernels get. The rows of one kv head are numbered r = i * G + g: head kvh * G + g of token i.
+struct PagedAttnParams {
+    PagedView pv;
+    int batch, H, G, total, max_new, block_mode, window, splits, row_tiles;
+    const int32_t *cu, *base;
+    const float *q;
+    int64_t qs;
+    float *out;
+    int64_t os;
+    float *ws;
+    float qscale; // scale * log2(e)
+};
+
+// Keys that rows [row0, row0 + rows) of a sequence with n new rows at `base` see between them.
+struct RowRange {
+    int lo, hi; // keys the tile's rows see between them
+};
+__device__ __forceinline__ RowRange tile_range(const PagedAttnParams &p, int base, int n, int row0, int rows) {
+    RowRange r;
+    const int i0 = row0 / p.G, i1 = min(n - 1, (row0 + rows - 1) / p.G);
+    r.hi = p.block_mode ? base + n : base + i1 + 1;
+    r.lo = !p.block_mode && p.window > 0 ? max(0, base + i0 - p.window + 1) : 0;
+    return r;
+}
+
 } // namespace fblt

@@ -23,18 +23,6 @@
 
 namespace fblt {
 
-struct PagedAttnParams {
-    PagedView pv;
-    int batch, H, G, total, max_new, block_mode, window, splits, row_tiles;
-    const int32_t *cu, *base;
-    const float *q;
-    int64_t qs;
-    float *out;
-    int64_t os;
-    float *ws;
-    float qscale; // scale * log2(e)
-};
-
 __device__ unsigned int g_paged_error; // 0 = ok; otherwise (code << 24) | blockIdx.x of the first CTA that gave up
 
 constexpr int kPsThreads = 160;
@@ -69,27 +57,6 @@ __device__ __forceinline__ void cp_async_8(void *smem_dst, const void *gmem_src)
 __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// x, y -> (hi, lo) planes of two halves each: 22 bits of a value of ordinary size
-__device__ __forceinline__ void split_half2(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
-}
-
-// Rows [rt * RT, ..) of kv head `kvh`'s G * n rows; row r is head r % G of token r / G.
-struct RowRange {
-    int lo, hi; // keys the tile's rows see between them
-};
-__device__ __forceinline__ RowRange tile_range(const PagedAttnParams &p, int base, int n, int row0, int rows) {
-    RowRange r;
-    const int i0 = row0 / p.G, i1 = min(n - 1, (row0 + rows - 1) / p.G);
-    r.hi = p.block_mode ? base + n : base + i1 + 1;
-    r.lo = !p.block_mode && p.window > 0 ? max(0, base + i0 - p.window + 1) : 0;
-    return r;
-}
-
 template <int HD, int FMT, int RB, int WR>
 __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAttnParams p) {
     using F = KvFormat<FMT>;
@@ -580,7 +547,11 @@ int paged_attn_check(const fblt_paged_attn_desc *d) {
 
 // ---- plan: tile of rows and pieces of the key range --------------------------------------------------------------
 
+int launch_paged_chunk(const PagedAttnParams &p, int hd, bool e4, cudaStream_t s); // paged_chunk.cu
+int chunk_take_error();
+
 struct PagedPlan {
+    bool chunk; // the tcgen05 kernel
     int rb, wr, row_tiles, splits;
     size_t need;
 };
@@ -588,18 +559,37 @@ struct PagedPlan {
 static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
     PagedPlan pl;
     const int64_t rows = (int64_t)d->max_new * (d->num_heads / d->cache.num_kv_heads);
-    // Two blocks of 8 rows a warp while their output (64 registers a block at head_dim 128) leaves room for more than
-    // one CTA on an SM: at 128 one block (block of 8 rows x 4 heads over 64 caches: 557 us, two blocks 708 us).
-    pl.rb = rows <= 8 || d->cache.head_dim == 128 ? 1 : 2;
-    pl.wr = rows <= 8 * pl.rb ? 1 : rows <= 16 * pl.rb ? 2 : 4;
-    const int rt = 8 * pl.rb * pl.wr;
-    pl.row_tiles = (int)((rows + rt - 1) / rt);
+    const int64_t units = (int64_t)d->batch * d->cache.num_kv_heads;
     int64_t s = d->splits;
-    if (s == 0) {
-        const int64_t ctas = (int64_t)d->batch * d->cache.num_kv_heads * pl.row_tiles, target = 148 * 4;
-        s = ctas >= target ? 1 : target / ctas;
-        const int64_t cap = d->max_len / 256; // a piece is worth a few stages
-        if (s > cap) s = cap;
+    pl.chunk = rows > 64;
+    if (pl.chunk) {
+        pl.rb = pl.wr = 0;
+        pl.row_tiles = (int)((rows + 255) / 256);
+        if (s == 0) {
+            // one CTA an SM: the number of pieces (of at least 1024 keys) that leaves the fewest SMs idle in the last wave
+            double best = 0.0;
+            for (int64_t c = 1; c <= 8 && (c == 1 || d->max_len / c >= 1024); ++c) {
+                const int64_t ctas = units * pl.row_tiles * c, waves = (ctas + 147) / 148;
+                const double use = (double)ctas / (double)(waves * 148) - 0.01 * (double)(c - 1);
+                if (use > best) {
+                    best = use;
+                    s = c;
+                }
+            }
+        }
+    } else {
+        // Two blocks of 8 rows a warp while their output (64 registers a block at head_dim 128) leaves room for more than
+        // one CTA on an SM: at 128 one block (block of 8 rows x 4 heads over 64 caches: 557 us, two blocks 708 us).
+        pl.rb = rows <= 8 || d->cache.head_dim == 128 ? 1 : 2;
+        pl.wr = rows <= 8 * pl.rb ? 1 : rows <= 16 * pl.rb ? 2 : 4;
+        const int rt = 8 * pl.rb * pl.wr;
+        pl.row_tiles = (int)((rows + rt - 1) / rt);
+        if (s == 0) {
+            const int64_t ctas = units * pl.row_tiles, target = 148 * 4;
+            s = ctas >= target ? 1 : target / ctas;
+            const int64_t cap = d->max_len / 256; // a piece is worth a few stages
+            if (s > cap) s = cap;
+        }
     }
     pl.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
     pl.need = pl.splits > 1 ? (size_t)d->total_rows * d->num_heads * pl.splits * (d->cache.head_dim + 4) * sizeof(float) : 0;
@@ -619,10 +609,11 @@ static int launch_stream_t(const PagedAttnParams &p, cudaStream_t s) {
 
 template <int HD>
 static int launch_paged(const PagedAttnParams &p, const PagedPlan &pl, bool e4, cudaStream_t s) {
-    int st;
-#define FBLT_PS(RB, WR) (e4 ? launch_stream_t<HD, FBLT_KV_E4M3, RB, WR>(p, s) : launch_stream_t<HD, FBLT_KV_INT8, RB, WR>(p, s))
     constexpr int B = HD == 128 ? 1 : 2;
-    if (pl.rb == 1 && pl.wr == 1) st = FBLT_PS(1, 1);
+    int st;
+    if (pl.chunk) st = launch_paged_chunk(p, HD, e4, s);
+#define FBLT_PS(RB, WR) (e4 ? launch_stream_t<HD, FBLT_KV_E4M3, RB, WR>(p, s) : launch_stream_t<HD, FBLT_KV_INT8, RB, WR>(p, s))
+    else if (pl.rb == 1 && pl.wr == 1) st = FBLT_PS(1, 1);
     else if (pl.wr == 1) st = FBLT_PS(B, 1);
     else if (pl.wr == 2) st = FBLT_PS(B, 2);
     else st = FBLT_PS(B, 4);
@@ -638,7 +629,8 @@ int paged_take_error() {
     unsigned int v = 0, zero = 0;
     if (cudaMemcpyFromSymbol(&v, g_paged_error, sizeof(v)) != cudaSuccess) return -1;
     if (v) cudaMemcpyToSymbol(g_paged_error, &zero, sizeof(zero));
-    return (int)v;
+    const int c = chunk_take_error();
+    return v ? (int)v : c;
 }
 
 } // namespace fblt

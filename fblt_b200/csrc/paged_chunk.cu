@@ -1,0 +1,458 @@
+// Attention of a chunk of new rows over the 8-bit paged KV cache on tcgen05 (fblt_paged_attn with many query rows per
+// kv head: prompts taken in chunks).
+//
+// CTA = (sequence, kv head, key range, 256 query rows as two tiles of 128), one per SM; K and V tiles of BN keys are
+// converted once for both query tiles. Products in fp32 class from 16-bit operands:
+//   S = Q K^T    an 8-bit code is a half as it stands, so K is one fp16 plane; Q (scaled by its row's power of two) is
+//                two, 22 bits. K's exponents multiply the columns of S when the softmax reads them.
+//   O += P V     code 2^e is a bf16 value, so V is one bf16 plane with its scale in it; P is three, cut off bit by bit
+//                (8 + 8 + 8 = all of fp32's 24), which needs no range of its own however unequal the rows of V are.
+// Two MMAs for every Q K^T, three for every P V: 5/2 of the products that bf16 attention would issue.
+//
+// Roles (13 warps), which meet on mbarriers only; every wait is bounded:
+//   softmax (2 x 4 warps)  one thread per query row (TMEM lane): running maximum and sum, P back to TMEM over the scores
+//                          it came from (32 keys: 32 columns of S become 48 of P; block c starts at column 48 c, S lies
+//                          at the end of the region, so a block never covers scores that have not been read). O stays in
+//                          TMEM and is rescaled only where a maximum has grown by more than 2^8.
+//   converters (4 warps)   pages -> registers (one tile ahead) -> 16-bit operands in shared memory, in 8-row x 16-byte
+//                          core matrices (K read K-major, V MN-major: the same bytes, no transposition)
+//   issuer (1 thread)      while one query tile's softmax runs, the tensor cores have the other tile's products
+#include "paged.cuh"
+#include "tc5.cuh"
+
+namespace fblt {
+
+constexpr int kPcThreads = 416, kPcSoft = 256, kPcConv = 128; // + the issuer's warp
+constexpr int kPcRows = 128;
+
+__device__ unsigned int g_chunk_error; // 0 = ok; otherwise (code << 24) | blockIdx.x of the first CTA that gave up
+
+template <int HD>
+struct PcShape {
+    static constexpr int BN = HD == 128 ? 64 : 128; // keys of a tile: S, P and O of two query tiles fit 512 columns
+    static constexpr int kQPlane = kPcRows * HD * 2, kKv = BN * HD * 2;
+    static constexpr int kOffKv = 4 * kQPlane; // two tiles, two planes of Q
+    static constexpr int kSmem = kOffKv + 4 * kKv;
+    static constexpr int kP = BN * 3 / 2, kS = kP - BN, kO = kP, kTile = 256; // TMEM columns of a query tile
+};
+
+// fp16 / bf16 operands, fp32 accumulate; B K-major or MN-major
+__host__ __device__ constexpr uint32_t pc_idesc(int n, bool bf16, bool mn_major) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(kPcRows >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+
+struct PcBars {
+    uint64_t q_full, k_full[2], v_full[2], kv_empty[2], s_full[2], p_ready[2], o_full, fin;
+};
+
+template <int HD, int FMT>
+__global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedAttnParams p) {
+    using F = KvFormat<FMT>;
+    using S = PcShape<HD>;
+    constexpr int BN = S::BN, CH = BN / 32, PR = HD + 4;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ PcBars bars;
+    __shared__ __align__(16) float kscale[2][BN];
+    __shared__ __align__(8) uint8_t present[2][8]; // groups of 16 keys whose page exists and that the CTA reads
+    __shared__ uint32_t tmem_slot;
+    __shared__ int s_abort;
+    const volatile int *abortp = &s_abort;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int kvh = blockIdx.x, split = blockIdx.y, b = blockIdx.z / p.row_tiles;
+    const int rt = p.row_tiles - 1 - (blockIdx.z - b * p.row_tiles); // later rows see more keys: they go first
+    int r0, n, base;
+    if (!paged_seq(p.pv, p.cu, p.base, p.total, b, r0, n, base)) return;
+    if (n > p.max_new && tid == 0) p.pv.raise(FBLT_PAGED_BAD_LENGTH);
+    const int rows = min(n, p.max_new) * p.G, row0 = rt * 2 * kPcRows;
+    if (row0 >= rows) return;
+    const int tiles = rows - row0 > kPcRows ? 2 : 1;
+    const RowRange rr = tile_range(p, base, n, row0, min(2 * kPcRows, rows - row0));
+    const int first = rr.lo & ~15, steps = (rr.hi - first + BN - 1) / BN, per = (steps + p.splits - 1) / p.splits;
+    const int st0 = min(steps, split * per), nst = min(steps, st0 + per) - st0;
+    const int kb0 = first + st0 * BN;
+    const uint32_t sbase = smem_u32(smem);
+
+    auto give_up = [&](unsigned code) {
+        *(volatile int *)&s_abort = 1;
+        atomicCAS(&g_chunk_error, 0u, (code << 24) | (blockIdx.x & 0xffffffu));
+    };
+
+    if (tid == 0) {
+        mbar_init(&bars.q_full, tiles * kPcRows);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.k_full[i], kPcConv);
+            mbar_init(&bars.v_full[i], kPcConv);
+            mbar_init(&bars.kv_empty[i], 1);
+            mbar_init(&bars.s_full[i], 1);
+            mbar_init(&bars.p_ready[i], kPcRows);
+        }
+        mbar_init(&bars.o_full, 1);
+        mbar_init(&bars.fin, 1);
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp < 8) {
+        // ================= softmax: this thread's query row =================
+        const int T = warp >> 2, rl = (warp & 3) * 32 + lane, r = row0 + T * kPcRows + rl;
+        if (T < tiles) {
+            const bool live = r < rows;
+            const int rc = min(r, rows - 1), i = rc / p.G, head = kvh * p.G + (rc - i * p.G), pos = base + i;
+            const int hi = p.block_mode ? base + n : pos + 1;
+            const int lo = !p.block_mode && p.window > 0 ? max(0, pos - p.window + 1) : 0;
+            const int span = hi - lo;
+            const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T * S::kTile;
+            // ---- query planes: q scale log2(e) 2^e with the row's largest value in [2^13, 2^14)
+            float down;
+            {
+                const float *src = p.q + (int64_t)(r0 + i) * p.qs + (int64_t)head * HD;
+                float a = 0.0f;
+#pragma unroll 4
+                for (int d = 0; d < HD; d += 4) {
+                    const float4 v = *reinterpret_cast<const float4 *>(src + d);
+                    const float w[4] = {v.x * p.qscale, v.y * p.qscale, v.z * p.qscale, v.w * p.qscale};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) a = finite_f(w[k]) ? fmaxf(a, fabsf(w[k])) : a;
+                }
+                const int e = min(13 - ((__float_as_int(a) >> 23) - 127), 126);
+                const float up = exp2_int(e);
+                down = exp2_int(-e);
+                uint8_t *dst = smem + T * 2 * S::kQPlane + rl * 16;
+#pragma unroll 2
+                for (int c = 0; c < HD / 8; ++c) {
+                    float w[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k += 4) {
+                        const float4 v = *reinterpret_cast<const float4 *>(src + c * 8 + k);
+                        w[k] = v.x * p.qscale * up, w[k + 1] = v.y * p.qscale * up;
+                        w[k + 2] = v.z * p.qscale * up, w[k + 3] = v.w * p.qscale * up;
+                    }
+                    uint4 h, l;
+                    split_half2(w[0], w[1], h.x, l.x);
+                    split_half2(w[2], w[3], h.y, l.y);
+                    split_half2(w[4], w[5], h.z, l.z);
+                    split_half2(w[6], w[7], h.w, l.w);
+                    *reinterpret_cast<uint4 *>(dst + c * (kPcRows * 16)) = h;
+                    *reinterpret_cast<uint4 *>(dst + S::kQPlane + c * (kPcRows * 16)) = l;
+                }
+                fence_async_smem();
+                mbar_arrive(&bars.q_full);
+            }
+            float m = -INFINITY, l = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < nst; ++j) {
+                const int st = j & 1, kb = kb0 + j * BN;
+                if (!mbar_wait_abort(&bars.k_full[st], (j >> 1) & 1, abortp) || !mbar_wait_abort(&bars.s_full[T], j & 1, abortp)) {
+                    if (lane == 0) give_up(0x51);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                bool all = true;
+#pragma unroll
+                for (int g = 0; g < BN / 16; ++g) all &= present[st][g] != 0;
+                bool masked = !__all_sync(0xffffffffu, all && kb >= lo && kb + BN <= hi);
+                // scores of 32 keys, times K's scales; what the row does not see, or is not finite, is -inf where `masked`
+                auto scores = [&](int c, float2(&y)[16]) {
+                    float v[32];
+                    tmem_ld32(trow + S::kS + c * 32, v);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float4 ks = *reinterpret_cast<const float4 *>(&kscale[st][c * 32 + k * 4]);
+                        y[2 * k] = __fmul2_rn(make_float2(v[4 * k], v[4 * k + 1]), make_float2(ks.x, ks.y));
+                        y[2 * k + 1] = __fmul2_rn(make_float2(v[4 * k + 2], v[4 * k + 3]), make_float2(ks.z, ks.w));
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const int d = kb + c * 32 + 2 * k - lo;
+                            const bool there = present[st][c * 2 + k / 8] != 0;
+                            y[k].x = there && (unsigned)d < (unsigned)span && finite_f(y[k].x) ? y[k].x : -INFINITY;
+                            y[k].y = there && (unsigned)(d + 1) < (unsigned)span && finite_f(y[k].y) ? y[k].y : -INFINITY;
+                        }
+                    }
+                };
+                // ---- pass 1: the row's maximum
+                float mx = -INFINITY;
+                float2 odd = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    float2 y[16];
+                    scores(c, y);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        mx = fmaxf(mx, fmaxf(y[k].x, y[k].y));
+                        odd = __ffma2_rn(y[k], make_float2(0.0f, 0.0f), odd);
+                    }
+                }
+                if (!masked && __any_sync(0xffffffffu, odd.x + odd.y != 0.0f)) { // NaN: a score is not finite
+                    masked = true;
+                    mx = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < CH; ++c) {
+                        float2 y[16];
+                        scores(c, y);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, fmaxf(y[k].x, y[k].y));
+                    }
+                }
+                mx *= down;
+                // ---- O follows the maximum only when that has grown by more than 2^8: until then weights exceed 1
+                const bool grow = mx > m + 8.0f || (m == -INFINITY && mx > m);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = grow ? t5_ex2(m - mx) : 1.0f; // 2^-inf = 0 where there was no maximum
+                    l *= f;
+                    if (grow) m = mx;
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < HD / 32; ++c) {
+                            float o[32];
+                            uint32_t w[32];
+                            tmem_ld32(trow + S::kO + c * 32, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * f);
+                            tmem_st32(trow + S::kO + c * 32, w);
+                        }
+                    }
+                }
+                // ---- pass 2: weights, their sum, and their three planes over the scores
+                const float mref = m == -INFINITY ? 0.0f : -m;
+                float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    float2 y[16];
+                    scores(c, y);
+                    uint32_t ph[16], pm[16], pl[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        float2 w = __ffma2_rn(y[k], make_float2(down, down), make_float2(mref, mref));
+                        w = make_float2(t5_ex2(w.x), t5_ex2(w.y));
+                        sum = __fadd2_rn(sum, w);
+                        ph[k] = __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x7632);
+                        w = __fadd2_rn(w, make_float2(-__uint_as_float(__float_as_uint(w.x) & 0xffff0000u),
+                                                      -__uint_as_float(__float_as_uint(w.y) & 0xffff0000u)));
+                        pm[k] = __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x7632);
+                        w = __fadd2_rn(w, make_float2(-__uint_as_float(__float_as_uint(w.x) & 0xffff0000u),
+                                                      -__uint_as_float(__float_as_uint(w.y) & 0xffff0000u)));
+                        pl[k] = __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x7632);
+                    }
+                    tmem_st16(trow + c * 48, ph);
+                    tmem_st16(trow + c * 48 + 16, pm);
+                    tmem_st16(trow + c * 48 + 32, pl);
+                }
+                l += sum.x + sum.y;
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&bars.p_ready[T]);
+            }
+            if (ok && nst > 0 && !mbar_wait_abort(&bars.o_full, 0, abortp)) {
+                if (lane == 0) give_up(0x52);
+                ok = false;
+            }
+            if (__all_sync(0xffffffffu, ok)) {
+                tc_fence_after();
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                float *dst = p.splits > 1 ? p.ws + (((int64_t)(r0 + i) * p.H + head) * p.splits + split) * PR
+                                          : p.out + (int64_t)(r0 + i) * p.os + (int64_t)head * HD;
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    float o[32];
+                    if (nst > 0) {
+                        tmem_ld32(trow + S::kO + c * 32, o);
+                        tc_wait_ld();
+                    }
+                    if (live) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            *reinterpret_cast<float4 *>(dst + c * 32 + k) =
+                                l > 0.0f ? make_float4(o[k] * inv, o[k + 1] * inv, o[k + 2] * inv, o[k + 3] * inv)
+                                         : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                }
+                if (live && p.splits > 1) *reinterpret_cast<float2 *>(dst + HD) = make_float2(m, l);
+            }
+        }
+    } else if (warp < 12) {
+        // ================= converters: 64 bytes (HD 32: 32) of one key's K and V each =================
+        constexpr int NP = HD == 32 ? 2 : 4; // pieces of 16 codes
+        const int ct = tid - kPcSoft, key = ct % BN, piece0 = (ct / BN) * NP;
+        auto look = [&](int j) -> int64_t { // row of this thread's key in the pool, -1: not there
+            const int k = kb0 + j * BN + key;
+            if (j >= nst || k < rr.lo || k >= rr.hi) return -1;
+            const int pi = k / p.pv.page_size, page = p.pv.page(b, pi);
+            if (page < 0) {
+                p.pv.raise(FBLT_PAGED_BAD_PAGE);
+                return -1;
+            }
+            return p.pv.row(page, kvh, k - pi * p.pv.page_size);
+        };
+        uint4 kr[NP], vr[NP];
+        float ks = 0.0f, vs = 0.0f;
+        bool here = false;
+        auto load = [&](int64_t row) { // a key that is not there: zeros
+            here = row >= 0;
+            ks = vs = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+            if (here) {
+                const uint4 *kp = reinterpret_cast<const uint4 *>(p.pv.kc + row * HD) + piece0;
+                const uint4 *vp = reinterpret_cast<const uint4 *>(p.pv.vc + row * HD) + piece0;
+#pragma unroll
+                for (int i = 0; i < NP; ++i) kr[i] = __ldg(kp + i);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) vr[i] = __ldg(vp + i);
+                ks = kv_scale<FMT>(p.pv.ke[row]);
+                vs = kv_scale<FMT>(p.pv.ve[row]);
+            }
+        };
+        load(look(0));
+        int64_t next = look(1);
+        for (int j = 0; j < nst; ++j) {
+            const int st = j & 1;
+            if (j >= 2 && !mbar_wait_abort(&bars.kv_empty[st], ((j >> 1) - 1) & 1, abortp)) {
+                if (lane == 0) give_up(0x53);
+                break;
+            }
+            uint8_t *kd = smem + S::kOffKv + st * 2 * S::kKv + key * 16, *vd = kd + S::kKv;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                uint4 x, y;
+                F::halves(kr[i].x, x.x, x.y);
+                F::halves(kr[i].y, x.z, x.w);
+                F::halves(kr[i].z, y.x, y.y);
+                F::halves(kr[i].w, y.z, y.w);
+                *reinterpret_cast<uint4 *>(kd + (piece0 + i) * 2 * (BN * 16)) = x;
+                *reinterpret_cast<uint4 *>(kd + ((piece0 + i) * 2 + 1) * (BN * 16)) = y;
+            }
+            const uint32_t vote = __ballot_sync(0xffffffffu, here);
+            if (piece0 == 0) {
+                kscale[st][key] = ks;
+                if ((lane & 15) == 0) present[st][key / 16] = ((vote >> lane) & 0xffff) != 0;
+            }
+            fence_async_smem();
+            mbar_arrive(&bars.k_full[st]);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+                uint32_t x[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float4 v = kv_values<FMT>(w[k], vs);
+                    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), c = __floats2bfloat162_rn(v.z, v.w);
+                    x[2 * k] = *reinterpret_cast<const uint32_t *>(&a);
+                    x[2 * k + 1] = *reinterpret_cast<const uint32_t *>(&c);
+                }
+                *reinterpret_cast<uint4 *>(vd + (piece0 + i) * 2 * (BN * 16)) = make_uint4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<uint4 *>(vd + ((piece0 + i) * 2 + 1) * (BN * 16)) = make_uint4(x[4], x[5], x[6], x[7]);
+            }
+            fence_async_smem();
+            mbar_arrive(&bars.v_full[st]);
+            load(next);
+            next = look(j + 2);
+        }
+    } else if (lane == 0) {
+        // ================= issuer =================
+        constexpr uint32_t kIdS = pc_idesc(BN, false, false), kIdO = pc_idesc(HD, true, true);
+        // S = Q K^T: a 16-deep product reads two 8-column core matrices, BN (128) rows apart
+        auto issue_s = [&](int T, int st) {
+            const uint32_t q = sbase + T * 2 * S::kQPlane, k = sbase + S::kOffKv + st * 2 * S::kKv, d = tmem + T * S::kTile + S::kS;
+#pragma unroll
+            for (int pl = 1; pl >= 0; --pl)
+#pragma unroll
+                for (int s = 0; s < HD / 16; ++s)
+                    mma_f16_ss(d, t5_desc(q + pl * S::kQPlane + s * 2 * (kPcRows * 16), kPcRows * 16, 128),
+                               t5_desc(k + s * 2 * (BN * 16), BN * 16, 128), kIdS, pl == 0 || s > 0);
+            tc_commit(&bars.s_full[T]);
+        };
+        bool ok = mbar_wait_abort(&bars.q_full, 0, abortp);
+        if (ok && nst > 0) {
+            ok = mbar_wait_abort(&bars.k_full[0], 0, abortp);
+            if (ok) {
+                tc_fence_after();
+                for (int T = 0; T < tiles; ++T) issue_s(T, 0);
+            }
+            for (int j = 0; j < nst && ok; ++j) {
+                const int st = j & 1;
+                for (int T = 0; T < tiles; ++T) {
+                    ok = mbar_wait_abort(&bars.p_ready[T], j & 1, abortp) && (T > 0 || mbar_wait_abort(&bars.v_full[st], (j >> 1) & 1, abortp));
+                    if (!ok) break;
+                    tc_fence_after();
+                    // O += P V: 16 keys are two 8-row core matrices of V, 128 bytes apart; 8 columns of O the next BN rows on
+                    const uint32_t v = sbase + S::kOffKv + st * 2 * S::kKv + S::kKv, a = tmem + T * S::kTile, d = a + S::kO;
+#pragma unroll
+                    for (int pl = 2; pl >= 0; --pl)
+#pragma unroll
+                        for (int s = 0; s < BN / 16; ++s)
+                            mma_f16_ts(d, a + (s >> 1) * 48 + pl * 16 + (s & 1) * 8, t5_desc(v + s * 256, 128, BN * 16), kIdO,
+                                       j > 0 || pl < 2 || s > 0);
+                    if (T == tiles - 1) tc_commit(&bars.kv_empty[st]);
+                    if (j + 1 < nst) {
+                        if (T == 0) {
+                            ok = mbar_wait_abort(&bars.k_full[st ^ 1], ((j + 1) >> 1) & 1, abortp);
+                            if (!ok) break;
+                            tc_fence_after();
+                        }
+                        issue_s(T, st ^ 1);
+                    }
+                }
+            }
+            if (ok) tc_commit(&bars.o_full);
+        }
+        if (!ok) give_up(0x54);
+        tc_commit(&bars.fin); // whatever was issued has completed before the TMEM is given back
+        mbar_wait(&bars.fin, 0);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+template <int HD, int FMT>
+static int launch_chunk_t(const PagedAttnParams &p, cudaStream_t s) {
+    FBLT_CUDA_TRY(cudaFuncSetAttribute(paged_chunk_kernel<HD, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PcShape<HD>::kSmem));
+    const dim3 grid((unsigned)p.pv.kvh, (unsigned)p.splits, (unsigned)(p.batch * p.row_tiles));
+    paged_chunk_kernel<HD, FMT><<<grid, kPcThreads, PcShape<HD>::kSmem, s>>>(p);
+    count_launch();
+    return check_launch("paged_chunk_kernel");
+}
+
+int launch_paged_chunk(const PagedAttnParams &p, int hd, bool e4, cudaStream_t s) {
+    switch (hd) {
+    case 32: return e4 ? launch_chunk_t<32, FBLT_KV_E4M3>(p, s) : launch_chunk_t<32, FBLT_KV_INT8>(p, s);
+    case 64: return e4 ? launch_chunk_t<64, FBLT_KV_E4M3>(p, s) : launch_chunk_t<64, FBLT_KV_INT8>(p, s);
+    default: return e4 ? launch_chunk_t<128, FBLT_KV_E4M3>(p, s) : launch_chunk_t<128, FBLT_KV_INT8>(p, s);
+    }
+}
+
+int chunk_take_error() {
+    unsigned int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_chunk_error, sizeof(v)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(g_chunk_error, &zero, sizeof(zero));
+    return (int)v;
+}
+
+} // namespace fblt
