@@ -22,7 +22,7 @@
 
 namespace fblt {
 
-constexpr int kPcThreads = 416, kPcSoft = 256, kPcConv = 128; // + the issuer's warp
+constexpr int kPcThreads = 512, kPcSoft = 256, kPcConv = 128; // + the issuer's warpgroup
 constexpr int kPcRows = 128;
 
 __device__ unsigned int g_chunk_error; // 0 = ok; otherwise (code << 24) | blockIdx.x of the first CTA that gave up
@@ -54,6 +54,15 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
                  : "memory");
 }
 
+// One lane of a converged warp. The compiler knows such a branch to be the work of one thread of a uniform warp, so the
+// descriptors of the products below stay in uniform registers; behind `lane == 0` each product first moves its operands
+// there, which took the issuer about 90 cycles an MMA.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 struct PcBars {
     uint64_t q_full, k_full[2], v_full[2], kv_empty[2], s_full[2], p_ready[2], o_full, fin;
 };
@@ -71,7 +80,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
     __shared__ int s_abort;
     const volatile int *abortp = &s_abort;
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int kvh = blockIdx.x, split = blockIdx.y, b = blockIdx.z / p.row_tiles;
     const int rt = p.row_tiles - 1 - (blockIdx.z - b * p.row_tiles); // later rows see more keys: they go first
     int r0, n, base;
@@ -114,7 +123,9 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
 
+    // Registers follow the roles: 256 x 200 + 128 x 72 + 128 x 40 = the 512 x 128 of the launch.
     if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         // ================= softmax: this thread's query row =================
         const int T = warp >> 2, rl = (warp & 3) * 32 + lane, r = row0 + T * kPcRows + rl;
         if (T < tiles) {
@@ -173,51 +184,46 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 bool all = true;
 #pragma unroll
                 for (int g = 0; g < BN / 16; ++g) all &= present[st][g] != 0;
-                bool masked = !__all_sync(0xffffffffu, all && kb >= lo && kb + BN <= hi);
-                // scores of 32 keys, times K's scales; what the row does not see, or is not finite, is -inf where `masked`
-                auto scores = [&](int c, float2(&y)[16]) {
-                    float v[32];
-                    tmem_ld32(trow + S::kS + c * 32, v);
+                const bool masked = !__all_sync(0xffffffffu, all && kb >= lo && kb + BN <= hi);
+                // ---- the row's scores times K's scales, all in registers, and their maximum; what the row does not see, or
+                // is not finite, is -inf where `masked`
+                float2 y[CH][16];
+                {
+                    float v[CH][32];
+#pragma unroll
+                    for (int c = 0; c < CH; ++c) tmem_ld32(trow + S::kS + c * 32, v[c]);
                     tc_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float4 ks = *reinterpret_cast<const float4 *>(&kscale[st][c * 32 + k * 4]);
-                        y[2 * k] = __fmul2_rn(make_float2(v[4 * k], v[4 * k + 1]), make_float2(ks.x, ks.y));
-                        y[2 * k + 1] = __fmul2_rn(make_float2(v[4 * k + 2], v[4 * k + 3]), make_float2(ks.z, ks.w));
+                    for (int c = 0; c < CH; ++c)
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) y[c][k] = make_float2(v[c][2 * k], v[c][2 * k + 1]);
+                }
+                float mx = -INFINITY;
+                float2 odd = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) {
+                        const float4 ks = *reinterpret_cast<const float4 *>(&kscale[st][c * 32 + k * 2]);
+                        y[c][k] = __fmul2_rn(y[c][k], make_float2(ks.x, ks.y));
+                        y[c][k + 1] = __fmul2_rn(y[c][k + 1], make_float2(ks.z, ks.w));
+                        mx = fmaxf(fmaxf(mx, y[c][k].x), y[c][k].y);
+                        mx = fmaxf(fmaxf(mx, y[c][k + 1].x), y[c][k + 1].y);
+                        odd = __ffma2_rn(y[c][k], make_float2(0.0f, 0.0f), odd);
+                        odd = __ffma2_rn(y[c][k + 1], make_float2(0.0f, 0.0f), odd);
                     }
-                    if (masked) {
+                if (masked || __any_sync(0xffffffffu, odd.x + odd.y != 0.0f)) { // NaN: a score is not finite
+                    mx = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < CH; ++c)
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
                             const int d = kb + c * 32 + 2 * k - lo;
                             const bool there = present[st][c * 2 + k / 8] != 0;
-                            y[k].x = there && (unsigned)d < (unsigned)span && finite_f(y[k].x) ? y[k].x : -INFINITY;
-                            y[k].y = there && (unsigned)(d + 1) < (unsigned)span && finite_f(y[k].y) ? y[k].y : -INFINITY;
+                            y[c][k].x = there && (unsigned)d < (unsigned)span && finite_f(y[c][k].x) ? y[c][k].x : -INFINITY;
+                            y[c][k].y = there && (unsigned)(d + 1) < (unsigned)span && finite_f(y[c][k].y) ? y[c][k].y : -INFINITY;
+                            mx = fmaxf(fmaxf(mx, y[c][k].x), y[c][k].y);
                         }
-                    }
-                };
-                // ---- pass 1: the row's maximum
-                float mx = -INFINITY;
-                float2 odd = make_float2(0.0f, 0.0f);
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    float2 y[16];
-                    scores(c, y);
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        mx = fmaxf(mx, fmaxf(y[k].x, y[k].y));
-                        odd = __ffma2_rn(y[k], make_float2(0.0f, 0.0f), odd);
-                    }
-                }
-                if (!masked && __any_sync(0xffffffffu, odd.x + odd.y != 0.0f)) { // NaN: a score is not finite
-                    masked = true;
-                    mx = -INFINITY;
-#pragma unroll 1
-                    for (int c = 0; c < CH; ++c) {
-                        float2 y[16];
-                        scores(c, y);
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, fmaxf(y[k].x, y[k].y));
-                    }
                 }
                 mx *= down;
                 // ---- O follows the maximum only when that has grown by more than 2^8: until then weights exceed 1
@@ -239,17 +245,15 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         }
                     }
                 }
-                // ---- pass 2: weights, their sum, and their three planes over the scores
+                // ---- weights, their sum, and their three planes over the scores
                 const float mref = m == -INFINITY ? 0.0f : -m;
                 float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
-                    float2 y[16];
-                    scores(c, y);
                     uint32_t ph[16], pm[16], pl[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        float2 w = __ffma2_rn(y[k], make_float2(down, down), make_float2(mref, mref));
+                        float2 w = __ffma2_rn(y[c][k], make_float2(down, down), make_float2(mref, mref));
                         w = make_float2(t5_ex2(w.x), t5_ex2(w.y));
                         sum = __fadd2_rn(sum, w);
                         ph[k] = __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x7632);
@@ -297,6 +301,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             }
         }
     } else if (warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         // ================= converters: 64 bytes (HD 32: 32) of one key's K and V each =================
         constexpr int NP = HD == 32 ? 2 : 4; // pieces of 16 codes
         const int ct = tid - kPcSoft, key = ct % BN, piece0 = (ct / BN) * NP;
@@ -374,57 +379,70 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             load(next);
             next = look(j + 2);
         }
-    } else if (lane == 0) {
-        // ================= issuer =================
-        constexpr uint32_t kIdS = pc_idesc(BN, false, false), kIdO = pc_idesc(HD, true, true);
-        // S = Q K^T: a 16-deep product reads two 8-column core matrices, BN (128) rows apart
-        auto issue_s = [&](int T, int st) {
-            const uint32_t q = sbase + T * 2 * S::kQPlane, k = sbase + S::kOffKv + st * 2 * S::kKv, d = tmem + T * S::kTile + S::kS;
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 12) {
+            // ================= issuer (the warp goes along, one lane issues) =================
+            constexpr uint32_t kIdS = pc_idesc(BN, false, false), kIdO = pc_idesc(HD, true, true);
+            // S = Q K^T: a 16-deep product reads two 8-column core matrices, BN (128) rows apart
+            auto issue_s = [&](int T, int st) {
+                const uint32_t q = sbase + T * 2 * S::kQPlane, k = sbase + S::kOffKv + st * 2 * S::kKv, d = tmem + T * S::kTile + S::kS;
+                if (elect_one()) {
 #pragma unroll
-            for (int pl = 1; pl >= 0; --pl)
+                    for (int pl = 1; pl >= 0; --pl)
 #pragma unroll
-                for (int s = 0; s < HD / 16; ++s)
-                    mma_f16_ss(d, t5_desc(q + pl * S::kQPlane + s * 2 * (kPcRows * 16), kPcRows * 16, 128),
-                               t5_desc(k + s * 2 * (BN * 16), BN * 16, 128), kIdS, pl == 0 || s > 0);
-            tc_commit(&bars.s_full[T]);
-        };
-        bool ok = mbar_wait_abort(&bars.q_full, 0, abortp);
-        if (ok && nst > 0) {
-            ok = mbar_wait_abort(&bars.k_full[0], 0, abortp);
-            if (ok) {
-                tc_fence_after();
-                for (int T = 0; T < tiles; ++T) issue_s(T, 0);
-            }
-            for (int j = 0; j < nst && ok; ++j) {
-                const int st = j & 1;
-                for (int T = 0; T < tiles; ++T) {
-                    ok = mbar_wait_abort(&bars.p_ready[T], j & 1, abortp) && (T > 0 || mbar_wait_abort(&bars.v_full[st], (j >> 1) & 1, abortp));
-                    if (!ok) break;
+                        for (int s = 0; s < HD / 16; ++s)
+                            mma_f16_ss(d, t5_desc(q + pl * S::kQPlane + s * 2 * (kPcRows * 16), kPcRows * 16, 128),
+                                       t5_desc(k + s * 2 * (BN * 16), BN * 16, 128), kIdS, pl == 0 || s > 0);
+                    tc_commit(&bars.s_full[T]);
+                }
+                __syncwarp();
+            };
+            bool ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.q_full, 0, abortp));
+            if (ok && nst > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.k_full[0], 0, abortp));
+                if (ok) {
                     tc_fence_after();
-                    // O += P V: 16 keys are two 8-row core matrices of V, 128 bytes apart; 8 columns of O the next BN rows on
-                    const uint32_t v = sbase + S::kOffKv + st * 2 * S::kKv + S::kKv, a = tmem + T * S::kTile, d = a + S::kO;
+                    for (int T = 0; T < tiles; ++T) issue_s(T, 0);
+                }
+                for (int j = 0; j < nst && ok; ++j) {
+                    const int st = j & 1;
+                    for (int T = 0; T < tiles; ++T) {
+                        ok = mbar_wait_abort(&bars.p_ready[T], j & 1, abortp) &&
+                             (T > 0 || mbar_wait_abort(&bars.v_full[st], (j >> 1) & 1, abortp));
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+                        // O += P V: 16 keys are two 8-row core matrices of V, 128 bytes apart; 8 columns of O the next BN rows on
+                        const uint32_t v = sbase + S::kOffKv + st * 2 * S::kKv + S::kKv, a = tmem + T * S::kTile, d = a + S::kO;
+                        if (elect_one()) {
 #pragma unroll
-                    for (int pl = 2; pl >= 0; --pl)
+                            for (int pl = 2; pl >= 0; --pl)
 #pragma unroll
-                        for (int s = 0; s < BN / 16; ++s)
-                            mma_f16_ts(d, a + (s >> 1) * 48 + pl * 16 + (s & 1) * 8, t5_desc(v + s * 256, 128, BN * 16), kIdO,
-                                       j > 0 || pl < 2 || s > 0);
-                    if (T == tiles - 1) tc_commit(&bars.kv_empty[st]);
-                    if (j + 1 < nst) {
-                        if (T == 0) {
-                            ok = mbar_wait_abort(&bars.k_full[st ^ 1], ((j + 1) >> 1) & 1, abortp);
-                            if (!ok) break;
-                            tc_fence_after();
+                                for (int s = 0; s < BN / 16; ++s)
+                                    mma_f16_ts(d, a + (s >> 1) * 48 + pl * 16 + (s & 1) * 8, t5_desc(v + s * 256, 128, BN * 16), kIdO,
+                                               j > 0 || pl < 2 || s > 0);
+                            if (T == tiles - 1) tc_commit(&bars.kv_empty[st]);
+                            if (j == nst - 1 && T == tiles - 1) tc_commit(&bars.o_full);
                         }
-                        issue_s(T, st ^ 1);
+                        __syncwarp();
+                        if (j + 1 < nst) {
+                            if (T == 0) {
+                                ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.k_full[st ^ 1], ((j + 1) >> 1) & 1, abortp));
+                                if (!ok) break;
+                                tc_fence_after();
+                            }
+                            issue_s(T, st ^ 1);
+                        }
                     }
                 }
             }
-            if (ok) tc_commit(&bars.o_full);
+            if (!ok && lane == 0) give_up(0x54);
+            // whatever was issued has completed before the TMEM is given back
+            if (elect_one()) tc_commit(&bars.fin);
+            __syncwarp();
+            mbar_wait(&bars.fin, 0);
         }
-        if (!ok) give_up(0x54);
-        tc_commit(&bars.fin); // whatever was issued has completed before the TMEM is given back
-        mbar_wait(&bars.fin, 0);
     }
     tc_fence_before();
     __syncthreads();
