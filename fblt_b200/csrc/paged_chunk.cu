@@ -63,6 +63,14 @@ __device__ __forceinline__ bool elect_one() {
     return one != 0;
 }
 
+// The nearest bf16 pair of w (first value in the low half), and what is left of w.
+__device__ __forceinline__ uint32_t bf16_plane(float2 &w) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(w.x, w.y);
+    const uint32_t b = *reinterpret_cast<const uint32_t *>(&h);
+    w = __fadd2_rn(w, make_float2(-__uint_as_float(b << 16), -__uint_as_float(b & 0xffff0000u)));
+    return b;
+}
+
 struct PcBars {
     uint64_t q_full, k_full[2], v_full[2], kv_empty[2], s_full[2], p_ready[2], o_full, fin;
 };
@@ -137,6 +145,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T * S::kTile;
             // ---- query planes: q scale log2(e) 2^e with the row's largest value in [2^13, 2^14)
             float down;
+            bool qbad = false; // a query value that is not finite
             {
                 const float *src = p.q + (int64_t)(r0 + i) * p.qs + (int64_t)head * HD;
                 float a = 0.0f;
@@ -145,7 +154,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                     const float4 v = *reinterpret_cast<const float4 *>(src + d);
                     const float w[4] = {v.x * p.qscale, v.y * p.qscale, v.z * p.qscale, v.w * p.qscale};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) a = finite_f(w[k]) ? fmaxf(a, fabsf(w[k])) : a;
+                    for (int k = 0; k < 4; ++k) {
+                        if (finite_f(w[k])) a = fmaxf(a, fabsf(w[k]));
+                        else qbad = true;
+                    }
                 }
                 const int e = min(13 - ((__float_as_int(a) >> 23) - 127), 126);
                 const float up = exp2_int(e);
@@ -185,8 +197,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
 #pragma unroll
                 for (int g = 0; g < BN / 16; ++g) all &= present[st][g] != 0;
                 const bool masked = !__all_sync(0xffffffffu, all && kb >= lo && kb + BN <= hi);
-                // ---- the row's scores times K's scales, all in registers, and their maximum; what the row does not see, or
-                // is not finite, is -inf where `masked`
+                // ---- the row's scores times K's scales, all in registers, and their maximum
                 float2 y[CH][16];
                 {
                     float v[CH][32];
@@ -198,8 +209,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
 #pragma unroll
                         for (int k = 0; k < 16; ++k) y[c][k] = make_float2(v[c][2 * k], v[c][2 * k + 1]);
                 }
-                float mx = -INFINITY;
-                float2 odd = make_float2(0.0f, 0.0f);
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -207,12 +217,13 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         const float4 ks = *reinterpret_cast<const float4 *>(&kscale[st][c * 32 + k * 2]);
                         y[c][k] = __fmul2_rn(y[c][k], make_float2(ks.x, ks.y));
                         y[c][k + 1] = __fmul2_rn(y[c][k + 1], make_float2(ks.z, ks.w));
-                        mx = fmaxf(fmaxf(mx, y[c][k].x), y[c][k].y);
-                        mx = fmaxf(fmaxf(mx, y[c][k + 1].x), y[c][k + 1].y);
-                        odd = __ffma2_rn(y[c][k], make_float2(0.0f, 0.0f), odd);
-                        odd = __ffma2_rn(y[c][k + 1], make_float2(0.0f, 0.0f), odd);
+                        top[k & 2] = fmaxf(fmaxf(top[k & 2], y[c][k].x), y[c][k].y);
+                        top[(k & 2) + 1] = fmaxf(fmaxf(top[(k & 2) + 1], y[c][k + 1].x), y[c][k + 1].y);
                     }
-                if (masked || __any_sync(0xffffffffu, odd.x + odd.y != 0.0f)) { // NaN: a score is not finite
+                float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * down;
+                // Sums of 8-bit codes times query planes below 2^14 stay far from overflow, so a score is not finite only
+                // where the query row is not, or where the scales took it past fp32's range (-inf weighs 0 by itself).
+                if (__any_sync(0xffffffffu, masked || qbad || !(mx < INFINITY))) {
                     mx = -INFINITY;
 #pragma unroll
                     for (int c = 0; c < CH; ++c)
@@ -220,12 +231,12 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         for (int k = 0; k < 16; ++k) {
                             const int d = kb + c * 32 + 2 * k - lo;
                             const bool there = present[st][c * 2 + k / 8] != 0;
-                            y[c][k].x = there && (unsigned)d < (unsigned)span && finite_f(y[c][k].x) ? y[c][k].x : -INFINITY;
-                            y[c][k].y = there && (unsigned)(d + 1) < (unsigned)span && finite_f(y[c][k].y) ? y[c][k].y : -INFINITY;
+                            y[c][k].x = there && (unsigned)d < (unsigned)span && finite_f(y[c][k].x * down) ? y[c][k].x : -INFINITY;
+                            y[c][k].y = there && (unsigned)(d + 1) < (unsigned)span && finite_f(y[c][k].y * down) ? y[c][k].y : -INFINITY;
                             mx = fmaxf(fmaxf(mx, y[c][k].x), y[c][k].y);
                         }
+                    mx *= down;
                 }
-                mx *= down;
                 // ---- O follows the maximum only when that has grown by more than 2^8: until then weights exceed 1
                 const bool grow = mx > m + 8.0f || (m == -INFINITY && mx > m);
                 if (__any_sync(0xffffffffu, grow)) {
@@ -247,7 +258,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 }
                 // ---- weights, their sum, and their three planes over the scores
                 const float mref = m == -INFINITY ? 0.0f : -m;
-                float2 sum = make_float2(0.0f, 0.0f);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
                     uint32_t ph[16], pm[16], pl[16];
@@ -255,20 +266,16 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                     for (int k = 0; k < 16; ++k) {
                         float2 w = __ffma2_rn(y[c][k], make_float2(down, down), make_float2(mref, mref));
                         w = make_float2(t5_ex2(w.x), t5_ex2(w.y));
-                        sum = __fadd2_rn(sum, w);
-                        ph[k] = __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x7632);
-                        w = __fadd2_rn(w, make_float2(-__uint_as_float(__float_as_uint(w.x) & 0xffff0000u),
-                                                      -__uint_as_float(__float_as_uint(w.y) & 0xffff0000u)));
-                        pm[k] = __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x7632);
-                        w = __fadd2_rn(w, make_float2(-__uint_as_float(__float_as_uint(w.x) & 0xffff0000u),
-                                                      -__uint_as_float(__float_as_uint(w.y) & 0xffff0000u)));
-                        pl[k] = __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x7632);
+                        sum[k & 1] = __fadd2_rn(sum[k & 1], w);
+                        ph[k] = bf16_plane(w);
+                        pm[k] = bf16_plane(w);
+                        pl[k] = bf16_plane(w);
                     }
                     tmem_st16(trow + c * 48, ph);
                     tmem_st16(trow + c * 48 + 16, pm);
                     tmem_st16(trow + c * 48 + 32, pl);
                 }
-                l += sum.x + sum.y;
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tc_wait_st();
                 tc_fence_before();
                 mbar_arrive(&bars.p_ready[T]);
