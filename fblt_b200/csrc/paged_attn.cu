@@ -29,6 +29,9 @@ constexpr int kPsThreads = 160;
 // A row's weights times the scales of V, p 2^ev, are put into halves in units of 2^(R - kPsHead), R within four of the
 // largest exponent that p 2^ev has had (R follows the row's maximum when that moves): at most 2^(kPsHead + 5), and what
 // is 2^-24 of the largest still has 11 bits, however unequal the rows of V are.
+// The tensor cores cut every sum off below 24 bits, a pull towards zero of about 2e-8 a product (5e-6 over 4800 keys):
+// after so many keys what they hold is added, rounded, to sums of its own.
+constexpr int kPsFold = 256;
 constexpr int kPsHead = 10, kPsNoUnit = -(1 << 20);
 
 template <int HD>
@@ -185,7 +188,9 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");
 
-        float m[RB], l[RB], c[RB], o[RB][NB][4];
+        float m[RB], l[RB], c[RB];
+        float o[RB][NB][4]; // the tensor cores' sums, a plane in each half
+        float2 sum[RB][NB]; // columns 2t and 2t + 1 of every block: what was folded
         int lo[RB], span[RB], R[RB]; // o holds sums of p v in units of 2^R
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
@@ -199,8 +204,22 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
             R[rb] = kPsNoUnit;
             c[rb] = crow[ri];
 #pragma unroll
-            for (int j = 0; j < NB; ++j) o[rb][j][0] = o[rb][j][1] = o[rb][j][2] = o[rb][j][3] = 0.0f;
+            for (int j = 0; j < NB; ++j) {
+                o[rb][j][0] = o[rb][j][1] = o[rb][j][2] = o[rb][j][3] = 0.0f;
+                sum[rb][j] = make_float2(0.0f, 0.0f);
+            }
         }
+        int held = 0; // stages in o
+        auto fold = [&]() {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    sum[rb][j] = __fadd2_rn(sum[rb][j], __fadd2_rn(make_float2(o[rb][j][0], o[rb][j][1]), make_float2(o[rb][j][2], o[rb][j][3])));
+                    o[rb][j][0] = o[rb][j][1] = o[rb][j][2] = o[rb][j][3] = 0.0f;
+                }
+            held = 0;
+        };
         const uint4 *myq = sq + wr * RB * KS * 32 + lane;
         float(&kscale)[S::kKeys] = scale[warp][0], (&vscale)[S::kKeys] = scale[warp][1];
         for (int st = wk; st < nst; st += WK) { // a stage belongs to the WR warps of one key share
@@ -343,16 +362,17 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
                         R[rb] += (int)down;
                         m[rb] = mn[rb];
 #pragma unroll
-                        for (int j = 0; j < NB; ++j)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) o[rb][j][k] *= f;
+                        for (int j = 0; j < NB; ++j) {
+                            o[rb][j][0] *= f, o[rb][j][1] *= f, o[rb][j][2] *= f, o[rb][j][3] *= f;
+                            sum[rb][j] = __fmul2_rn(sum[rb][j], make_float2(f, f));
+                        }
                     }
                 }
                 float top[RB]; // the largest p 2^(ev - et)
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
                     const float mref = m[rb] == -INFINITY ? 0.0f : -m[rb];
-                    float2 sum = make_float2(0.0f, 0.0f);
+                    float2 add = make_float2(0.0f, 0.0f);
                     top[rb] = 0.0f;
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
@@ -362,12 +382,12 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
                             float2 &y = x[rb][u][nb];
                             y = __fadd2_rn(y, make_float2(mref, mref));
                             y = make_float2(t5_ex2(y.x), t5_ex2(y.y));
-                            sum = __fadd2_rn(sum, y);
+                            add = __fadd2_rn(add, y);
                             y = __fmul2_rn(y, nb ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y));
                             top[rb] = fmaxf(top[rb], fmaxf(y.x, y.y));
                         }
                     }
-                    l[rb] += sum.x + sum.y;
+                    l[rb] += add.x + add.y;
                 }
                 bool raise = false;
 #pragma unroll
@@ -381,9 +401,10 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
                         const float f = R[rb] - Rn < -126 ? 0.0f : exp2_int(R[rb] - Rn);
                         R[rb] = Rn;
 #pragma unroll
-                        for (int j = 0; j < NB; ++j)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) o[rb][j][k] *= f;
+                        for (int j = 0; j < NB; ++j) {
+                            o[rb][j][0] *= f, o[rb][j][1] *= f, o[rb][j][2] *= f, o[rb][j][3] *= f;
+                            sum[rb][j] = __fmul2_rn(sum[rb][j], make_float2(f, f));
+                        }
                     }
                 }
                 uint4 pa[RB][U];
@@ -428,9 +449,11 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
                     }
                 }
             }
+            if (++held == kPsFold / S::kKeys) fold();
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[slot]);
         }
+        fold();
         // ---- the warps' shares of the keys meet in shared memory (every copy has landed: the ring is free)
         asm volatile("bar.sync 1, 128;" ::: "memory");
         float *part = reinterpret_cast<float *>(smem);
@@ -450,10 +473,10 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
 #pragma unroll
                 for (int j = 0; j < NB; j += 4) {
                     float4 v;
-                    v.x = (o[rb][j][h] + o[rb][j][2 + h]) * kDown * unit;
-                    v.y = (o[rb][j + 1][h] + o[rb][j + 1][2 + h]) * kDown * unit;
-                    v.z = (o[rb][j + 2][h] + o[rb][j + 2][2 + h]) * kDown * unit;
-                    v.w = (o[rb][j + 3][h] + o[rb][j + 3][2 + h]) * kDown * unit;
+                    v.x = (h ? sum[rb][j].y : sum[rb][j].x) * kDown * unit;
+                    v.y = (h ? sum[rb][j + 1].y : sum[rb][j + 1].x) * kDown * unit;
+                    v.z = (h ? sum[rb][j + 2].y : sum[rb][j + 2].x) * kDown * unit;
+                    v.w = (h ? sum[rb][j + 3].y : sum[rb][j + 3].x) * kDown * unit;
                     *reinterpret_cast<float4 *>(part + row * PR + (2 * t + h) * NB + j) = v;
                 }
         }

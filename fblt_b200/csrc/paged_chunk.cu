@@ -2,21 +2,21 @@
 // kv head: prompts taken in chunks).
 //
 // CTA = (sequence, kv head, key range, 256 query rows as two tiles of 128), one per SM; K and V tiles of BN keys are
-// converted once for both query tiles. Products in fp32 class from 16-bit operands:
-//   S = Q K^T    an 8-bit code is a half as it stands, so K is one fp16 plane; Q (scaled by its row's power of two) is
-//                two, 22 bits. K's exponents multiply the columns of S when the softmax reads them.
-//   O += P V     code 2^e is a bf16 value, so V is one bf16 plane with its scale in it; P is three, cut off bit by bit
-//                (8 + 8 + 8 = all of fp32's 24), which needs no range of its own however unequal the rows of V are.
-// Two MMAs for every Q K^T, three for every P V: 5/2 of the products that bf16 attention would issue.
+// converted once for both query tiles. An 8-bit code is a half as it stands, so K and V are ONE fp16 plane each and the
+// 22 bits of fp32 class come from two planes of Q and of P: two MMAs where 16-bit attention has one.
+//   S = Q K^T    Q is scaled by its row's power of two; K's exponents multiply the columns of S as the softmax reads them.
+//   O += P V     V's exponents within a tile go into its halves where they lie within 2^4 of each other (rows of one
+//                head: nearly always), relative to the tile's largest, 2^et; into P's columns otherwise. O is in units of
+//                2^R, a row's own R, which follows the largest p 2^et the row has had, so that P's halves keep the 22
+//                bits of what counts; et, R and the maximum meet in the exponent of 2^x and cost nothing per score.
 //
-// Roles (13 warps), which meet on mbarriers only; every wait is bounded:
+// Roles (13 warps at work), which meet on mbarriers only; every wait is bounded:
 //   softmax (2 x 4 warps)  one thread per query row (TMEM lane): running maximum and sum, P back to TMEM over the scores
-//                          it came from (32 keys: 32 columns of S become 48 of P; block c starts at column 48 c, S lies
-//                          at the end of the region, so a block never covers scores that have not been read). O stays in
-//                          TMEM and is rescaled only where a maximum has grown by more than 2^8.
-//   converters (4 warps)   pages -> registers (one tile ahead) -> 16-bit operands in shared memory, in 8-row x 16-byte
-//                          core matrices (K read K-major, V MN-major: the same bytes, no transposition)
-//   issuer (1 thread)      while one query tile's softmax runs, the tensor cores have the other tile's products
+//                          it came from. O stays in TMEM and is rescaled only where a maximum has grown by more than 2^4.
+//   converters (4 warps)   pages -> registers (one tile ahead) -> halves in shared memory, in 8-row x 16-byte core
+//                          matrices (K read K-major, V MN-major: the same bytes, no transposition)
+//   issuer (1 warp)        while one query tile's softmax runs, the tensor cores have the other tile's products
+// Q's planes are TMEM operands (head_dim 128: the first one; the other stays in shared memory).
 #include "paged.cuh"
 #include "tc5.cuh"
 
@@ -30,15 +30,23 @@ __device__ unsigned int g_chunk_error; // 0 = ok; otherwise (code << 24) | block
 template <int HD>
 struct PcShape {
     static constexpr int BN = HD == 128 ? 64 : 128; // keys of a tile: S, P and O of two query tiles fit 512 columns
-    static constexpr int kQPlane = kPcRows * HD * 2, kKv = BN * HD * 2;
-    static constexpr int kOffKv = 4 * kQPlane; // two tiles, two planes of Q
-    static constexpr int kSmem = kOffKv + 4 * kKv;
-    static constexpr int kP = BN * 3 / 2, kS = kP - BN, kO = kP, kTile = 256; // TMEM columns of a query tile
+    static constexpr int kQPlane = HD == 128 ? kPcRows * HD * 2 : 0, kKv = BN * HD * 2;
+    static constexpr int kOffKv = 2 * kQPlane; // head_dim 128: the second plane of Q of both tiles
+    static constexpr int kOffSum = kOffKv + 4 * kKv; // head_dim 32, 64: folded sums, see the softmax
+    static constexpr int kSmem = kOffSum + (HD == 128 ? 0 : 2 * kPcRows * HD * 4);
+    // TMEM columns of a query tile: S / P, O; behind both tiles the planes of Q
+    static constexpr int kO = BN, kTile = BN + HD, kQCols = HD / 2, kQTile = HD == 128 ? kQCols : 2 * kQCols, kQ = 2 * kTile;
+    static_assert(kQ + 2 * kQTile <= 512, "TMEM");
 };
+constexpr int kPcHead = 10;   // P in units of 2^(R - kPcHead), R at most 4 below the largest exponent: halves up to 2^15
+constexpr int kPcFold = 512;  // keys whose products the tensor cores sum: they cut every sum off below 24 bits, which pulls
+                              // O towards zero by about 2e-8 an MMA (9e-6 over 31 k keys in eight pieces; 512 keys are 64
+                              // MMAs); what they have is then added, rounded, to sums of its own
+constexpr int kPcNarrow = 4;  // V's exponents go into its halves where they lie this close
 
-// fp16 / bf16 operands, fp32 accumulate; B K-major or MN-major
-__host__ __device__ constexpr uint32_t pc_idesc(int n, bool bf16, bool mn_major) {
-    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+// fp16 operands, fp32 accumulate; B K-major or MN-major
+__host__ __device__ constexpr uint32_t pc_idesc(int n, bool mn_major) {
+    return (1u << 4) | ((mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(kPcRows >> 4) << 24);
 }
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -63,26 +71,30 @@ __device__ __forceinline__ bool elect_one() {
     return one != 0;
 }
 
-// The nearest bf16 pair of w (first value in the low half), and what is left of w.
-__device__ __forceinline__ uint32_t bf16_plane(float2 &w) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(w.x, w.y);
-    const uint32_t b = *reinterpret_cast<const uint32_t *>(&h);
-    w = __fadd2_rn(w, make_float2(-__uint_as_float(b << 16), -__uint_as_float(b & 0xffff0000u)));
-    return b;
+// Barrier of the four converter warps that tells all of them whether any has failed.
+__device__ __forceinline__ bool converters_or(bool x) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any)
+                 : "r"((uint32_t)x)
+                 : "memory");
+    return any != 0;
 }
 
 struct PcBars {
-    uint64_t q_full, k_full[2], v_full[2], kv_empty[2], s_full[2], p_ready[2], o_full, fin;
+    uint64_t q_full, kv_full[2], kv_empty[2], s_full[2], p_ready[2], o_full, fin;
 };
 
 template <int HD, int FMT>
 __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedAttnParams p) {
     using F = KvFormat<FMT>;
     using S = PcShape<HD>;
-    constexpr int BN = S::BN, CH = BN / 32, PR = HD + 4;
+    constexpr int BN = S::BN, CH = BN / 32, PR = HD + 4, kFold = kPcFold / BN;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ PcBars bars;
-    __shared__ __align__(16) float kscale[2][BN];
+    __shared__ __align__(16) float kscale[2][BN], vscale[2][BN];
+    __shared__ int vtop[2][2]; // largest exponent of the tile's V, and whether they are too far apart for its halves
+    __shared__ int vrange[2][4][2];
     __shared__ __align__(8) uint8_t present[2][8]; // groups of 16 keys whose page exists and that the CTA reads
     __shared__ uint32_t tmem_slot;
     __shared__ int s_abort;
@@ -111,8 +123,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
     if (tid == 0) {
         mbar_init(&bars.q_full, tiles * kPcRows);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&bars.k_full[i], kPcConv);
-            mbar_init(&bars.v_full[i], kPcConv);
+            mbar_init(&bars.kv_full[i], kPcConv);
             mbar_init(&bars.kv_empty[i], 1);
             mbar_init(&bars.s_full[i], 1);
             mbar_init(&bars.p_ready[i], kPcRows);
@@ -162,37 +173,76 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 const int e = min(13 - ((__float_as_int(a) >> 23) - 127), 126);
                 const float up = exp2_int(e);
                 down = exp2_int(-e);
-                uint8_t *dst = smem + T * 2 * S::kQPlane + rl * 16;
-#pragma unroll 2
-                for (int c = 0; c < HD / 8; ++c) {
-                    float w[8];
+                const uint32_t tq = tmem + ((uint32_t)((warp & 3) * 32) << 16) + S::kQ + T * S::kQTile;
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t h[16], lw[16];
 #pragma unroll
-                    for (int k = 0; k < 8; k += 4) {
-                        const float4 v = *reinterpret_cast<const float4 *>(src + c * 8 + k);
-                        w[k] = v.x * p.qscale * up, w[k + 1] = v.y * p.qscale * up;
-                        w[k + 2] = v.z * p.qscale * up, w[k + 3] = v.w * p.qscale * up;
+                    for (int k = 0; k < 32; k += 4) {
+                        const float4 v = *reinterpret_cast<const float4 *>(src + c * 32 + k);
+                        split_half2(v.x * p.qscale * up, v.y * p.qscale * up, h[k / 2], lw[k / 2]);
+                        split_half2(v.z * p.qscale * up, v.w * p.qscale * up, h[k / 2 + 1], lw[k / 2 + 1]);
                     }
-                    uint4 h, l;
-                    split_half2(w[0], w[1], h.x, l.x);
-                    split_half2(w[2], w[3], h.y, l.y);
-                    split_half2(w[4], w[5], h.z, l.z);
-                    split_half2(w[6], w[7], h.w, l.w);
-                    *reinterpret_cast<uint4 *>(dst + c * (kPcRows * 16)) = h;
-                    *reinterpret_cast<uint4 *>(dst + S::kQPlane + c * (kPcRows * 16)) = l;
+                    tmem_st16(tq + c * 16, h);
+                    if (HD == 128) { // K-major core matrices
+                        uint8_t *dst = smem + T * S::kQPlane + rl * 16 + c * 4 * (kPcRows * 16);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            *reinterpret_cast<uint4 *>(dst + k * (kPcRows * 16)) = make_uint4(lw[4 * k], lw[4 * k + 1], lw[4 * k + 2], lw[4 * k + 3]);
+                    } else {
+                        tmem_st16(tq + S::kQCols + c * 16, lw);
+                    }
                 }
+                tc_wait_st();
+                tc_fence_before();
                 fence_async_smem();
                 mbar_arrive(&bars.q_full);
             }
+            float *dst = p.splits > 1 ? p.ws + (((int64_t)(r0 + i) * p.H + head) * p.splits + split) * PR
+                                      : p.out + (int64_t)(r0 + i) * p.os + (int64_t)head * HD;
+            // Sums that were folded (`since`: how far O's unit has moved from theirs) lie in shared memory, a thread's next to
+            // its neighbours'. At head_dim 128 there is no room for them: they lie in the warp's 32 output rows, in an order
+            // of their own, lane l's k-th four values at row 4 (k % 8) + l / 8, column 32 (k / 8) + 4 (l % 8), so that an
+            // access is four whole lines; a warp with fewer rows uses each row for itself.
+            const bool full = __all_sync(0xffffffffu, live);
+            float since = 1.0f;
+            auto place = [&](int k) -> float4 * {
+                if (HD <= 64) return reinterpret_cast<float4 *>(smem + S::kOffSum) + (T * (HD / 4) + k) * kPcRows + rl;
+                const uint64_t row = __shfl_sync(0xffffffffu, (uint64_t)dst, 4 * (k & 7) + (lane >> 3));
+                return full ? reinterpret_cast<float4 *>(row) + 8 * (k >> 3) + (lane & 7) : reinterpret_cast<float4 *>(dst) + k;
+            };
             float m = -INFINITY, l = 0.0f;
-            bool ok = true;
-            for (int j = 0; j < nst; ++j) {
+            int R = 0;
+            bool ok = nst == 0 || mbar_wait_abort(&bars.kv_full[0], 0, abortp);
+            if (!ok && lane == 0) give_up(0x55);
+            for (int j = 0; j < nst && ok; ++j) { // the tile's scales are there: waited for at the end of the step before
                 const int st = j & 1, kb = kb0 + j * BN;
-                if (!mbar_wait_abort(&bars.k_full[st], (j >> 1) & 1, abortp) || !mbar_wait_abort(&bars.s_full[T], j & 1, abortp)) {
+                if (!mbar_wait_abort(&bars.s_full[T], j & 1, abortp)) {
                     if (lane == 0) give_up(0x51);
                     ok = false;
                     break;
                 }
                 tc_fence_after();
+                if (j > 0 && j % kFold == 0) { // O is complete: S came behind it
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; ++c) {
+                        float o[32];
+                        float4 *at[8], v[8];
+                        tmem_ld32(trow + S::kO + c * 32, o);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            at[k] = place(8 * c + k);
+                            v[k] = j > kFold && (live || HD <= 64) ? *at[k] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+                        tc_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if (live || HD <= 64)
+                                *at[k] = make_float4(fmaf(v[k].x, since, o[4 * k]), fmaf(v[k].y, since, o[4 * k + 1]),
+                                                     fmaf(v[k].z, since, o[4 * k + 2]), fmaf(v[k].w, since, o[4 * k + 3]));
+                    }
+                    since = 1.0f;
+                }
                 bool all = true;
 #pragma unroll
                 for (int g = 0; g < BN / 16; ++g) all &= present[st][g] != 0;
@@ -202,14 +252,14 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 {
                     float v[CH][32];
 #pragma unroll
-                    for (int c = 0; c < CH; ++c) tmem_ld32(trow + S::kS + c * 32, v[c]);
+                    for (int c = 0; c < CH; ++c) tmem_ld32(trow + c * 32, v[c]);
                     tc_wait_ld();
 #pragma unroll
                     for (int c = 0; c < CH; ++c)
 #pragma unroll
                         for (int k = 0; k < 16; ++k) y[c][k] = make_float2(v[c][2 * k], v[c][2 * k + 1]);
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float peak[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -217,10 +267,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         const float4 ks = *reinterpret_cast<const float4 *>(&kscale[st][c * 32 + k * 2]);
                         y[c][k] = __fmul2_rn(y[c][k], make_float2(ks.x, ks.y));
                         y[c][k + 1] = __fmul2_rn(y[c][k + 1], make_float2(ks.z, ks.w));
-                        top[k & 2] = fmaxf(fmaxf(top[k & 2], y[c][k].x), y[c][k].y);
-                        top[(k & 2) + 1] = fmaxf(fmaxf(top[(k & 2) + 1], y[c][k + 1].x), y[c][k + 1].y);
+                        peak[k & 2] = fmaxf(fmaxf(peak[k & 2], y[c][k].x), y[c][k].y);
+                        peak[(k & 2) + 1] = fmaxf(fmaxf(peak[(k & 2) + 1], y[c][k + 1].x), y[c][k + 1].y);
                     }
-                float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * down;
+                float mx = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3])) * down;
                 // Sums of 8-bit codes times query planes below 2^14 stay far from overflow, so a score is not finite only
                 // where the query row is not, or where the scales took it past fp32's range (-inf weighs 0 by itself).
                 if (__any_sync(0xffffffffu, masked || qbad || !(mx < INFINITY))) {
@@ -237,48 +287,93 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         }
                     mx *= down;
                 }
-                // ---- O follows the maximum only when that has grown by more than 2^8: until then weights exceed 1
-                const bool grow = mx > m + 8.0f || (m == -INFINITY && mx > m);
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float f = grow ? t5_ex2(m - mx) : 1.0f; // 2^-inf = 0 where there was no maximum
-                    l *= f;
-                    if (grow) m = mx;
-                    if (j > 0) {
-#pragma unroll 1
-                        for (int c = 0; c < HD / 32; ++c) {
-                            float o[32];
-                            uint32_t w[32];
-                            tmem_ld32(trow + S::kO + c * 32, o);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * f);
-                            tmem_st32(trow + S::kO + c * 32, w);
-                        }
-                    }
+                // ---- O and its unit follow the maximum only when that has grown by more than 2^4 (weights exceed 1 until then),
+                // and the unit alone where p 2^et has passed 2^(R + 4)
+                const int et = vtop[st][0];
+                const bool wide = vtop[st][1] != 0;
+                const bool grow = mx > m + 4.0f || (m == -INFINITY && mx > m);
+                float f = 1.0f;
+                if (grow) {
+                    const float d = m == -INFINITY ? -4096.0f : fmaxf(m - mx, -4096.0f), whole = floorf(d);
+                    l *= t5_ex2(d);
+                    f = m == -INFINITY ? 0.0f : t5_ex2(d - whole);
+                    R = m == -INFINITY ? et - 4096 : R + (int)whole;
+                    m = mx;
                 }
-                // ---- weights, their sum, and their three planes over the scores
                 const float mref = m == -INFINITY ? 0.0f : -m;
-                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                int top = et + (int)floorf(fminf(fmaxf(mx + mref, -4096.0f), 64.0f)); // the tile's largest p 2^et
+                if (wide) {
+                    float w = 0.0f;
 #pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    uint32_t ph[16], pm[16], pl[16];
+                    for (int c = 0; c < CH; ++c)
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        float2 w = __ffma2_rn(y[c][k], make_float2(down, down), make_float2(mref, mref));
-                        w = make_float2(t5_ex2(w.x), t5_ex2(w.y));
-                        sum[k & 1] = __fadd2_rn(sum[k & 1], w);
-                        ph[k] = bf16_plane(w);
-                        pm[k] = bf16_plane(w);
-                        pl[k] = bf16_plane(w);
-                    }
-                    tmem_st16(trow + c * 48, ph);
-                    tmem_st16(trow + c * 48 + 16, pm);
-                    tmem_st16(trow + c * 48 + 32, pl);
+                        for (int k = 0; k < 16; ++k) {
+                            w = fmaxf(w, t5_ex2(fmaf(y[c][k].x, down, mref)) * vscale[st][c * 32 + 2 * k]);
+                            w = fmaxf(w, t5_ex2(fmaf(y[c][k].y, down, mref)) * vscale[st][c * 32 + 2 * k + 1]);
+                        }
+                    top = w > 0.0f ? et + (__float_as_int(w) >> 23) - 127 : R;
                 }
-                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                const bool raise = mx > -INFINITY && top > R + 4;
+                if (raise) {
+                    f *= R - top < -126 ? 0.0f : exp2_int(R - top);
+                    R = top;
+                }
+                since *= f;
+                if (j % kFold != 0 && __any_sync(0xffffffffu, grow || raise)) {
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; ++c) {
+                        float o[32];
+                        uint32_t w[32];
+                        tmem_ld32(trow + S::kO + c * 32, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * f);
+                        tmem_st32(trow + S::kO + c * 32, w);
+                    }
+                }
+                // ---- weights in units of 2^(R - head), their sum, and their two planes over the scores
+                const int lift = min(max(et - R + kPcHead, -4096), 126); // p 2^et 2^-(R - head) = 2^(s - m + lift)
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                if (!__any_sync(0xffffffffu, wide || lift < -64)) {
+                    const float ref = mref + (float)lift;
+#pragma unroll
+                    for (int c = 0; c < CH; ++c) {
+                        uint32_t ph[16], pl[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            float2 w = __ffma2_rn(y[c][k], make_float2(down, down), make_float2(ref, ref));
+                            w = make_float2(t5_ex2(w.x), t5_ex2(w.y));
+                            sum[k & 1] = __fadd2_rn(sum[k & 1], w);
+                            split_half2(w.x, w.y, ph[k], pl[k]);
+                        }
+                        tmem_st16(trow + c * 32, ph);
+                        tmem_st16(trow + c * 32 + 16, pl);
+                    }
+                    l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) * exp2_int(-lift);
+                } else { // the sum is taken before V's scales
+                    const float fw = lift < -126 ? 0.0f : exp2_int(lift);
+#pragma unroll
+                    for (int c = 0; c < CH; ++c) {
+                        uint32_t ph[16], pl[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float2 w = make_float2(t5_ex2(fmaf(y[c][k].x, down, mref)), t5_ex2(fmaf(y[c][k].y, down, mref)));
+                            sum[k & 1] = __fadd2_rn(sum[k & 1], w);
+                            const float a = wide ? vscale[st][c * 32 + 2 * k] : 1.0f, e = wide ? vscale[st][c * 32 + 2 * k + 1] : 1.0f;
+                            split_half2(w.x * a * fw, w.y * e * fw, ph[k], pl[k]);
+                        }
+                        tmem_st16(trow + c * 32, ph);
+                        tmem_st16(trow + c * 32 + 16, pl);
+                    }
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                }
                 tc_wait_st();
                 tc_fence_before();
                 mbar_arrive(&bars.p_ready[T]);
+                if (j + 1 < nst && !mbar_wait_abort(&bars.kv_full[st ^ 1], ((j + 1) >> 1) & 1, abortp)) {
+                    if (lane == 0) give_up(0x55);
+                    ok = false;
+                }
             }
             if (ok && nst > 0 && !mbar_wait_abort(&bars.o_full, 0, abortp)) {
                 if (lane == 0) give_up(0x52);
@@ -286,9 +381,15 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             }
             if (__all_sync(0xffffffffu, ok)) {
                 tc_fence_after();
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                float *dst = p.splits > 1 ? p.ws + (((int64_t)(r0 + i) * p.H + head) * p.splits + split) * PR
-                                          : p.out + (int64_t)(r0 + i) * p.os + (int64_t)head * HD;
+                // 2^(R - head) in two steps: it may lie below what one float holds
+                const float inv = (l > 0.0f ? 1.0f / l : 0.0f) * (1.0f / (1 << kPcHead)), unit = R < -126 ? 0.0f : exp2_int(min(R, 127));
+                float4 v[HD / 4];
+#pragma unroll
+                for (int k = 0; k < HD / 4; ++k) {
+                    const float4 *at = place(k);
+                    v[k] = nst > kFold && live ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                __syncwarp(); // every lane has read before the rows are written
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) {
                     float o[32];
@@ -298,10 +399,13 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                     }
                     if (live) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4)
-                            *reinterpret_cast<float4 *>(dst + c * 32 + k) =
-                                l > 0.0f ? make_float4(o[k] * inv, o[k + 1] * inv, o[k + 2] * inv, o[k + 3] * inv)
+                        for (int k = 0; k < 8; ++k) {
+                            const float4 w = v[8 * c + k];
+                            *reinterpret_cast<float4 *>(dst + c * 32 + 4 * k) =
+                                l > 0.0f ? make_float4(fmaf(w.x, since, o[4 * k]) * inv * unit, fmaf(w.y, since, o[4 * k + 1]) * inv * unit,
+                                                       fmaf(w.z, since, o[4 * k + 2]) * inv * unit, fmaf(w.w, since, o[4 * k + 3]) * inv * unit)
                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
                     }
                 }
                 if (live && p.splits > 1) *reinterpret_cast<float2 *>(dst + HD) = make_float2(m, l);
@@ -323,11 +427,12 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             return p.pv.row(page, kvh, k - pi * p.pv.page_size);
         };
         uint4 kr[NP], vr[NP];
-        float ks = 0.0f, vs = 0.0f;
+        float ks = 0.0f;
+        int ev = 0;
         bool here = false;
         auto load = [&](int64_t row) { // a key that is not there: zeros
             here = row >= 0;
-            ks = vs = 0.0f;
+            ks = 0.0f;
 #pragma unroll
             for (int i = 0; i < NP; ++i) kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
             if (here) {
@@ -338,17 +443,15 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
 #pragma unroll
                 for (int i = 0; i < NP; ++i) vr[i] = __ldg(vp + i);
                 ks = kv_scale<FMT>(p.pv.ke[row]);
-                vs = kv_scale<FMT>(p.pv.ve[row]);
+                ev = min(max((int)p.pv.ve[row], F::kEmin), F::kEmax);
             }
         };
         load(look(0));
         int64_t next = look(1);
         for (int j = 0; j < nst; ++j) {
             const int st = j & 1;
-            if (j >= 2 && !mbar_wait_abort(&bars.kv_empty[st], ((j >> 1) - 1) & 1, abortp)) {
-                if (lane == 0) give_up(0x53);
-                break;
-            }
+            const bool lost = j >= 2 && !mbar_wait_abort(&bars.kv_empty[st], ((j >> 1) - 1) & 1, abortp);
+            if (lost && lane == 0) give_up(0x53);
             uint8_t *kd = smem + S::kOffKv + st * 2 * S::kKv + key * 16, *vd = kd + S::kKv;
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
@@ -365,24 +468,45 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 kscale[st][key] = ks;
                 if ((lane & 15) == 0) present[st][key / 16] = ((vote >> lane) & 0xffff) != 0;
             }
-            fence_async_smem();
-            mbar_arrive(&bars.k_full[st]);
+            // ---- the tile's range of V exponents (keys that are there), then its halves
+            const int hi_e = __reduce_max_sync(0xffffffffu, here ? ev : -1000), lo_e = __reduce_min_sync(0xffffffffu, here ? ev : 1000);
+            if (lane == 0) {
+                vrange[st][warp - 8][0] = hi_e;
+                vrange[st][warp - 8][1] = lo_e;
+            }
+            if (converters_or(lost)) break; // all four warps go on or none
+            int et = vrange[st][0][0], eb = vrange[st][0][1];
+#pragma unroll
+            for (int i = 1; i < 4; ++i) {
+                et = max(et, vrange[st][i][0]);
+                eb = min(eb, vrange[st][i][1]);
+            }
+            const bool none = et < F::kEmin, wide = !none && et - eb > kPcNarrow;
+            if (ct == 0) {
+                vtop[st][0] = none ? 0 : et;
+                vtop[st][1] = wide;
+            }
+            const int below = here ? et - ev : 0; // 2^-below goes into the halves, or into P's columns
+            if (piece0 == 0) vscale[st][key] = below > 126 ? 0.0f : exp2_int(-below);
+            const __half2 vs = wide ? __float2half2_rn(1.0f) : __float2half2_rn(exp2_int(-below));
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
                 uint32_t x[8];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float4 v = kv_values<FMT>(w[k], vs);
-                    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), c = __floats2bfloat162_rn(v.z, v.w);
-                    x[2 * k] = *reinterpret_cast<const uint32_t *>(&a);
-                    x[2 * k + 1] = *reinterpret_cast<const uint32_t *>(&c);
+                    F::halves(w[k], x[2 * k], x[2 * k + 1]);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        __half2 &hv = *reinterpret_cast<__half2 *>(&x[2 * k + q]);
+                        hv = __hmul2(hv, vs); // exact: a code has 8 bits, and 2^-4 of the least is a half
+                    }
                 }
                 *reinterpret_cast<uint4 *>(vd + (piece0 + i) * 2 * (BN * 16)) = make_uint4(x[0], x[1], x[2], x[3]);
                 *reinterpret_cast<uint4 *>(vd + ((piece0 + i) * 2 + 1) * (BN * 16)) = make_uint4(x[4], x[5], x[6], x[7]);
             }
             fence_async_smem();
-            mbar_arrive(&bars.v_full[st]);
+            mbar_arrive(&bars.kv_full[st]);
             load(next);
             next = look(j + 2);
         }
@@ -390,24 +514,28 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 12) {
             // ================= issuer (the warp goes along, one lane issues) =================
-            constexpr uint32_t kIdS = pc_idesc(BN, false, false), kIdO = pc_idesc(HD, true, true);
+            constexpr uint32_t kIdS = pc_idesc(BN, false), kIdO = pc_idesc(HD, true);
             // S = Q K^T: a 16-deep product reads two 8-column core matrices, BN (128) rows apart
             auto issue_s = [&](int T, int st) {
-                const uint32_t q = sbase + T * 2 * S::kQPlane, k = sbase + S::kOffKv + st * 2 * S::kKv, d = tmem + T * S::kTile + S::kS;
+                const uint32_t q = tmem + S::kQ + T * S::kQTile, k = sbase + S::kOffKv + st * 2 * S::kKv, d = tmem + T * S::kTile;
                 if (elect_one()) {
 #pragma unroll
                     for (int pl = 1; pl >= 0; --pl)
 #pragma unroll
-                        for (int s = 0; s < HD / 16; ++s)
-                            mma_f16_ss(d, t5_desc(q + pl * S::kQPlane + s * 2 * (kPcRows * 16), kPcRows * 16, 128),
-                                       t5_desc(k + s * 2 * (BN * 16), BN * 16, 128), kIdS, pl == 0 || s > 0);
+                        for (int s = 0; s < HD / 16; ++s) {
+                            const uint64_t kd = t5_desc(k + s * 2 * (BN * 16), BN * 16, 128);
+                            if (HD == 128 && pl == 1)
+                                mma_f16_ss(d, t5_desc(sbase + T * S::kQPlane + s * 2 * (kPcRows * 16), kPcRows * 16, 128), kd, kIdS, s > 0);
+                            else
+                                mma_f16_ts(d, q + pl * S::kQCols + s * 8, kd, kIdS, pl == 0 || s > 0);
+                        }
                     tc_commit(&bars.s_full[T]);
                 }
                 __syncwarp();
             };
             bool ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.q_full, 0, abortp));
             if (ok && nst > 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.k_full[0], 0, abortp));
+                ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.kv_full[0], 0, abortp));
                 if (ok) {
                     tc_fence_after();
                     for (int T = 0; T < tiles; ++T) issue_s(T, 0);
@@ -415,27 +543,25 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 for (int j = 0; j < nst && ok; ++j) {
                     const int st = j & 1;
                     for (int T = 0; T < tiles; ++T) {
-                        ok = mbar_wait_abort(&bars.p_ready[T], j & 1, abortp) &&
-                             (T > 0 || mbar_wait_abort(&bars.v_full[st], (j >> 1) & 1, abortp));
-                        ok = __all_sync(0xffffffffu, ok);
+                        ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.p_ready[T], j & 1, abortp));
                         if (!ok) break;
                         tc_fence_after();
                         // O += P V: 16 keys are two 8-row core matrices of V, 128 bytes apart; 8 columns of O the next BN rows on
                         const uint32_t v = sbase + S::kOffKv + st * 2 * S::kKv + S::kKv, a = tmem + T * S::kTile, d = a + S::kO;
                         if (elect_one()) {
 #pragma unroll
-                            for (int pl = 2; pl >= 0; --pl)
+                            for (int pl = 1; pl >= 0; --pl)
 #pragma unroll
                                 for (int s = 0; s < BN / 16; ++s)
-                                    mma_f16_ts(d, a + (s >> 1) * 48 + pl * 16 + (s & 1) * 8, t5_desc(v + s * 256, 128, BN * 16), kIdO,
-                                               j > 0 || pl < 2 || s > 0);
+                                    mma_f16_ts(d, a + (s >> 1) * 32 + pl * 16 + (s & 1) * 8, t5_desc(v + s * 256, 128, BN * 16), kIdO,
+                                               j % kFold != 0 || pl < 1 || s > 0);
                             if (T == tiles - 1) tc_commit(&bars.kv_empty[st]);
                             if (j == nst - 1 && T == tiles - 1) tc_commit(&bars.o_full);
                         }
                         __syncwarp();
                         if (j + 1 < nst) {
                             if (T == 0) {
-                                ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.k_full[st ^ 1], ((j + 1) >> 1) & 1, abortp));
+                                ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.kv_full[st ^ 1], ((j + 1) >> 1) & 1, abortp));
                                 if (!ok) break;
                                 tc_fence_after();
                             }

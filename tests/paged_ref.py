@@ -100,11 +100,12 @@ def attention(q, k, v, base, scale, block, window):
     denominator carry it both: twice. Weights and values then carry 22 bits, and a sum over L keys is made of at most
     3 L / 8 + 64 additions of 2^-23.
 
-    Weights times V's scales, p 2^e, may be held in halves in units of 2^(R - 10), R at most one above the exponent of
-    the row's largest p 2^e (key k*): half a step of a half's fixed-point end is 2^-25 of that unit, an error of
-    2^-34 p* 2^e* in each weight and so of 2^-34 p* 2^e* Qmax in its product with a code. The largest |v| of row k* is at
-    least Qmax / 2 * 2^e* (e is the least one that will do), so max_d sum_k p_k |v_kd| >= p* 2^e* Qmax / 2, and L keys
-    give at most L 2^-33 of that maximum over d (it shows where an element's own sum leaves out the large rows)."""
+    Weights times V's scales, p 2^e, may be held in halves in units of 2^(R - 10), R at most five above the exponent of
+    the row's largest p 2^e (key k*; four for the exponents of a tile that are taken as one, one for rounding a moved
+    maximum down): half a step of a half's fixed-point end is 2^-25 of that unit, an error of 2^-30 p* 2^e* in each
+    weight and so of 2^-30 p* 2^e* Qmax in its product with a code. The largest |v| of row k* is at least Qmax / 2 * 2^e*
+    (e is the least one that will do), so max_d sum_k p_k |v_kd| >= p* 2^e* Qmax / 2, and L keys give at most L 2^-29 of
+    that maximum over d (it shows where an element's own sum leaves out the large rows)."""
     n, H, hd = q.shape
     KV, L = k.shape[1], k.shape[0]
     q, k, v = q.double().cpu(), k.double().cpu(), v.double().cpu()
@@ -130,5 +131,5 @@ def attention(q, k, v, base, scale, block, window):
         live = torch.where(torch.isfinite(s), a, torch.zeros_like(a)).amax(-1, keepdim=True)
         ds = live * (2.0 ** -22 + (hd + 8) * 2.0 ** -23) + 2.0 ** -22
         pv = p @ vv.abs()
-        tol[:, h] = pv * (2 * ds + 2.0 ** -21 + (3 * L / 8 + 64) * 2.0 ** -23) + pv.amax(-1, keepdim=True) * L * 2.0 ** -33 + 1e-37
+        tol[:, h] = pv * (2 * ds + 2.0 ** -21 + (3 * L / 8 + 64) * 2.0 ** -23) + pv.amax(-1, keepdim=True) * L * 2.0 ** -29 + 1e-37
     return out, tol
