@@ -4,9 +4,10 @@
 // CTA = (sequence, kv head, key range, 256 query rows as two tiles of 128), one per SM; K and V tiles of BN keys are
 // converted once for both query tiles. An 8-bit code is a half as it stands, so K and V are ONE fp16 plane each and the
 // 22 bits of fp32 class come from two planes of Q and of P: two MMAs where 16-bit attention has one.
-//   S = Q K^T    Q is scaled by its row's power of two; K's exponents multiply the columns of S as the softmax reads them.
-//   O += P V     V's exponents within a tile go into its halves where they lie within 2^4 of each other (rows of one
-//                head: nearly always), relative to the tile's largest, 2^et; into P's columns otherwise. O is in units of
+// The exponents of a tile's K (V) go into its halves, relative to the tile's largest, where they lie within 2^4 of each
+// other (rows of one head: nearly always); otherwise they multiply the columns of S (P).
+//   S = Q K^T    Q is scaled by its row's power of two.
+//   O += P V     2^et is the largest scale of the tile's V. O is in units of
 //                2^R, a row's own R, which follows the largest p 2^et the row has had, so that P's halves keep the 22
 //                bits of what counts; et, R and the maximum meet in the exponent of 2^x and cost nothing per score.
 //
@@ -42,7 +43,7 @@ constexpr int kPcHead = 10;   // P in units of 2^(R - kPcHead), R at most 4 belo
 constexpr int kPcFold = 512;  // keys whose products the tensor cores sum: they cut every sum off below 24 bits, which pulls
                               // O towards zero by about 2e-8 an MMA (9e-6 over 31 k keys in eight pieces; 512 keys are 64
                               // MMAs); what they have is then added, rounded, to sums of its own
-constexpr int kPcNarrow = 4;  // V's exponents go into its halves where they lie this close
+constexpr int kPcNarrow = 4;  // exponents of a tile go into its halves where they lie this close
 
 // fp16 operands, fp32 accumulate; B K-major or MN-major
 __host__ __device__ constexpr uint32_t pc_idesc(int n, bool mn_major) {
@@ -81,6 +82,12 @@ __device__ __forceinline__ bool converters_or(bool x) {
     return any != 0;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 struct PcBars {
     uint64_t q_full, kv_full[2], kv_empty[2], s_full[2], p_ready[2], o_full, fin;
 };
@@ -93,8 +100,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ PcBars bars;
     __shared__ __align__(16) float kscale[2][BN], vscale[2][BN];
-    __shared__ int vtop[2][2]; // largest exponent of the tile's V, and whether they are too far apart for its halves
-    __shared__ int vrange[2][4][2];
+    __shared__ __align__(16) int top_of[2][4]; // largest exponent of the tile's K, of its V; whether each is too wide for its halves
+    __shared__ int4 range[2][4];
     __shared__ __align__(8) uint8_t present[2][8]; // groups of 16 keys whose page exists and that the CTA reads
     __shared__ uint32_t tmem_slot;
     __shared__ int s_abort;
@@ -155,7 +162,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             const int span = hi - lo;
             const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T * S::kTile;
             // ---- query planes: q scale log2(e) 2^e with the row's largest value in [2^13, 2^14)
-            float down;
+            int qe; // the row of Q was multiplied by 2^qe
             bool qbad = false; // a query value that is not finite
             {
                 const float *src = p.q + (int64_t)(r0 + i) * p.qs + (int64_t)head * HD;
@@ -170,9 +177,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         else qbad = true;
                     }
                 }
-                const int e = min(13 - ((__float_as_int(a) >> 23) - 127), 126);
-                const float up = exp2_int(e);
-                down = exp2_int(-e);
+                qe = min(13 - ((__float_as_int(a) >> 23) - 127), 126);
+                const float up = exp2_int(qe);
                 const uint32_t tq = tmem + ((uint32_t)((warp & 3) * 32) << 16) + S::kQ + T * S::kQTile;
 #pragma unroll 1
                 for (int c = 0; c < HD / 32; ++c) {
@@ -264,16 +270,15 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 for (int c = 0; c < CH; ++c)
 #pragma unroll
                     for (int k = 0; k < 16; k += 2) {
-                        const float4 ks = *reinterpret_cast<const float4 *>(&kscale[st][c * 32 + k * 2]);
-                        y[c][k] = __fmul2_rn(y[c][k], make_float2(ks.x, ks.y));
-                        y[c][k + 1] = __fmul2_rn(y[c][k + 1], make_float2(ks.z, ks.w));
-                        peak[k & 2] = fmaxf(fmaxf(peak[k & 2], y[c][k].x), y[c][k].y);
-                        peak[(k & 2) + 1] = fmaxf(fmaxf(peak[(k & 2) + 1], y[c][k + 1].x), y[c][k + 1].y);
+                        peak[k & 2] = max3(peak[k & 2], y[c][k].x, y[c][k].y);
+                        peak[(k & 2) + 1] = max3(peak[(k & 2) + 1], y[c][k + 1].x, y[c][k + 1].y);
                     }
+                const int4 tops = *reinterpret_cast<const int4 *>(top_of[st]);
+                const float down = exp2_int(min(max(tops.x + F::kShift - qe, -126), 126));
                 float mx = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3])) * down;
                 // Sums of 8-bit codes times query planes below 2^14 stay far from overflow, so a score is not finite only
                 // where the query row is not, or where the scales took it past fp32's range (-inf weighs 0 by itself).
-                if (__any_sync(0xffffffffu, masked || qbad || !(mx < INFINITY))) {
+                if (__any_sync(0xffffffffu, masked || tops.z || qbad || !(mx < INFINITY))) {
                     mx = -INFINITY;
 #pragma unroll
                     for (int c = 0; c < CH; ++c)
@@ -281,6 +286,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         for (int k = 0; k < 16; ++k) {
                             const int d = kb + c * 32 + 2 * k - lo;
                             const bool there = present[st][c * 2 + k / 8] != 0;
+                            if (tops.z) {
+                                y[c][k].x *= kscale[st][c * 32 + 2 * k];
+                                y[c][k].y *= kscale[st][c * 32 + 2 * k + 1];
+                            }
                             y[c][k].x = there && (unsigned)d < (unsigned)span && finite_f(y[c][k].x * down) ? y[c][k].x : -INFINITY;
                             y[c][k].y = there && (unsigned)(d + 1) < (unsigned)span && finite_f(y[c][k].y * down) ? y[c][k].y : -INFINITY;
                             mx = fmaxf(fmaxf(mx, y[c][k].x), y[c][k].y);
@@ -289,8 +298,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 }
                 // ---- O and its unit follow the maximum only when that has grown by more than 2^4 (weights exceed 1 until then),
                 // and the unit alone where p 2^et has passed 2^(R + 4)
-                const int et = vtop[st][0];
-                const bool wide = vtop[st][1] != 0;
+                const int et = tops.y;
+                const bool wide = tops.w != 0;
                 const bool grow = mx > m + 4.0f || (m == -INFINITY && mx > m);
                 float f = 1.0f;
                 if (grow) {
@@ -427,12 +436,11 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             return p.pv.row(page, kvh, k - pi * p.pv.page_size);
         };
         uint4 kr[NP], vr[NP];
-        float ks = 0.0f;
-        int ev = 0;
+        int ek = 0, ev = 0;
         bool here = false;
         auto load = [&](int64_t row) { // a key that is not there: zeros
             here = row >= 0;
-            ks = 0.0f;
+            ek = ev = 0;
 #pragma unroll
             for (int i = 0; i < NP; ++i) kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
             if (here) {
@@ -442,7 +450,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 for (int i = 0; i < NP; ++i) kr[i] = __ldg(kp + i);
 #pragma unroll
                 for (int i = 0; i < NP; ++i) vr[i] = __ldg(vp + i);
-                ks = kv_scale<FMT>(p.pv.ke[row]);
+                ek = min(max((int)p.pv.ke[row], F::kEmin), F::kEmax);
                 ev = min(max((int)p.pv.ve[row], F::kEmin), F::kEmax);
             }
         };
@@ -452,59 +460,49 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             const int st = j & 1;
             const bool lost = j >= 2 && !mbar_wait_abort(&bars.kv_empty[st], ((j >> 1) - 1) & 1, abortp);
             if (lost && lane == 0) give_up(0x53);
-            uint8_t *kd = smem + S::kOffKv + st * 2 * S::kKv + key * 16, *vd = kd + S::kKv;
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                uint4 x, y;
-                F::halves(kr[i].x, x.x, x.y);
-                F::halves(kr[i].y, x.z, x.w);
-                F::halves(kr[i].z, y.x, y.y);
-                F::halves(kr[i].w, y.z, y.w);
-                *reinterpret_cast<uint4 *>(kd + (piece0 + i) * 2 * (BN * 16)) = x;
-                *reinterpret_cast<uint4 *>(kd + ((piece0 + i) * 2 + 1) * (BN * 16)) = y;
-            }
-            const uint32_t vote = __ballot_sync(0xffffffffu, here);
-            if (piece0 == 0) {
-                kscale[st][key] = ks;
-                if ((lane & 15) == 0) present[st][key / 16] = ((vote >> lane) & 0xffff) != 0;
-            }
-            // ---- the tile's range of V exponents (keys that are there), then its halves
-            const int hi_e = __reduce_max_sync(0xffffffffu, here ? ev : -1000), lo_e = __reduce_min_sync(0xffffffffu, here ? ev : 1000);
-            if (lane == 0) {
-                vrange[st][warp - 8][0] = hi_e;
-                vrange[st][warp - 8][1] = lo_e;
+            // ---- the tile's range of exponents (keys that are there)
+            {
+                const int4 r = make_int4(__reduce_max_sync(0xffffffffu, here ? ek : -1000), __reduce_min_sync(0xffffffffu, here ? ek : 1000),
+                                         __reduce_max_sync(0xffffffffu, here ? ev : -1000), __reduce_min_sync(0xffffffffu, here ? ev : 1000));
+                if (lane == 0) range[st][warp - 8] = r;
             }
             if (converters_or(lost)) break; // all four warps go on or none
-            int et = vrange[st][0][0], eb = vrange[st][0][1];
+            int4 e = range[st][0];
 #pragma unroll
             for (int i = 1; i < 4; ++i) {
-                et = max(et, vrange[st][i][0]);
-                eb = min(eb, vrange[st][i][1]);
+                const int4 r = range[st][i];
+                e = make_int4(max(e.x, r.x), min(e.y, r.y), max(e.z, r.z), min(e.w, r.w));
             }
-            const bool none = et < F::kEmin, wide = !none && et - eb > kPcNarrow;
-            if (ct == 0) {
-                vtop[st][0] = none ? 0 : et;
-                vtop[st][1] = wide;
+            const bool none = e.x < F::kEmin, kwide = !none && e.x - e.y > kPcNarrow, vwide = !none && e.z - e.w > kPcNarrow;
+            const int kbelow = here ? e.x - ek : 0, vbelow = here ? e.z - ev : 0; // 2^-below: into the halves or the columns
+            if (ct == 0) *reinterpret_cast<int4 *>(top_of[st]) = make_int4(none ? 0 : e.x, none ? 0 : e.z, kwide, vwide);
+            const uint32_t vote = __ballot_sync(0xffffffffu, here);
+            if (piece0 == 0) {
+                kscale[st][key] = kbelow > 126 ? 0.0f : exp2_int(-kbelow);
+                vscale[st][key] = vbelow > 126 ? 0.0f : exp2_int(-vbelow);
+                if ((lane & 15) == 0) present[st][key / 16] = ((vote >> lane) & 0xffff) != 0;
             }
-            const int below = here ? et - ev : 0; // 2^-below goes into the halves, or into P's columns
-            if (piece0 == 0) vscale[st][key] = below > 126 ? 0.0f : exp2_int(-below);
-            const __half2 vs = wide ? __float2half2_rn(1.0f) : __float2half2_rn(exp2_int(-below));
+            auto put = [&](uint8_t *dst, const uint4(&raw)[NP], __half2 s) {
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-                uint32_t x[8];
+                for (int i = 0; i < NP; ++i) {
+                    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    uint32_t x[8];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    F::halves(w[k], x[2 * k], x[2 * k + 1]);
+                    for (int k = 0; k < 4; ++k) {
+                        F::halves(w[k], x[2 * k], x[2 * k + 1]);
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        __half2 &hv = *reinterpret_cast<__half2 *>(&x[2 * k + q]);
-                        hv = __hmul2(hv, vs); // exact: a code has 8 bits, and 2^-4 of the least is a half
+                        for (int q = 0; q < 2; ++q) {
+                            __half2 &hv = *reinterpret_cast<__half2 *>(&x[2 * k + q]);
+                            hv = __hmul2(hv, s); // exact: a code has 8 bits, and 2^-4 of the least is a half
+                        }
                     }
+                    *reinterpret_cast<uint4 *>(dst + (piece0 + i) * 2 * (BN * 16)) = make_uint4(x[0], x[1], x[2], x[3]);
+                    *reinterpret_cast<uint4 *>(dst + ((piece0 + i) * 2 + 1) * (BN * 16)) = make_uint4(x[4], x[5], x[6], x[7]);
                 }
-                *reinterpret_cast<uint4 *>(vd + (piece0 + i) * 2 * (BN * 16)) = make_uint4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<uint4 *>(vd + ((piece0 + i) * 2 + 1) * (BN * 16)) = make_uint4(x[4], x[5], x[6], x[7]);
-            }
+            };
+            uint8_t *kd = smem + S::kOffKv + st * 2 * S::kKv + key * 16;
+            put(kd, kr, __float2half2_rn(kwide ? 1.0f : exp2_int(-kbelow)));
+            put(kd + S::kKv, vr, __float2half2_rn(vwide ? 1.0f : exp2_int(-vbelow)));
             fence_async_smem();
             mbar_arrive(&bars.kv_full[st]);
             load(next);
