@@ -121,9 +121,11 @@ struct KvFormat<FBLT_KV_INT8> {
         h23 = *reinterpret_cast<const uint32_t *>(&y);
     }
     static __device__ __forceinline__ uint32_t codes(float a, float b, float c, float d) {
-        const uint32_t i = (uint32_t)__float2int_rn(a) & 0xff, j = (uint32_t)__float2int_rn(b) & 0xff;
-        const uint32_t k = (uint32_t)__float2int_rn(c) & 0xff, l = (uint32_t)__float2int_rn(d) & 0xff;
-        return i | (j << 8) | (k << 16) | (l << 24);
+        // 1.5 * 2^23 + x rounds x to the nearest integer, ties to even, and has it in its low bits
+        const float o = 12582912.0f;
+        const uint32_t i = __byte_perm(__float_as_uint(a + o), __float_as_uint(b + o), 0x0040);
+        const uint32_t j = __byte_perm(__float_as_uint(c + o), __float_as_uint(d + o), 0x0040);
+        return __byte_perm(i, j, 0x5410);
     }
 };
 

@@ -3,7 +3,9 @@
 //
 // All three are one pass over the data: head_dim / 4 lanes hold one (row, head) in registers, four values each, so the
 // sum of squares and the largest magnitude are shuffles inside those lanes and nothing is read twice. What bounds
-// them is HBM (reading and writing every value once).
+// them is HBM (reading and writing every value once), as long as a value costs few instructions: lanes keep a head and
+// walk down the rows of their CTA, so that what belongs to the head (pointers, gains, the kind of work) is set up once
+// and a row costs additions (with a division per value group instead, the launch was bound by instruction issue).
 #include "paged.cuh"
 
 namespace fblt {
@@ -12,10 +14,9 @@ constexpr int kRowThreads = 256;
 constexpr int kMaxRows = 16; // rows of one CTA
 
 struct RowInfo {
-    int pos;  // < 0: the row is not to be touched
-    int page; // < 0: no page
-    int slot;
-    int b;
+    int64_t at; // row of head 0 in the pool (PagedView::row), < 0: no page
+    int pos;    // < 0: the row is not to be touched
+    int pad;
 };
 
 struct NormRopeParams {
@@ -32,136 +33,221 @@ struct NormRopeParams {
     const int32_t *cu, *base;    // append
 };
 
-// Sequence, position and page of a packed row: the last b with cu[b] <= r.
+// Sequence, position and page of packed row r, by a whole warp: the last b with cu[b] <= r is found 32 ways at a time
+// (three look-ups for 32 k sequences instead of fifteen). Every lane gets the answer.
 __device__ __forceinline__ RowInfo find_row(const PagedView &pv, const int32_t *cu, const int32_t *base, int batch, int total,
-                                            int r) {
+                                            int r, int lane) {
     RowInfo ri;
-    int lo = 0, hi = batch;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(cu + mid) <= r) lo = mid;
-        else hi = mid;
+    ri.pad = 0;
+    int lo = 0, n = batch; // the answer lies in [lo, lo + n)
+    {
+        // sequences of one length: the row says which one it is
+        const int at = (int)((int64_t)r * batch / total);
+        if (__ldg(cu + at) <= r && r < __ldg(cu + at + 1)) {
+            lo = at;
+            n = 1;
+        }
     }
-    ri.b = lo;
-    ri.pos = ri.page = -1;
-    ri.slot = 0;
-    int r0, n, p0;
-    if (!paged_seq(pv, cu, base, total, lo, r0, n, p0)) return ri;
-    if (r < r0 || r >= r0 + n) {
+    while (n > 1) {
+        const int step = (n + 31) >> 5, at = lo + lane * step;
+        const bool le = lane * step < n && __ldg(cu + at) <= r;
+        const int k = max(0, __popc(__ballot_sync(0xffffffffu, le)) - 1); // cu ascends: the lanes that say yes are the first ones
+        lo += k * step;
+        n = min(step, n - k * step);
+    }
+    ri.at = -1;
+    ri.pos = -1;
+    int r0, count, p0;
+    if (!paged_seq(pv, cu, base, total, lo, r0, count, p0)) return ri;
+    if (r < r0 || r >= r0 + count) {
         pv.raise(FBLT_PAGED_BAD_LENGTH);
         return ri;
     }
     ri.pos = p0 + (r - r0);
-    const int pi = ri.pos / pv.page_size;
-    ri.slot = ri.pos - pi * pv.page_size;
-    ri.page = pv.page(lo, pi);
-    if (ri.page < 0) pv.raise(FBLT_PAGED_BAD_PAGE);
+    const int pi = ri.pos / pv.page_size, page = pv.page(lo, pi);
+    if (page < 0) pv.raise(FBLT_PAGED_BAD_PAGE);
+    else ri.at = pv.row(page, 0, ri.pos - pi * pv.page_size);
     return ri;
 }
 
-template <int LANES>
-__device__ __forceinline__ float group_sum(float v) {
+// Sums and maxima over the lanes of one head; groups of a warp may be in different branches, so each names its own lanes.
+template <int LANES, class T>
+__device__ __forceinline__ T group_sum(uint32_t mask, T v) {
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
     return v;
 }
 template <int LANES>
-__device__ __forceinline__ float group_max(float v) {
+__device__ __forceinline__ float group_max(uint32_t mask, float v) {
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o));
     return v;
 }
 
-// FMT < 0: norm + rotation only. Otherwise units qh .. qh + kh are K, the next kh V, both quantised into the pages.
+// Four values of a lane into the codes of their row, whose exponent the group agrees on.
+template <int FMT, int LANES>
+__device__ __forceinline__ uint32_t quantise4(const PagedView &pv, uint32_t mask, const float (&v)[4], int &e, bool live) {
+    using F = KvFormat<FMT>;
+    const float top = (float)F::kQmax;
+    float a = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    const float odd = fmaf(v[0], 0.0f, v[1] * 0.0f) + fmaf(v[2], 0.0f, v[3] * 0.0f); // 0, or NaN
+    float w[4] = {v[0], v[1], v[2], v[3]};
+    const bool bad = !(odd == 0.0f);
+    if (bad) { // the exponent comes from the finite values; NaN becomes 0, an infinity the largest code
+        if (live) pv.raise(FBLT_PAGED_NONFINITE);
+        a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (finite_f(w[i])) a = fmaxf(a, fabsf(w[i]));
+            else if (isnan(w[i])) w[i] = 0.0f;
+        }
+    }
+    e = F::exponent(group_max<LANES>(mask, a));
+    const float s = exp2_int(-e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] *= s;
+    if (bad || e == F::kEmax) { // elsewhere |w| <= Qmax already
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = fminf(fmaxf(w[i], -top), top);
+    }
+    return F::codes(w[0], w[1], w[2], w[3]);
+}
+
+// The float that lies between a double's neighbours below and above it and is odd where the double is none: rounding it
+// once more, to fewer bits, gives what rounding the double would have given.
+__device__ __forceinline__ float round_odd(double d) {
+    const float f = __double2float_rz(d);
+    return (double)f == d || isnan(d) ? f : __int_as_float(__float_as_int(f) | 1);
+}
+
+// 1 / sqrt(a) to 2^-43: the single-precision estimate y (2^-22) and one step of Newton's iteration, y + y (1 - a y^2) / 2.
+__device__ __forceinline__ double rsqrt_43(double a) {
+    const double y = (double)rsqrtf((float)a);
+    return a > 1e-30 && a < 1e30 ? fma(0.5 * y, fma(-a * y, y, 1.0), y) : rsqrt(a);
+}
+
+// FMT < 0: norm + rotation only; the heads of K and of Q. Otherwise K, V (both quantised into the pages) and Q.
+// K rows that are normalised or rotated before they are quantised go through 64 bits: a code beside a border is decided
+// by the last bits of fp32, and this way it is the code of the definition.
 template <int HD, int FMT>
-__global__ void __launch_bounds__(kRowThreads) norm_rope_kernel(const NormRopeParams p) {
-    constexpr int LPH = HD / 4, GROUPS = kRowThreads / LPH, U = 2;
+__global__ void __launch_bounds__(kRowThreads, 4) norm_rope_kernel(const NormRopeParams p) {
+    constexpr int LPH = HD / 4, GROUPS = kRowThreads / LPH, U = FMT < 0 ? 4 : 2;
     constexpr bool APPEND = FMT >= 0;
-    using F = KvFormat<(FMT >= 0 ? FMT : 0)>;
     __shared__ RowInfo info[kMaxRows];
     const int tid = threadIdx.x;
     const int64_t row0 = (int64_t)blockIdx.x * p.rows_per_cta;
     const int nrows = (int)min((int64_t)p.rows_per_cta, p.rows - row0);
-    if (tid < nrows) {
-        if (APPEND) {
-            info[tid] = find_row(p.pv, p.cu, p.base, p.batch, (int)p.rows, (int)row0 + tid);
-        } else {
-            RowInfo ri;
-            ri.pos = p.pos ? p.pos[row0 + tid] : 0;
-            ri.page = ri.slot = ri.b = 0;
-            info[tid] = ri;
+    const int units = p.qh + (APPEND ? 2 : 1) * p.kh;
+    const int group = tid / LPH, lane = tid % LPH;
+    const uint32_t mask = LPH == 32 ? 0xffffffffu : ((1u << (LPH & 31)) - 1) << ((tid & 31) / LPH * LPH);
+    if (APPEND) {
+        for (int r = tid >> 5; r < nrows; r += kRowThreads / 32) {
+            const RowInfo ri = find_row(p.pv, p.cu, p.base, p.batch, (int)p.rows, (int)row0 + r, tid & 31);
+            if ((tid & 31) == 0) {
+                info[r] = ri;
+                if (p.cs && ri.pos >= p.rope_len) p.pv.raise(FBLT_PAGED_BAD_POSITION);
+            }
         }
-        if (p.cs && (info[tid].pos < 0 ? !APPEND : info[tid].pos >= p.rope_len)) p.pv.raise(FBLT_PAGED_BAD_POSITION);
+    } else if (tid < nrows) {
+        RowInfo ri;
+        ri.pos = p.pos ? p.pos[row0 + tid] : 0;
+        ri.at = ri.pad = 0;
+        info[tid] = ri;
+        if (p.cs && (ri.pos < 0 || ri.pos >= p.rope_len)) p.pv.raise(FBLT_PAGED_BAD_POSITION);
     }
     __syncthreads();
-    const int units = p.qh + (APPEND ? 2 : 1) * p.kh, items = nrows * units;
-    const int group = tid / LPH, lane = tid % LPH;
-    for (int it0 = 0; it0 < items; it0 += GROUPS * U) { // the same trip count for every lane of a warp
-        float4 x[U];
-        int row[U], unit[U];
+    const float2 *cs = reinterpret_cast<const float2 *>(p.cs) + lane, *sn = reinterpret_cast<const float2 *>(p.sn) + lane;
+    for (int unit = group; unit < units; unit += GROUPS) {
+        // K first, then V, then Q: the long way through 64 bits runs beside the others' work, not behind it
+        const int nkv = APPEND ? 2 * p.kh : p.kh;
+        const int kind = unit >= nkv ? 0 : unit < p.kh ? 1 : 2, head = unit - (kind == 0 ? nkv : kind == 1 ? 0 : p.kh);
+        const int64_t ss = kind == 0 ? p.qs : kind == 1 ? p.ks : p.vs, ds = kind == 0 ? p.qos : p.kos;
+        const float *src = (kind == 0 ? p.q : kind == 1 ? p.k : p.v) + row0 * ss + head * HD + lane * 4;
+        if (!APPEND || kind == 0) {
+            float *dst = (kind == 0 ? p.qo : p.ko) + row0 * ds + head * HD + lane * 4;
+            const float *gain = kind == 0 ? p.qg : p.kg;
+            const float4 g = gain ? __ldg(reinterpret_cast<const float4 *>(gain) + lane) : make_float4(1.f, 1.f, 1.f, 1.f);
+            for (int r = 0; r < nrows; r += U) {
+                float4 x[U];
+                float2 c[U], s[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int it = it0 + u * GROUPS + group;
-            row[u] = it < items ? it / units : 0;
-            unit[u] = it < items ? it - row[u] * units : -1;
-            if (APPEND && info[row[u]].pos < 0) unit[u] = -1;
-            x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (unit[u] >= 0) {
-                const int64_t r = row0 + row[u];
-                const float *src = unit[u] < p.qh                  ? p.q + r * p.qs + (int64_t)unit[u] * HD
-                                   : !APPEND || unit[u] < p.qh + p.kh ? p.k + r * p.ks + (int64_t)(unit[u] - p.qh) * HD
-                                                                   : p.v + r * p.vs + (int64_t)(unit[u] - p.qh - p.kh) * HD;
-                x[u] = *reinterpret_cast<const float4 *>(src + lane * 4);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool is_q = unit[u] < p.qh, is_v = APPEND && unit[u] >= p.qh + p.kh;
-            const float *gain = is_v ? nullptr : is_q ? p.qg : p.kg;
-            const float ss = group_sum<LPH>(x[u].x * x[u].x + x[u].y * x[u].y + (x[u].z * x[u].z + x[u].w * x[u].w));
-            if (gain) {
-                const float inv = __frsqrt_rn(ss * (1.0f / HD) + p.eps);
-                const float4 g = __ldg(reinterpret_cast<const float4 *>(gain) + lane);
-                x[u].x *= inv * g.x;
-                x[u].y *= inv * g.y;
-                x[u].z *= inv * g.z;
-                x[u].w *= inv * g.w;
-            }
-            const int pos = info[row[u]].pos;
-            if (p.cs && !is_v && unit[u] >= 0 && pos >= 0 && pos < p.rope_len)
-                x[u] = rope_rotate4(x[u], p.cs, p.sn, pos, HD / 2, lane * 2);
-            if (!APPEND || is_q) {
-                if (unit[u] >= 0) {
-                    const int64_t r = row0 + row[u];
-                    float *dst = is_q ? p.qo + r * p.qos + (int64_t)unit[u] * HD : p.ko + r * p.kos + (int64_t)(unit[u] - p.qh) * HD;
-                    *reinterpret_cast<float4 *>(dst + lane * 4) = x[u];
-                }
-            }
-            if (APPEND) {
-                // 0 for what is not finite: the exponent comes from the finite values
-                const float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-                float a = 0.0f;
-                bool odd = false;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (finite_f(v[i])) a = fmaxf(a, fabsf(v[i]));
-                    else odd = true;
-                }
-                const int e = F::exponent(group_max<LPH>(a));
-                if (unit[u] >= 0 && !is_q) {
-                    if (odd) p.pv.raise(FBLT_PAGED_NONFINITE);
-                    const RowInfo ri = info[row[u]];
-                    if (ri.page >= 0) {
-                        const float s = exp2_int(-e), top = (float)F::kQmax;
-                        float y[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) y[i] = isnan(v[i]) ? 0.0f : fminf(fmaxf(v[i] * s, -top), top);
-                        const int64_t at = p.pv.row(ri.page, unit[u] - p.qh - (is_v ? p.kh : 0), ri.slot);
-                        uint8_t *code = (is_v ? p.pv.vc : p.pv.kc) + at * HD + lane * 4;
-                        *reinterpret_cast<uint32_t *>(code) = F::codes(y[0], y[1], y[2], y[3]);
-                        if (lane == 0) (is_v ? p.pv.ve : p.pv.ke)[at] = (int8_t)e;
+                for (int u = 0; u < U; ++u) {
+                    if (r + u >= nrows) break;
+                    x[u] = *reinterpret_cast<const float4 *>(src + (int64_t)u * ss);
+                    const int pos = info[r + u].pos;
+                    if (p.cs && (unsigned)pos < (unsigned)p.rope_len) {
+                        c[u] = __ldg(cs + (int64_t)pos * (HD / 4));
+                        s[u] = __ldg(sn + (int64_t)pos * (HD / 4));
                     }
                 }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (r + u >= nrows) break;
+                    const int pos = info[r + u].pos;
+                    if (gain) {
+                        const float sum = group_sum<LPH>(mask, x[u].x * x[u].x + x[u].y * x[u].y + (x[u].z * x[u].z + x[u].w * x[u].w));
+                        const float inv = rsqrtf(fmaf(sum, 1.0f / HD, p.eps));
+                        x[u] = make_float4(x[u].x * (inv * g.x), x[u].y * (inv * g.y), x[u].z * (inv * g.z), x[u].w * (inv * g.w));
+                    }
+                    if (p.cs && (unsigned)pos < (unsigned)p.rope_len) {
+                        rope_rotate(x[u].x, x[u].y, c[u].x, s[u].x);
+                        rope_rotate(x[u].z, x[u].w, c[u].y, s[u].y);
+                    }
+                    if (!APPEND || pos >= 0) *reinterpret_cast<float4 *>(dst + (int64_t)u * ds) = x[u];
+                }
+                src += (int64_t)U * ss;
+                dst += (int64_t)U * ds;
+            }
+        }
+        if constexpr (APPEND) {
+            if (kind == 0) continue;
+            uint8_t *codes = (kind == 1 ? p.pv.kc : p.pv.vc) + lane * 4;
+            int8_t *exps = kind == 1 ? p.pv.ke : p.pv.ve;
+            const int64_t skip = (int64_t)head * p.pv.page_size; // from head 0's row of a page to this head's
+            const bool norm = kind == 1 && p.kg, rope = kind == 1 && p.cs;
+            double g[4] = {1.0, 1.0, 1.0, 1.0};
+            if (norm) {
+                const float4 f = __ldg(reinterpret_cast<const float4 *>(p.kg) + lane);
+                g[0] = f.x, g[1] = f.y, g[2] = f.z, g[3] = f.w;
+            }
+            for (int r = 0; r < nrows; r += U) {
+                float4 x[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (r + u < nrows) x[u] = *reinterpret_cast<const float4 *>(src + (int64_t)u * ss);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (r + u >= nrows) break;
+                    const RowInfo ri = info[r + u];
+                    float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+                    if (norm || rope) {
+                        double d[4] = {v[0], v[1], v[2], v[3]};
+                        if (norm) {
+                            const double sum = group_sum<LPH>(mask, d[0] * d[0] + d[1] * d[1] + (d[2] * d[2] + d[3] * d[3]));
+                            const double inv = rsqrt_43(sum * (1.0 / HD) + (double)p.eps);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) d[i] *= inv * g[i];
+                        }
+                        if (rope && (unsigned)ri.pos < (unsigned)p.rope_len) {
+                            const float2 c = __ldg(cs + (int64_t)ri.pos * (HD / 4)), s = __ldg(sn + (int64_t)ri.pos * (HD / 4));
+                            const double a = d[0], b = d[2];
+                            d[0] = a * (double)c.x - d[1] * (double)s.x;
+                            d[1] = d[1] * (double)c.x + a * (double)s.x;
+                            d[2] = b * (double)c.y - d[3] * (double)s.y;
+                            d[3] = d[3] * (double)c.y + b * (double)s.y;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = round_odd(d[i]);
+                    }
+                    int e;
+                    const uint32_t w = quantise4<FMT, LPH>(p.pv, mask, v, e, ri.pos >= 0);
+                    if (ri.at >= 0) {
+                        const int64_t at = ri.at + skip;
+                        *reinterpret_cast<uint32_t *>(codes + at * HD) = w;
+                        if (lane == 0) exps[at] = (int8_t)e;
+                    }
+                }
+                src += (int64_t)U * ss;
             }
         }
     }
@@ -177,50 +263,55 @@ struct ReadParams {
 
 template <int HD, int FMT, bool BF16>
 __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(const ReadParams p) {
-    constexpr int LPH = HD / 4, GROUPS = kRowThreads / LPH, U = 4;
+    constexpr int LPH = HD / 4, GROUPS = kRowThreads / LPH, U = 8;
     __shared__ RowInfo info[kMaxRows];
     const int tid = threadIdx.x;
     const int64_t row0 = (int64_t)blockIdx.x * p.rows_per_cta;
     const int nrows = (int)min((int64_t)p.rows_per_cta, p.rows - row0);
-    if (tid < nrows) info[tid] = find_row(p.pv, p.cu, p.start, p.batch, p.rows, (int)row0 + tid);
+    for (int r = tid >> 5; r < nrows; r += kRowThreads / 32) {
+        const RowInfo ri = find_row(p.pv, p.cu, p.start, p.batch, p.rows, (int)row0 + r, tid & 31);
+        if ((tid & 31) == 0) info[r] = ri;
+    }
     __syncthreads();
-    const int kh = p.pv.kvh, skip = p.ko ? 0 : kh, units = (p.ko && p.vo ? 2 : 1) * kh, items = nrows * units;
-    const int group = tid / LPH, lane = tid % LPH;
-    for (int it0 = group; it0 < items; it0 += GROUPS * U) {
-        uint32_t w[U];
-        int row[U], unit[U], e[U];
+    const int kh = p.pv.kvh, units = (p.ko && p.vo ? 2 : 1) * kh, group = tid / LPH, lane = tid % LPH;
+    for (int unit = group; unit < units; unit += GROUPS) {
+        const bool is_v = !p.ko || unit >= kh;
+        const int head = unit >= kh ? unit - kh : unit;
+        const int64_t skip = (int64_t)head * p.pv.page_size, ds = is_v ? p.vos : p.kos;
+        const uint8_t *codes = (is_v ? p.pv.vc : p.pv.kc) + skip * HD + lane * 4;
+        const int8_t *exps = (is_v ? p.pv.ve : p.pv.ke) + skip;
+        int64_t to = row0 * ds + head * HD + lane * 4;
+        void *dst = is_v ? p.vo : p.ko;
+        for (int r = 0; r < nrows; r += U) {
+            uint32_t w[U];
+            int e[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int it = it0 + u * GROUPS;
-            row[u] = it < items ? it / units : 0;
-            unit[u] = it < items ? it - row[u] * units + skip : -1;
-            const RowInfo ri = info[row[u]];
-            if (ri.pos < 0) unit[u] = -1;
-            w[u] = 0;
-            e[u] = 0;
-            if (unit[u] >= 0 && ri.page >= 0) {
-                const bool is_v = unit[u] >= kh;
-                const int64_t at = p.pv.row(ri.page, unit[u] - (is_v ? kh : 0), ri.slot);
-                w[u] = *reinterpret_cast<const uint32_t *>((is_v ? p.pv.vc : p.pv.kc) + at * HD + lane * 4);
-                e[u] = (is_v ? p.pv.ve : p.pv.ke)[at];
+            for (int u = 0; u < U; ++u) {
+                if (r + u >= nrows) break;
+                const int64_t at = info[r + u].at;
+                w[u] = 0;
+                e[u] = 0;
+                if (at >= 0) {
+                    w[u] = *reinterpret_cast<const uint32_t *>(codes + at * HD);
+                    e[u] = exps[at];
+                }
             }
-        }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (unit[u] < 0) continue;
-            const bool is_v = unit[u] >= kh;
-            const int64_t at = (row0 + row[u]) * (is_v ? p.vos : p.kos) + (int64_t)(unit[u] - (is_v ? kh : 0)) * HD + lane * 4;
-            const float4 x = kv_values<FMT>(w[u], kv_scale<FMT>(e[u]));
-            void *dst = is_v ? p.vo : p.ko;
-            if (BF16) {
-                const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x, x.y), hi = __floats2bfloat162_rn(x.z, x.w);
-                uint2 o;
-                o.x = *reinterpret_cast<const uint32_t *>(&lo);
-                o.y = *reinterpret_cast<const uint32_t *>(&hi);
-                *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(dst) + at) = o;
-            } else {
-                *reinterpret_cast<float4 *>(static_cast<float *>(dst) + at) = x;
+            for (int u = 0; u < U; ++u) {
+                if (r + u >= nrows) break;
+                if (info[r + u].pos < 0) continue;
+                const float4 x = kv_values<FMT>(w[u], kv_scale<FMT>(e[u]));
+                if (BF16) {
+                    const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x, x.y), hi = __floats2bfloat162_rn(x.z, x.w);
+                    uint2 o;
+                    o.x = *reinterpret_cast<const uint32_t *>(&lo);
+                    o.y = *reinterpret_cast<const uint32_t *>(&hi);
+                    *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(dst) + to + (int64_t)u * ds) = o;
+                } else {
+                    *reinterpret_cast<float4 *>(static_cast<float *>(dst) + to + (int64_t)u * ds) = x;
+                }
             }
+            to += (int64_t)U * ds;
         }
     }
 }
@@ -229,7 +320,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(const ReadParam
 // and the loop has loads to overlap).
 static int rows_per_cta(int64_t rows) {
     const int64_t r = rows / (148 * 16);
-    return r < 1 ? 1 : r > 8 ? 8 : (int)r;
+    return r < 1 ? 1 : r > kMaxRows ? kMaxRows : (int)r;
 }
 
 static bool aligned16(const void *p) { return !(((uintptr_t)p) & 15); }

@@ -83,10 +83,10 @@ def norm_rope(x, gain, eps, cos, sin, pos):
 
 
 def norm_rope_tol(y: torch.Tensor) -> torch.Tensor:
-    """Bound of the fp32 error at y [..., hd] (float64 result). The sum of squares is a tree of at most 9 roundings
-    per term, halved by the root; its rsqrt, the products with the gain and the value round four times: 9 * 2^-24
-    relative. The rotation adds a product and a sum, 2 * 2^-24 of |y0 c| + |y1 s| <= sqrt(2) hypot: 16 * 2^-24 of
-    the pair's length covers both."""
+    """Bound of the fp32 error at y [..., hd] (float64 result). The sum of squares is a tree of at most 9 roundings per
+    term, with the mean and eps 11, halved by the root: 5.5 * 2^-24 relative; rsqrt is off by at most 2 units of the last
+    place, 4 * 2^-24, and two products round: 11.5 * 2^-24. The rotation adds a product and a sum, 2 * 2^-24 of
+    |y0 c| + |y1 s| <= sqrt(2) hypot: 16 * 2^-24 of the pair's length covers both."""
     h = torch.sqrt(y[..., 0::2] ** 2 + y[..., 1::2] ** 2)
     return 16 * U24 * torch.repeat_interleave(h, 2, dim=-1) + 1e-37
 

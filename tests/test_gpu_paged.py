@@ -242,8 +242,13 @@ def test_append_with_norm_and_rotation(cuda_lib, fmt, hd, heads, kv):
     assert ((q.reshape(rows, heads, hd).double().cpu() - wq).abs() <= R.norm_rope_tol(wq)).all()
     wk = R.norm_rope(was[:, heads * hd:(heads + kv) * hd].reshape(rows, kv, hd), kg, eps, cos, sin, pos)
     wv = was[:, (heads + kv) * hd:].reshape(rows, kv, hd).double().cpu()
+    kc, ke = R.quantise(wk.numpy().reshape(-1, hd), fmt)  # the definition's codes: K goes through 64 bits
+    kc, ke = kc.reshape(rows, kv, hd), ke.reshape(rows, kv)
     r = 0
     for b, (n, p) in enumerate(zip(new, base)):
+        for i in range(n):
+            pg, slot = int(c.page_table[b, (p + i) // page]), (p + i) % page
+            assert (c.k_codes[pg, :, slot].cpu().numpy() == kc[r + i]).all() and (c.k_exp[pg, :, slot].cpu().numpy() == ke[r + i]).all()
         for want, codes, exp, tol in ((wk, c.k_codes, c.k_exp, R.norm_rope_tol(wk)), (wv, c.v_codes, c.v_exp, torch.zeros_like(wv))):
             for i in range(n):
                 pg, slot = int(c.page_table[b, (p + i) // page]), (p + i) % page
