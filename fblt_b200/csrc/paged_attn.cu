@@ -8,8 +8,9 @@
 //
 //   * CTA = (sequence, kv head, key range, tile of query rows); the rows of one kv head are its G query heads of every
 //     new token, so grouped heads and drafted blocks read a key once.
-//   * A producer warp copies stages of 64 keys (four groups of 16, each inside one page) into a ring with untiled
-//     bulk copies; group i lies 32 bytes further round the banks than group i - 1.
+//   * Stages of 64 keys (head_dim 128: 32), four groups that lie in one page each, are copied ahead into shared memory:
+//     by every warp for itself, or, where warps share the keys, by a producer warp; group i lies 32 bytes further round
+//     the banks than group i - 1.
 //   * Four consumer warps multiply with mma.sync m16n8k16 in fp16: codes ARE halves (an 8-bit code has at most 8
 //     significant bits), and the 16 rows of the A operand are 8 query rows in two planes, q = hi + lo with 22 bits
 //     in all, so q . code is fp32 class in ONE instruction and hi + lo are added in registers. Probabilities go back
@@ -25,7 +26,6 @@ namespace fblt {
 
 __device__ unsigned int g_paged_error; // 0 = ok; otherwise (code << 24) | blockIdx.x of the first CTA that gave up
 
-constexpr int kPsThreads = 160;
 // A row's weights times the scales of V, p 2^ev, are put into halves in units of 2^(R - kPsHead), R within four of the
 // largest exponent that p 2^ev has had (R follows the row's maximum when that moves): at most 2^(kPsHead + 5), and what
 // is 2^-24 of the largest still has 11 bits, however unequal the rows of V are.
@@ -41,8 +41,8 @@ struct PsShape {
     static constexpr int kGroup = kPer * HD;            // their bytes
     static constexpr int kPitch = kGroup + 32;          // see the bank skew above
     static constexpr int kOffV = 4 * kPitch, kOffE = 8 * kPitch;
-    static constexpr int kStage = 8 * kPitch + 2 * kKeys + (HD == 128 ? 64 : 0); // K groups, V groups, exponents
-    static constexpr int kStages = 8;
+    static constexpr int kStage = 8 * kPitch + 128; // K groups, V groups, exponents
+    static constexpr int kStages = 8; // of the CTA; a warp's own: kStages / 4
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
@@ -61,7 +61,7 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 template <int HD, int FMT, int RB, int WR>
-__global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(WR == 1 ? 128 : 160) paged_stream_kernel(const PagedAttnParams p) {
     using F = KvFormat<FMT>;
     using S = PsShape<HD>;
     constexpr int WK = 4 / WR, RT = 8 * RB * WR, KS = HD / 16, NB = HD / 8, PR = HD + 4, NS = S::kStages;
@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem;
     uint4 *sq = reinterpret_cast<uint4 *>(smem + NS * S::kStage); // [RB * WR][KS][32] A fragments
-    __shared__ uint64_t full[NS], empty[NS];
+    __shared__ uint64_t full[NS], empty[NS]; // WR > 1
     __shared__ uint32_t vmask[NS];
     __shared__ float crow[RT], sm[WK * RT], sl[WK * RT];
     __shared__ __align__(16) float scale[4][2][S::kKeys]; // a warp's own: the stage's scales of K and of V
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
     const int st0 = min(stages, split * per), nst = min(stages, st0 + per) - st0;
     const int kb0 = first + st0 * S::kKeys;
 
-    if (tid == 0) {
+    if (WR > 1 && tid == 0) {
         for (int i = 0; i < NS; ++i) {
             mbar_init(&full[i], 33);
             mbar_init(&empty[i], WR);
@@ -99,23 +99,24 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
+    // Rows of the pool where this lane's group begins, -1: not there. Eight stages at a time, a lane per group: stage
+    // first + every * (lane / 4), group lane % 4.
+    auto look = [&](int first, int every) -> int64_t {
+        const int st = first + every * (lane >> 2), key = kb0 + st * S::kKeys + (lane & 3) * S::kPer;
+        if (st >= nst || key >= rr.hi) return -1;
+        const int pi = key / p.pv.page_size, page = p.pv.page(b, pi);
+        if (page < 0) p.pv.raise(FBLT_PAGED_BAD_PAGE);
+        return page < 0 ? -1 : p.pv.row(page, kvh, key - pi * p.pv.page_size);
+    };
 
-    if (warp == 4) {
-        // ---- producer: 16 bytes a lane and copy; pages are looked up eight stages (a lane per group) at a time, one
-        // look-up ahead
-        auto look = [&](int st) -> int64_t {
-            const int key = kb0 + (st + (lane >> 2)) * S::kKeys + (lane & 3) * S::kPer;
-            if (st + (lane >> 2) >= nst || key >= rr.hi) return -1;
-            const int pi = key / p.pv.page_size, page = p.pv.page(b, pi);
-            if (page < 0) p.pv.raise(FBLT_PAGED_BAD_PAGE);
-            return page < 0 ? -1 : p.pv.row(page, kvh, key - pi * p.pv.page_size);
-        };
-        int64_t now = -1, next = look(0);
+    if (WR > 1 && warp == 4) {
+        // ---- producer; pages are looked up eight stages ahead
+        int64_t now = -1, next = look(0, 1);
         for (int st = 0; st < nst; ++st) {
             const int slot = st % NS;
             if ((st & 7) == 0) {
                 now = next;
-                next = look(st + 8);
+                next = look(st + 8, 1);
             }
             const int64_t at = __shfl_sync(0xffffffffu, now, (st & 7) * 4 + (lane & 3));
             const uint32_t ok = __ballot_sync(0xffffffffu, at >= 0) & 15;
@@ -131,26 +132,21 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
                 }
             }
             uint8_t *stage = ring + slot * S::kStage;
-#pragma unroll
-            for (int gi = 0; gi < 4; ++gi) {
-                const int64_t row = __shfl_sync(0xffffffffu, at, gi);
-                if (!((ok >> gi) & 1)) continue;
-                const uint8_t *ksrc = p.pv.kc + row * HD + lane * 16, *vsrc = p.pv.vc + row * HD + lane * 16;
-                uint8_t *kdst = stage + gi * S::kPitch + lane * 16;
-#pragma unroll
-                for (int c = 0; c < S::kGroup; c += 512) {
-                    cp_async_16(kdst + c, ksrc + c);
-                    cp_async_16(kdst + S::kOffV + c, vsrc + c);
-                }
-                if (lane < S::kPer / 4) // K's exponents, then V's, eight at a time
-                    cp_async_8(stage + S::kOffE + (lane & 1) * S::kKeys + gi * S::kPer + (lane >> 1) * 8,
-                               ((lane & 1) ? p.pv.ve : p.pv.ke) + row + (lane >> 1) * 8);
-            }
-            cp_async_arrive(&full[slot]); // one arrival a lane, when its copies have landed
             if (lane == 0) {
                 vmask[slot] = ok;
-                mbar_arrive(&full[slot]);
+                mbar_expect_tx(&full[slot], __popc(ok) * 2 * S::kGroup);
             }
+            __syncwarp();
+            // lane = (group, K / V): its codes as one bulk copy, its exponents in eights
+            const int64_t row = __shfl_sync(0xffffffffu, at, (lane >> 1) & 3);
+            if (lane < 8 && row >= 0) {
+                const int gi = lane >> 1, v = lane & 1;
+                bulk_load(stage + v * S::kOffV + gi * S::kPitch, (v ? p.pv.vc : p.pv.kc) + row * HD, S::kGroup, &full[slot]);
+#pragma unroll
+                for (int k = 0; k < S::kPer; k += 8)
+                    cp_async_8(stage + S::kOffE + v * S::kKeys + gi * S::kPer + k, (v ? p.pv.ve : p.pv.ke) + row + k);
+            }
+            cp_async_arrive(&full[slot]); // one arrival a lane, when its exponents have landed
         }
         asm volatile("cp.async.wait_all;" ::: "memory"); // nothing is in flight when the CTA goes
     } else {
@@ -222,16 +218,8 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
         };
         const uint4 *myq = sq + wr * RB * KS * 32 + lane;
         float(&kscale)[S::kKeys] = scale[warp][0], (&vscale)[S::kKeys] = scale[warp][1];
-        for (int st = wk; st < nst; st += WK) { // a stage belongs to the WR warps of one key share
-            const int slot = st % NS;
-            if (!mbar_wait_abort(&full[slot], (st / NS) & 1, (const volatile int *)&s_abort)) {
-                *(volatile int *)&s_abort = 1;
-                if (lane == 0) atomicCAS(&g_paged_error, 0u, (0x42u << 24) | (blockIdx.x & 0xffffffu));
-                break;
-            }
-            const uint8_t *stage = ring + slot * S::kStage;
-            const int kb = kb0 + st * S::kKeys;
-            const uint32_t here = vmask[slot];
+        // one stage: keys kb .., groups `here` of it have landed
+        auto work = [&](uint8_t *stage, int kb, uint32_t here) {
             const bool there = (here >> t) & 1; // this lane's scores and V rows are keys of group t
             // every key of the stage is there and every row of the warp sees it
             const bool whole = __all_sync(0xffffffffu, here == 15 && kb >= lo[0] && kb + S::kKeys <= lo[0] + span[0] &&
@@ -242,7 +230,7 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
                 for (int i = lane; i < S::kKeys * (HD / 16); i += 32) {
                     const int k = i / (HD / 16), grp = k / S::kPer;
                     if (kb + k < rr.lo || kb + k >= rr.hi || !((here >> grp) & 1))
-                        *reinterpret_cast<uint4 *>(ring + slot * S::kStage + S::kOffV + grp * S::kPitch + (k % S::kPer) * HD + (i % (HD / 16)) * 16) =
+                        *reinterpret_cast<uint4 *>(stage + S::kOffV + grp * S::kPitch + (k % S::kPer) * HD + (i % (HD / 16)) * 16) =
                             make_uint4(0, 0, 0, 0);
                 }
             }
@@ -450,8 +438,63 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
                 }
             }
             if (++held == kPsFold / S::kKeys) fold();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[slot]);
+        };
+        if constexpr (WR == 1) {
+            // The warp copies its own stages (wk, wk + 4, ..): sixteen bytes a lane and copy, two stages in turn. One producer
+            // for all four warps spent 1450 clocks a stage on issuing them, half of what a warp spends on using one.
+            uint8_t *mine = ring + warp * (NS / 4) * S::kStage;
+            const int count = (nst - wk + 3) / 4;
+            int64_t now = -1, next = look(wk, 4);
+            uint32_t flying = 0; // groups of stage i at bits 4 (i % 2) ..
+            auto fetch = [&](int i) { // i ascends by one
+                if ((i & 7) == 0) {
+                    now = next;
+                    next = look(wk + 4 * (i + 8), 4);
+                }
+                const int64_t at = __shfl_sync(0xffffffffu, now, (i & 7) * 4 + (lane & 3));
+                const uint32_t ok = i < count ? __ballot_sync(0xffffffffu, at >= 0) & 15 : 0;
+                flying = (flying & ~(15u << 4 * (i & 1))) | ok << 4 * (i & 1);
+                uint8_t *stage = mine + (i & 1) * S::kStage;
+#pragma unroll
+                for (int gi = 0; gi < 4; ++gi) {
+                    const int64_t row = __shfl_sync(0xffffffffu, at, gi);
+                    if (!((ok >> gi) & 1)) continue;
+                    const uint8_t *ksrc = p.pv.kc + row * HD + lane * 16, *vsrc = p.pv.vc + row * HD + lane * 16;
+                    uint8_t *kdst = stage + gi * S::kPitch + lane * 16;
+#pragma unroll
+                    for (int c = 0; c < S::kGroup; c += 512) {
+                        cp_async_16(kdst + c, ksrc + c);
+                        cp_async_16(kdst + S::kOffV + c, vsrc + c);
+                    }
+                    if (lane < S::kPer / 4) // K's exponents, then V's, eight at a time
+                        cp_async_8(stage + S::kOffE + (lane & 1) * S::kKeys + gi * S::kPer + (lane >> 1) * 8,
+                                   ((lane & 1) ? p.pv.ve : p.pv.ke) + row + (lane >> 1) * 8);
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            static_assert(NS / 4 == 2, "two stages a warp");
+            fetch(0);
+            fetch(1);
+            for (int i = 0; i < count; ++i) {
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                __syncwarp();
+                work(mine + (i & 1) * S::kStage, kb0 + (wk + 4 * i) * S::kKeys, (flying >> 4 * (i & 1)) & 15);
+                __syncwarp();
+                fetch(i + 2);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else {
+            for (int st = wk; st < nst; st += WK) { // a stage belongs to the WR warps of one key share
+                const int slot = st % NS;
+                if (!mbar_wait_abort(&full[slot], (st / NS) & 1, (const volatile int *)&s_abort)) {
+                    *(volatile int *)&s_abort = 1;
+                    if (lane == 0) atomicCAS(&g_paged_error, 0u, (0x42u << 24) | (blockIdx.x & 0xffffffu));
+                    break;
+                }
+                work(ring + slot * S::kStage, kb0 + st * S::kKeys, vmask[slot]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[slot]);
+            }
         }
         fold();
         // ---- the warps' shares of the keys meet in shared memory (every copy has landed: the ring is free)
@@ -481,7 +524,7 @@ __global__ void __launch_bounds__(kPsThreads) paged_stream_kernel(const PagedAtt
                 }
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (*(volatile int *)&s_abort) return;
+        if (WR > 1 && *(volatile int *)&s_abort) return;
         for (int it = tid; it < RT * (HD / 4); it += 128) {
             const int ri = it / (HD / 4), d = (it - ri * (HD / 4)) * 4, r = row0 + ri;
             if (r >= rows) continue;
@@ -625,7 +668,7 @@ static int launch_stream_t(const PagedAttnParams &p, cudaStream_t s) {
     static_assert(4 / WR * 8 * RB * WR * (HD + 4) * 4 <= smem, "the merge area fits the ring");
     FBLT_CUDA_TRY(cudaFuncSetAttribute(paged_stream_kernel<HD, FMT, RB, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const dim3 grid((unsigned)p.pv.kvh, (unsigned)p.splits, (unsigned)(p.batch * p.row_tiles));
-    paged_stream_kernel<HD, FMT, RB, WR><<<grid, kPsThreads, smem, s>>>(p);
+    paged_stream_kernel<HD, FMT, RB, WR><<<grid, WR == 1 ? 128 : 160, smem, s>>>(p);
     count_launch();
     return check_launch("paged_stream_kernel");
 }

@@ -31,9 +31,13 @@ def _ptr(t) -> Optional[int]:
     raise TypeError(type(t))
 
 
+# the current stream's handle without an object around it (a microsecond of a decode step's call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _stream_ptr(stream) -> Optional[int]:
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream or None
+        return _raw_stream(torch.cuda.current_device()) or None
     if isinstance(stream, torch.cuda.Stream):
         return stream.cuda_stream or None
     return stream
