@@ -34,7 +34,8 @@ struct PcShape {
     static constexpr int kQPlane = HD == 128 ? kPcRows * HD * 2 : 0, kKv = BN * HD * 2;
     static constexpr int kOffKv = 2 * kQPlane; // head_dim 128: the second plane of Q of both tiles
     static constexpr int kOffSum = kOffKv + 4 * kKv; // head_dim 32, 64: folded sums, see the softmax
-    static constexpr int kSmem = kOffSum + (HD == 128 ? 0 : 2 * kPcRows * HD * 4);
+    // (and, before and after the loop, rows on their way between memory and the threads: 4 KB a warp, Q's planes whole)
+    static constexpr int kSmem = kOffSum + 2 * kPcRows * (HD == 128 ? 64 : HD) * 4;
     // TMEM columns of a query tile: S / P, O; behind both tiles the planes of Q
     static constexpr int kO = BN, kTile = BN + HD, kQCols = HD / 2, kQTile = HD == 128 ? kQCols : 2 * kQCols, kQ = 2 * kTile;
     static_assert(kQ + 2 * kQTile <= 512, "TMEM");
@@ -103,6 +104,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
     __shared__ __align__(16) int top_of[2][4]; // largest exponent of the tile's K, of its V; whether each is too wide for its halves
     __shared__ int4 range[2][4];
     __shared__ __align__(8) uint8_t present[2][8]; // groups of 16 keys whose page exists and that the CTA reads
+    __shared__ int q_exp[2][kPcRows]; // power of two of a query row; + 4096 where a value of it is not finite
     __shared__ uint32_t tmem_slot;
     __shared__ int s_abort;
     const volatile int *abortp = &s_abort;
@@ -161,44 +163,71 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             const int lo = !p.block_mode && p.window > 0 ? max(0, pos - p.window + 1) : 0;
             const int span = hi - lo;
             const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16) + T * S::kTile;
-            // ---- query planes: q scale log2(e) 2^e with the row's largest value in [2^13, 2^14)
+            // ---- query planes: q scale log2(e) 2^e with the row's largest value in [2^13, 2^14). Rows come in whole (HD / 4
+            // lanes each; a thread that read its own row took 20 to 40 thousand clocks), the planes go through shared
+            // memory to the threads that own them, 16-byte units exchanged within a row so that columns are free of conflicts.
             int qe; // the row of Q was multiplied by 2^qe
-            bool qbad = false; // a query value that is not finite
+            bool qbad; // a query value that is not finite
             {
-                const float *src = p.q + (int64_t)(r0 + i) * p.qs + (int64_t)head * HD;
-                float a = 0.0f;
-#pragma unroll 4
-                for (int d = 0; d < HD; d += 4) {
-                    const float4 v = *reinterpret_cast<const float4 *>(src + d);
-                    const float w[4] = {v.x * p.qscale, v.y * p.qscale, v.z * p.qscale, v.w * p.qscale};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (finite_f(w[k])) a = fmaxf(a, fabsf(w[k]));
-                        else qbad = true;
-                    }
-                }
-                qe = min(13 - ((__float_as_int(a) >> 23) - 127), 126);
-                const float up = exp2_int(qe);
-                const uint32_t tq = tmem + ((uint32_t)((warp & 3) * 32) << 16) + S::kQ + T * S::kQTile;
+                constexpr int LPR = HD / 4, RPI = 32 / LPR, UNITS = HD / 8, B = 8; // lanes a row, rows an instruction, units a row
+                uint8_t *hold = smem + S::kOffSum + T * kPcRows * (HD == 128 ? 64 : HD) * 4; // first plane, then (HD <= 64) the second
+                const int q4 = lane % LPR;
 #pragma unroll 1
-                for (int c = 0; c < HD / 32; ++c) {
-                    uint32_t h[16], lw[16];
+                for (int it = 0; it < 32 / RPI; it += B) {
+                    float4 v[B];
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4) {
-                        const float4 v = *reinterpret_cast<const float4 *>(src + c * 32 + k);
-                        split_half2(v.x * p.qscale * up, v.y * p.qscale * up, h[k / 2], lw[k / 2]);
-                        split_half2(v.z * p.qscale * up, v.w * p.qscale * up, h[k / 2 + 1], lw[k / 2 + 1]);
+                    for (int k = 0; k < B; ++k) {
+                        const int rr_ = min(row0 + T * kPcRows + (warp & 3) * 32 + (it + k) * RPI + lane / LPR, rows - 1), ii = rr_ / p.G;
+                        if (it + k < 32 / RPI)
+                            v[k] = *reinterpret_cast<const float4 *>(p.q + (int64_t)(r0 + ii) * p.qs +
+                                                                     (int64_t)(kvh * p.G + (rr_ - ii * p.G)) * HD + q4 * 4);
                     }
-                    tmem_st16(tq + c * 16, h);
-                    if (HD == 128) { // K-major core matrices
-                        uint8_t *dst = smem + T * S::kQPlane + rl * 16 + c * 4 * (kPcRows * 16);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            *reinterpret_cast<uint4 *>(dst + k * (kPcRows * 16)) = make_uint4(lw[4 * k], lw[4 * k + 1], lw[4 * k + 2], lw[4 * k + 3]);
-                    } else {
-                        tmem_st16(tq + S::kQCols + c * 16, lw);
+                    for (int k = 0; k < B; ++k) {
+                        if (it + k >= 32 / RPI) break;
+                        const int row = (warp & 3) * 32 + (it + k) * RPI + lane / LPR;
+                        const float w[4] = {v[k].x * p.qscale, v[k].y * p.qscale, v[k].z * p.qscale, v[k].w * p.qscale};
+                        float a = 0.0f;
+                        bool odd = false;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (finite_f(w[e])) a = fmaxf(a, fabsf(w[e]));
+                            else odd = true;
+                        }
+#pragma unroll
+                        for (int o = LPR / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+                        const uint32_t odds = __ballot_sync(0xffffffffu, odd);
+                        const int e = min(13 - ((__float_as_int(a) >> 23) - 127), 126);
+                        const float up = exp2_int(e);
+                        uint2 h, l;
+                        split_half2(w[0] * up, w[1] * up, h.x, l.x);
+                        split_half2(w[2] * up, w[3] * up, h.y, l.y);
+                        const int at = row * (HD * 2) + (((q4 >> 1) ^ (row & 7 & (UNITS - 1))) * 16) + (q4 & 1) * 8;
+                        *reinterpret_cast<uint2 *>(hold + at) = h;
+                        if (HD == 128) // K-major core matrices
+                            *reinterpret_cast<uint2 *>(smem + T * S::kQPlane + (q4 >> 1) * (kPcRows * 16) + row * 16 + (q4 & 1) * 8) = l;
+                        else
+                            *reinterpret_cast<uint2 *>(hold + kPcRows * HD * 2 + at) = l;
+                        if (q4 == 0) q_exp[T][row] = e + ((odds >> (lane / LPR * LPR)) & (LPR == 32 ? 0xffffffffu : (1u << (LPR & 31)) - 1) ? 4096 : 0);
                     }
                 }
+                __syncwarp();
+                qbad = q_exp[T][rl] > 2048;
+                qe = q_exp[T][rl] - (qbad ? 4096 : 0);
+                const uint32_t tq = tmem + ((uint32_t)((warp & 3) * 32) << 16) + S::kQ + T * S::kQTile;
+#pragma unroll
+                for (int pl = 0; pl < (HD == 128 ? 1 : 2); ++pl)
+#pragma unroll
+                    for (int c = 0; c < UNITS / 4; ++c) {
+                        uint32_t x[16];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(hold + pl * (kPcRows * HD * 2) + rl * (HD * 2) +
+                                                                             (((4 * c + k) ^ (rl & 7 & (UNITS - 1))) * 16));
+                            x[4 * k] = v.x, x[4 * k + 1] = v.y, x[4 * k + 2] = v.z, x[4 * k + 3] = v.w;
+                        }
+                        tmem_st16(tq + pl * S::kQCols + c * 16, x);
+                    }
                 tc_wait_st();
                 tc_fence_before();
                 fence_async_smem();
@@ -398,7 +427,11 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                     const float4 *at = place(k);
                     v[k] = nst > kFold && live ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
-                __syncwarp(); // every lane has read before the rows are written
+                __syncwarp(); // every lane has read before anything is written
+                // 32 columns at a time through 4 KB of the warp's own (k-th four values of lane l at slot l ^ k of piece k), so that
+                // a store writes four whole lines
+                uint8_t *hold = HD <= 64 ? reinterpret_cast<uint8_t *>(place(0) - lane) : smem + S::kOffSum + warp * 4096;
+                constexpr int kPiece = HD <= 64 ? kPcRows * 16 : 512;
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) {
                     float o[32];
@@ -406,16 +439,23 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         tmem_ld32(trow + S::kO + c * 32, o);
                         tc_wait_ld();
                     }
-                    if (live) {
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const float4 w = v[8 * c + k];
-                            *reinterpret_cast<float4 *>(dst + c * 32 + 4 * k) =
-                                l > 0.0f ? make_float4(fmaf(w.x, since, o[4 * k]) * inv * unit, fmaf(w.y, since, o[4 * k + 1]) * inv * unit,
-                                                       fmaf(w.z, since, o[4 * k + 2]) * inv * unit, fmaf(w.w, since, o[4 * k + 3]) * inv * unit)
-                                         : make_float4(0.f, 0.f, 0.f, 0.f);
-                        }
+                    for (int k = 0; k < 8; ++k) {
+                        const float4 w = v[8 * c + k];
+                        *reinterpret_cast<float4 *>(hold + k * kPiece + (lane ^ k) * 16) =
+                            l > 0.0f ? make_float4(fmaf(w.x, since, o[4 * k]) * inv * unit, fmaf(w.y, since, o[4 * k + 1]) * inv * unit,
+                                                   fmaf(w.z, since, o[4 * k + 2]) * inv * unit, fmaf(w.w, since, o[4 * k + 3]) * inv * unit)
+                                     : make_float4(0.f, 0.f, 0.f, 0.f);
                     }
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int row = 4 * k + (lane >> 3), q = lane & 7;
+                        const float4 w = *reinterpret_cast<const float4 *>(hold + q * kPiece + (row ^ q) * 16);
+                        float *to = reinterpret_cast<float *>(__shfl_sync(0xffffffffu, (uint64_t)dst, row));
+                        if (__shfl_sync(0xffffffffu, (int)live, row)) *reinterpret_cast<float4 *>(to + c * 32 + q * 4) = w;
+                    }
+                    __syncwarp();
                 }
                 if (live && p.splits > 1) *reinterpret_cast<float2 *>(dst + HD) = make_float2(m, l);
             }
