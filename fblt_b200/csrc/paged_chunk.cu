@@ -169,7 +169,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             int qe; // the row of Q was multiplied by 2^qe
             bool qbad; // a query value that is not finite
             {
-                constexpr int LPR = HD / 4, RPI = 32 / LPR, UNITS = HD / 8, B = 8; // lanes a row, rows an instruction, units a row
+                constexpr int LPR = HD / 4, RPI = 32 / LPR, UNITS = HD / 8, B = HD == 32 ? 8 : 16; // lanes a row, rows an instruction, units a row
+                const uint64_t own = (uint64_t)(p.q + (int64_t)(r0 + i) * p.qs + (int64_t)head * HD);
                 uint8_t *hold = smem + S::kOffSum + T * kPcRows * (HD == 128 ? 64 : HD) * 4; // first plane, then (HD <= 64) the second
                 const int q4 = lane % LPR;
 #pragma unroll 1
@@ -177,14 +178,11 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                     float4 v[B];
 #pragma unroll
                     for (int k = 0; k < B; ++k) {
-                        const int rr_ = min(row0 + T * kPcRows + (warp & 3) * 32 + (it + k) * RPI + lane / LPR, rows - 1), ii = rr_ / p.G;
-                        if (it + k < 32 / RPI)
-                            v[k] = *reinterpret_cast<const float4 *>(p.q + (int64_t)(r0 + ii) * p.qs +
-                                                                     (int64_t)(kvh * p.G + (rr_ - ii * p.G)) * HD + q4 * 4);
+                        const uint64_t row = __shfl_sync(0xffffffffu, own, (it + k) * RPI + lane / LPR);
+                        v[k] = reinterpret_cast<const float4 *>(row)[q4];
                     }
 #pragma unroll
                     for (int k = 0; k < B; ++k) {
-                        if (it + k >= 32 / RPI) break;
                         const int row = (warp & 3) * 32 + (it + k) * RPI + lane / LPR;
                         const float w[4] = {v[k].x * p.qscale, v[k].y * p.qscale, v[k].z * p.qscale, v[k].w * p.qscale};
                         float a = 0.0f;
@@ -259,22 +257,28 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 }
                 tc_fence_after();
                 if (j > 0 && j % kFold == 0) { // O is complete: S came behind it
+                    constexpr int W = HD == 128 ? 16 : 8; // fours of columns whose sums are read together
 #pragma unroll 1
-                    for (int c = 0; c < HD / 32; ++c) {
-                        float o[32];
-                        float4 *at[8], v[8];
-                        tmem_ld32(trow + S::kO + c * 32, o);
+                    for (int c = 0; c < HD / 4; c += W) {
+                        float4 v[W];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            at[k] = place(8 * c + k);
-                            v[k] = j > kFold && (live || HD <= 64) ? *at[k] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (int k = 0; k < W; ++k) {
+                            const float4 *at = place(c + k);
+                            v[k] = j > kFold && (live || HD <= 64) ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
                         }
-                        tc_wait_ld();
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            if (live || HD <= 64)
-                                *at[k] = make_float4(fmaf(v[k].x, since, o[4 * k]), fmaf(v[k].y, since, o[4 * k + 1]),
-                                                     fmaf(v[k].z, since, o[4 * k + 2]), fmaf(v[k].w, since, o[4 * k + 3]));
+                        for (int h = 0; h < W; h += 8) {
+                            float o[32];
+                            tmem_ld32(trow + S::kO + (c + h) * 4, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                float4 *at = place(c + h + k);
+                                if (live || HD <= 64)
+                                    *at = make_float4(fmaf(v[h + k].x, since, o[4 * k]), fmaf(v[h + k].y, since, o[4 * k + 1]),
+                                                      fmaf(v[h + k].z, since, o[4 * k + 2]), fmaf(v[h + k].w, since, o[4 * k + 3]));
+                            }
+                        }
                     }
                     since = 1.0f;
                 }
