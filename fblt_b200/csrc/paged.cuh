@@ -6,6 +6,7 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <atomic>
 #include <limits.h>
 #include <string.h>
 
@@ -48,6 +49,18 @@ inline PagedView paged_view(const fblt_paged_cache &c) {
     v.kvh = c.num_kv_heads;
     v.status = c.status;
     return v;
+}
+
+// Raises a kernel's dynamic shared memory limit on the current device, once (the call costs a microsecond of a decode
+// step). `done`: a bit per device ordinal; devices past 63 are set every time.
+inline int allow_smem(const void *kernel, int bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    FBLT_CUDA_TRY(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (bit & done.load(std::memory_order_relaxed)) return FBLT_OK;
+    FBLT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return FBLT_OK;
 }
 
 int validate_paged_cache(const fblt_paged_cache &c, int batch, const char *who); // paged_cache.cu

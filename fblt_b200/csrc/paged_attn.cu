@@ -15,7 +15,7 @@
 //     significant bits), and the 16 rows of the A operand are 8 query rows in two planes, q = hi + lo with 22 bits
 //     in all, so q . code is fp32 class in ONE instruction and hi + lo are added in registers. Probabilities go back
 //     the same way for P V. The exponents of K multiply scores, those of V probabilities: per (row, key), not per value.
-//     tcgen05 would need 128 rows of A; 8 .. 64 exist.
+//     tcgen05 would need 128 rows of A; 8 .. 32 exist.
 //   * Both products see keys and head_dim in an order of our own choosing (a sum has none): lane t of a quad takes 16
 //     neighbouring codes of a K row, lane g 1/8 of a V row, and the 16 keys of one product are 4 of each group, so
 //     that with the 32-byte skew V's column-wise reads touch every bank once.
@@ -627,7 +627,9 @@ static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
     const int64_t rows = (int64_t)d->max_new * (d->num_heads / d->cache.num_kv_heads);
     const int64_t units = (int64_t)d->batch * d->cache.num_kv_heads;
     int64_t s = d->splits;
-    pl.chunk = rows > 64;
+    // 64 caches of 1.5 to 8 k keys, 8 kv heads, head_dim 64 / 128: 32 rows 339 / 551 us streamed, 395 / 623 us as a chunk;
+    // 48 rows 630 / 882 us and 396 / 640 us (a streaming CTA's warps each read all keys once more for every 8 or 16 rows).
+    pl.chunk = rows > 32;
     if (pl.chunk) {
         pl.rb = pl.wr = 0;
         pl.row_tiles = (int)((rows + 255) / 256);
@@ -647,7 +649,7 @@ static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
         // Two blocks of 8 rows a warp while their output (64 registers a block at head_dim 128) leaves room for more than
         // one CTA on an SM: at 128 one block (block of 8 rows x 4 heads over 64 caches: 557 us, two blocks 708 us).
         pl.rb = rows <= 8 || d->cache.head_dim == 128 ? 1 : 2;
-        pl.wr = rows <= 8 * pl.rb ? 1 : rows <= 16 * pl.rb ? 2 : 4;
+        pl.wr = rows <= 8 * pl.rb ? 1 : rows <= 16 * pl.rb ? 2 : 4; // 4: head_dim 128 alone, 17 .. 32 rows
         const int rt = 8 * pl.rb * pl.wr;
         pl.row_tiles = (int)((rows + rt - 1) / rt);
         if (s == 0) {
@@ -666,7 +668,8 @@ template <int HD, int FMT, int RB, int WR>
 static int launch_stream_t(const PagedAttnParams &p, cudaStream_t s) {
     constexpr int smem = PsShape<HD>::kStages * PsShape<HD>::kStage + RB * WR * (HD / 16) * 512;
     static_assert(4 / WR * 8 * RB * WR * (HD + 4) * 4 <= smem, "the merge area fits the ring");
-    FBLT_CUDA_TRY(cudaFuncSetAttribute(paged_stream_kernel<HD, FMT, RB, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<uint64_t> done{0};
+    if (const int st = allow_smem((const void *)paged_stream_kernel<HD, FMT, RB, WR>, smem, done)) return st;
     const dim3 grid((unsigned)p.pv.kvh, (unsigned)p.splits, (unsigned)(p.batch * p.row_tiles));
     paged_stream_kernel<HD, FMT, RB, WR><<<grid, WR == 1 ? 128 : 160, smem, s>>>(p);
     count_launch();
@@ -682,7 +685,8 @@ static int launch_paged(const PagedAttnParams &p, const PagedPlan &pl, bool e4, 
     else if (pl.rb == 1 && pl.wr == 1) st = FBLT_PS(1, 1);
     else if (pl.wr == 1) st = FBLT_PS(B, 1);
     else if (pl.wr == 2) st = FBLT_PS(B, 2);
-    else st = FBLT_PS(B, 4);
+    else if constexpr (B == 1) st = FBLT_PS(B, 4);
+    else return fail(FBLT_ERR_UNSUPPORTED, "paged_attn: no kernel for this tile of rows");
 #undef FBLT_PS
     if (st != FBLT_OK || p.splits <= 1) return st;
     const int64_t units = (int64_t)p.total * p.H, per = 256 / (HD / 4);

@@ -626,7 +626,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
 
 template <int HD, int FMT>
 static int launch_chunk_t(const PagedAttnParams &p, cudaStream_t s) {
-    FBLT_CUDA_TRY(cudaFuncSetAttribute(paged_chunk_kernel<HD, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PcShape<HD>::kSmem));
+    static std::atomic<uint64_t> done{0};
+    if (const int st = allow_smem((const void *)paged_chunk_kernel<HD, FMT>, PcShape<HD>::kSmem, done)) return st;
     const dim3 grid((unsigned)p.pv.kvh, (unsigned)p.splits, (unsigned)(p.batch * p.row_tiles));
     paged_chunk_kernel<HD, FMT><<<grid, kPcThreads, PcShape<HD>::kSmem, s>>>(p);
     count_launch();
