@@ -177,7 +177,9 @@ struct PagedAttnParams {
     float qscale; // scale * log2(e)
 };
 
-// Keys that rows [row0, row0 + rows) of a sequence with n new rows at `base` see between them.
+// Keys that rows [row0, row0 + rows) of a sequence with n new rows at `base` see between them. Positions beyond the page
+// table hold no key, and however large a length is, nothing walks past them (nor past where a stage's last key would leave
+// 32 bits).
 struct RowRange {
     int lo, hi; // keys the tile's rows see between them
 };
@@ -186,6 +188,13 @@ __device__ __forceinline__ RowRange tile_range(const PagedAttnParams &p, int bas
     const int i0 = row0 / p.G, i1 = min(n - 1, (row0 + rows - 1) / p.G);
     r.hi = p.block_mode ? base + n : base + i1 + 1;
     r.lo = !p.block_mode && p.window > 0 ? max(0, base + i0 - p.window + 1) : 0;
+    const int64_t room = (int64_t)p.pv.max_pages * p.pv.page_size;
+    const int cap = room < INT_MAX - 4096 ? (int)room : (INT_MAX - 4096) & ~15;
+    if (r.hi > cap) {
+        p.pv.raise(FBLT_PAGED_BAD_PAGE);
+        r.hi = cap;
+    }
+    r.lo = min(r.lo, r.hi);
     return r;
 }
 

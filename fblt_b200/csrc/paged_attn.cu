@@ -602,6 +602,8 @@ int paged_attn_check(const fblt_paged_attn_desc *d) {
     if (d->splits < 0) return fail(FBLT_ERR_ARG, "%s: negative splits", who);
     if (!(fabsf(d->scale) < INFINITY)) return fail(FBLT_ERR_ARG, "%s: scale must be finite", who);
     if (d->batch > 65535) return fail(FBLT_ERR_LIMIT, "%s: batch exceeds 65535 per launch", who);
+    if ((int64_t)d->max_new * (d->num_heads / d->cache.num_kv_heads) > INT_MAX / 2)
+        return fail(FBLT_ERR_LIMIT, "%s: max_new * num_heads / num_kv_heads exceeds 2^30", who);
     if (d->batch == 0 || d->total_rows == 0 || d->max_new == 0) return FBLT_OK;
     if (!d->cu_new || !d->base_len || !d->q || !d->out) return fail(FBLT_ERR_ARG, "%s: NULL buffer", who);
     const int64_t E = (int64_t)d->num_heads * d->cache.head_dim;
@@ -725,6 +727,8 @@ extern "C" int fblt_paged_attn(const fblt_paged_attn_desc *d, void *workspace, s
     }
     if ((int64_t)d->batch * pl.row_tiles > 65535)
         return fail(FBLT_ERR_LIMIT, "paged_attn: batch * row tiles (%d) exceed 65535 per launch", pl.row_tiles);
+    if (pl.splits > 1 && (int64_t)d->total_rows * d->num_heads * (d->cache.head_dim / 4) / 256 >= INT_MAX)
+        return fail(FBLT_ERR_LIMIT, "paged_attn: too many rows to merge in one launch");
     PagedAttnParams p;
     memset(&p, 0, sizeof(p));
     p.pv = paged_view(d->cache);

@@ -506,8 +506,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             if (lost && lane == 0) give_up(0x53);
             // ---- the tile's range of exponents (keys that are there)
             {
-                const int4 r = make_int4(__reduce_max_sync(0xffffffffu, here ? ek : -1000), __reduce_min_sync(0xffffffffu, here ? ek : 1000),
-                                         __reduce_max_sync(0xffffffffu, here ? ev : -1000), __reduce_min_sync(0xffffffffu, here ? ev : 1000));
+                // (a row with the least exponent, as a row of zeros has, does not make a tile wide)
+                const bool sk = here && ek > F::kEmin, sv = here && ev > F::kEmin;
+                const int4 r = make_int4(__reduce_max_sync(0xffffffffu, here ? ek : -1000), __reduce_min_sync(0xffffffffu, sk ? ek : 1000),
+                                         __reduce_max_sync(0xffffffffu, here ? ev : -1000), __reduce_min_sync(0xffffffffu, sv ? ev : 1000));
                 if (lane == 0) range[st][warp - 8] = r;
             }
             if (converters_or(lost)) break; // all four warps go on or none
@@ -517,7 +519,11 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 const int4 r = range[st][i];
                 e = make_int4(max(e.x, r.x), min(e.y, r.y), max(e.z, r.z), min(e.w, r.w));
             }
-            const bool none = e.x < F::kEmin, kwide = !none && e.x - e.y > kPcNarrow, vwide = !none && e.z - e.w > kPcNarrow;
+            // Beside rows 2^60 larger, a row with the least exponent is one of zeros; nearer to it the tile counts as wide.
+            auto is_wide = [&](int most, int least) {
+                return most > F::kEmin && (most < F::kEmin + 60 ? most - F::kEmin > kPcNarrow : most - least > kPcNarrow);
+            };
+            const bool none = e.x < F::kEmin, kwide = is_wide(e.x, e.y), vwide = is_wide(e.z, e.w);
             const int kbelow = here ? e.x - ek : 0, vbelow = here ? e.z - ev : 0; // 2^-below: into the halves or the columns
             if (ct == 0) *reinterpret_cast<int4 *>(top_of[st]) = make_int4(none ? 0 : e.x, none ? 0 : e.z, kwide, vwide);
             const uint32_t vote = __ballot_sync(0xffffffffu, here);
@@ -545,8 +551,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 }
             };
             uint8_t *kd = smem + S::kOffKv + st * 2 * S::kKv + key * 16;
-            put(kd, kr, __float2half2_rn(kwide ? 1.0f : exp2_int(-kbelow)));
-            put(kd + S::kKv, vr, __float2half2_rn(vwide ? 1.0f : exp2_int(-vbelow)));
+            put(kd, kr, __float2half2_rn(kwide ? 1.0f : kbelow > 24 ? 0.0f : exp2_int(-kbelow)));
+            put(kd + S::kKv, vr, __float2half2_rn(vwide ? 1.0f : vbelow > 24 ? 0.0f : exp2_int(-vbelow)));
             fence_async_smem();
             mbar_arrive(&bars.kv_full[st]);
             load(next);

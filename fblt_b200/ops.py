@@ -541,6 +541,26 @@ def dv_commit(logits: torch.Tensor, width: int, x: torch.Tensor, l: torch.Tensor
 # The make_* functions check their tensors and fill a descriptor that keeps them alive (`keep`); it is made once for a
 # program's buffers and launched as often as it likes.
 
+
+def _keep(d, *tensors):
+    """Keeps the tensors of a descriptor alive and notes the device that all of them have to be on."""
+    d.keep = tensors
+    devices = {t.device.index for t in tensors if isinstance(t, torch.Tensor)}
+    devices |= {t.k_codes.device.index for t in tensors if isinstance(t, PagedKvCache)}
+    if len(devices) != 1:
+        raise ValueError(f"tensors on different devices: {sorted(devices)}")
+    d.device = devices.pop()
+    return d
+
+
+def _stream_on(d, stream) -> Optional[int]:
+    """The stream's handle; kernels are launched on the current device, where the descriptor's tensors have to be."""
+    current = torch.cuda.current_device()
+    if current != d.device or (isinstance(stream, torch.cuda.Stream) and stream.device_index != current):
+        raise ValueError(f"tensors on device {d.device}, current device {current}, stream {stream}")
+    return _raw_stream(current) or None if stream is None else _stream_ptr(stream)
+
+
 _KV_FORMATS = {"e4m3": L.KV_E4M3, "int8": L.KV_INT8}
 
 
@@ -650,12 +670,11 @@ def make_qk_norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], pos:
         d.pos = _table(pos, rows, "pos").data_ptr()
     if status is not None:
         d.status = _table(status, 1, "status").data_ptr()
-    d.keep = [q, k, pos, q_out, k_out, q_gain, k_gain, rope_cos, rope_sin, status]
-    return d
+    return _keep(d, q, k, pos, q_out, k_out, q_gain, k_gain, rope_cos, rope_sin, status)
 
 
 def qk_norm_rope(d: L.QkNormRopeDesc, stream=None) -> None:
-    L.check(L.load().fblt_qk_norm_rope(C.byref(d), _stream_ptr(stream)))
+    L.check(L.load().fblt_qk_norm_rope(C.byref(d), _stream_on(d, stream)))
 
 
 def make_paged_append(cache: PagedKvCache, cu_new: torch.Tensor, base_len: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
@@ -678,12 +697,11 @@ def make_paged_append(cache: PagedKvCache, cu_new: torch.Tensor, base_len: torch
         raise ValueError("q, q_out, k and v have one row count")
     d.q_gain, d.k_gain = _vector(q_gain, hd, "q_gain"), _vector(k_gain, hd, "k_gain")
     _rope(d, rope_cos, rope_sin, hd)
-    d.keep = [cache, cu_new, base_len, k, v, q, q_out, q_gain, k_gain, rope_cos, rope_sin]
-    return d
+    return _keep(d, cache, cu_new, base_len, k, v, q, q_out, q_gain, k_gain, rope_cos, rope_sin)
 
 
 def paged_append(d: L.PagedAppendDesc, stream=None) -> None:
-    L.check(L.load().fblt_paged_append(C.byref(d), _stream_ptr(stream)))
+    L.check(L.load().fblt_paged_append(C.byref(d), _stream_on(d, stream)))
 
 
 def make_paged_read(cache: PagedKvCache, cu_rows: torch.Tensor, k_out: Optional[torch.Tensor], v_out: Optional[torch.Tensor], *,
@@ -701,12 +719,11 @@ def make_paged_read(cache: PagedKvCache, cu_rows: torch.Tensor, k_out: Optional[
         if t is not None:
             setattr(d, name, _rows(t, cache.num_kv_heads * cache.head_dim, name, (torch.float32, torch.bfloat16)).data_ptr())
             setattr(d, name + "_stride", t.stride(0))
-    d.keep = [cache, cu_rows, k_out, v_out, start]
-    return d
+    return _keep(d, cache, cu_rows, k_out, v_out, start)
 
 
 def paged_read(d: L.PagedReadDesc, stream=None) -> None:
-    L.check(L.load().fblt_paged_read(C.byref(d), _stream_ptr(stream)))
+    L.check(L.load().fblt_paged_read(C.byref(d), _stream_on(d, stream)))
 
 
 def make_paged_attn(cache: PagedKvCache, cu_new: torch.Tensor, base_len: torch.Tensor, q: torch.Tensor, out: torch.Tensor,
@@ -724,19 +741,18 @@ def make_paged_attn(cache: PagedKvCache, cu_new: torch.Tensor, base_len: torch.T
     if q.shape[0] != out.shape[0]:
         raise ValueError("q and out have one row count")
     d.scale = float(scale)
-    d.keep = [cache, cu_new, base_len, q, out]
-    return d
+    return _keep(d, cache, cu_new, base_len, q, out)
 
 
 def paged_attn_workspace(d: L.PagedAttnDesc) -> Optional[torch.Tensor]:
     n = L.load().fblt_paged_attn_workspace(C.byref(d))
-    return torch.empty(n, dtype=torch.uint8, device="cuda") if n else None
+    return torch.empty(n, dtype=torch.uint8, device=d.keep[0].k_codes.device) if n else None
 
 
 def paged_attn(d: L.PagedAttnDesc, workspace: Optional[torch.Tensor] = None, stream=None) -> None:
     wp = workspace.data_ptr() if workspace is not None else None
     wn = workspace.numel() if workspace is not None else 0
-    L.check(L.load().fblt_paged_attn(C.byref(d), wp, wn, _stream_ptr(stream)))
+    L.check(L.load().fblt_paged_attn(C.byref(d), wp, wn, _stream_on(d, stream)))
 
 
 class PagedStepPlan:
@@ -760,8 +776,8 @@ class PagedStepPlan:
         a = make_paged_attn(cache, cu_new, base_len, self._comb, self.out, num_heads, max_new, max_len, 1.0,
                             block_mode=block_mode, window=window)
         self._ws = paged_attn_workspace(a)
-        self._keep = [w_qkv, w_proj, cache, cu_new, base_len, q_gain, k_gain, rope_cos, rope_sin]
         d = self.desc = L.PagedStepDesc()
+        _keep(d, cache, cu_new, base_len, q_gain, k_gain, rope_cos, rope_sin, w_qkv.buf, w_proj.buf)
         d.cache, d.batch, d.num_heads, d.total_rows, d.max_new = cache.desc, cache.batch, num_heads, total_rows, max_new
         d.max_len, d.block_mode, d.window, d.precision = max_len, int(block_mode), window, precision
         d.cu_new, d.base_len = cu_new.data_ptr(), base_len.data_ptr()
@@ -775,7 +791,7 @@ class PagedStepPlan:
         _rope(d, rope_cos, rope_sin, hd)
 
     def run(self, stream=None) -> None:
-        L.check(L.load().fblt_paged_self_attention_step(C.byref(self.desc), _stream_ptr(stream)))
+        L.check(L.load().fblt_paged_self_attention_step(C.byref(self.desc), _stream_on(self.desc, stream)))
 
 
 # --------------------------------------------------------------------------- host-buffer sessions

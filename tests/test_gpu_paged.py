@@ -579,6 +579,56 @@ def test_on_another_stream(cuda_lib):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("n", [1, 20, 150])
+def test_lengths_far_beyond_the_page_table(cuda_lib, n):
+    """A length near 2^31: nothing walks past the table; the keys that exist are attended to and the rest is reported."""
+    c = make_cache(150, "int8", [64], 2, 64, 16, extra_cols=0)
+    fill_cache(c, 151, [64])
+    base = 2**31 - 1 - n - 5000
+    q, out = attend(c, [n], [base], 4, 152, max_len=4096)
+    assert c.status_bits() == L.PAGED_BAD_PAGE
+    k, v = stored(c, 0, 64, "k"), stored(c, 0, 64, "v")
+    want, tol = R.attention(q.view(n, 4, 64), k, v, 10**6, 0.125, False, 0)
+    assert ((out.view(n, 4, 64).double().cpu() - want).abs() <= tol).all()
+    _, out = attend(c, [n], [base], 4, 152, max_len=4096, window=100)  # a window that has left the table
+    assert bool((out == 0).all()) and c.status_bits() == L.PAGED_BAD_PAGE
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n", [1, 200])
+def test_rows_of_zeros_and_of_the_smallest_values(cuda_lib, fmt, n):
+    """Zeros in K and V between ordinary rows, and caches whose every value lies near the smallest exponent."""
+    hd, kv, base = 64, 2, 250
+    for size in (1.0, 2.0 ** -119, 2.0 ** -90):
+        c = make_cache(160, fmt, [base + n], kv, hd, 16)
+        g = gen(161)
+        k, v = randn(g, base + n, kv * hd) * size, randn(g, base + n, kv * hd) * size
+        k[::7], v[::5] = 0, 0
+        ops.paged_append(ops.make_paged_append(c, cu([base + n]), i32([0]), k, v))
+        q = randn(g, n, 4 * hd) / size
+        q, out = attend(c, [n], [base], 4, 0, q=q)
+        check_attention(c, q, out, [n], [base], 4)
+
+
+def test_two_calls_at_once(cuda_lib):
+    """The same kernels on two streams at the same time, each with its own workspace and status."""
+    jobs = []
+    for seed, new, base in ((170, [1, 1], [900, 3000]), (171, [300], [2000])):
+        c = make_cache(seed, "e4m3", [b + n for b, n in zip(base, new)], 2, 64, 32)
+        fill_cache(c, seed + 5, [b + n for b, n in zip(base, new)])
+        q = randn(gen(seed), sum(new), 4 * 64)
+        out = torch.empty_like(q)
+        d = ops.make_paged_attn(c, cu(new), i32(base), q, out, 4, max(new), 3100, 0.125, splits=3)
+        jobs.append((d, ops.paged_attn_workspace(d), torch.cuda.Stream(), c, q, out, new, base))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for d, ws, s, *_ in jobs:
+            ops.paged_attn(d, ws, s)
+    torch.cuda.synchronize()
+    for d, ws, s, c, q, out, new, base in jobs:
+        check_attention(c, q, out, new, base, 4)
+
+
 def test_bindings_refuse_wrong_tensors(cuda_lib):
     c = make_cache(140, "e4m3", [32], 2, 64, 16)
     k = torch.zeros(4, 128, device="cuda")
@@ -594,3 +644,7 @@ def test_bindings_refuse_wrong_tensors(cuda_lib):
         ops.make_paged_read(c, cu([4]), k, k.bfloat16())
     with pytest.raises(ValueError):
         ops.PagedKvCache(c.k_codes, c.v_codes, c.k_exp.float(), c.v_exp, c.page_table, "e4m3")
+    d = ops.make_paged_append(c, cu([4]), i32([0]), k, k)
+    d.device = 1  # as if the tensors were on another device than the current one
+    with pytest.raises(ValueError):
+        ops.paged_append(d)

@@ -108,7 +108,8 @@ def test_read_refuses(bad):
     (dict(num_heads=0), L.ERR_ARG), (dict(window=-1), L.ERR_ARG), (dict(splits=-1), L.ERR_ARG), (dict(scale=float("inf")), L.ERR_ARG),
     (dict(scale=float("nan")), L.ERR_ARG), (dict(batch=65536), L.ERR_LIMIT), (dict(cu_new=None), L.ERR_ARG), (dict(q=None), L.ERR_ARG),
     (dict(base_len=None), L.ERR_ARG), (dict(out=None), L.ERR_ARG), (dict(q_stride=255), L.ERR_ARG), (dict(out_stride=258), L.ERR_ARG),
-    (dict(q=P + 8), L.ERR_ARG)])
+    (dict(q=P + 8), L.ERR_ARG), (dict(max_new=2**30, num_heads=8, q_stride=512, out_stride=512), L.ERR_LIMIT),
+    (dict(max_new=2**28), L.ERR_LIMIT)])
 def test_attention_refuses(bad, want):
     assert L.load().fblt_paged_attn(C.byref(attn(**bad)), P, 1 << 30, None) == want
 
