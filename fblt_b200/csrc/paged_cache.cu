@@ -6,6 +6,10 @@
 // them is HBM (reading and writing every value once), as long as a value costs few instructions: lanes keep a head and
 // walk down the rows of their CTA, so that what belongs to the head (pointers, gains, the kind of work) is set up once
 // and a row costs additions (with a division per value group instead, the launch was bound by instruction issue).
+//
+// Measured (B200): norm + rotation of a prompt's q and k, 680 MB moved: 123 us, 5.5 TB/s; a prompt appended and read back
+// 354 us against 223 us of bytes (K goes through 64-bit arithmetic, and a row's page is two dependent loads); 1.26 GB read
+// back from caches 209 us, 6.1 TB/s; one token's rows 4.6 us, a launch.
 #include "paged.cuh"
 
 namespace fblt {

@@ -12,7 +12,8 @@
  *       mask given as a descriptor derived from the patcher's boundary array,
  *       never a dense matrix). These return an int status and never exit.
  *
- * All tensors are fp32. Pointers named "device" must be CUDA device pointers
+ * All tensors are fp32, but for the codes and exponents of the paged 8-bit KV
+ * cache (its section says what they hold). Pointers named "device" must be CUDA device pointers
  * of the current device; everything else is host memory. No entry point
  * requires the caller to synchronise; work is ordered on the stream passed in
  * (NULL = the legacy default stream, which is what the reference uses,
