@@ -65,13 +65,9 @@ inline int allow_smem(const void *kernel, int bytes, std::atomic<uint64_t> &done
 
 int validate_paged_cache(const fblt_paged_cache &c, int batch, const char *who); // paged_cache.cu
 
-// New rows of sequence b: packed rows [r0, r0 + n), first position base. False (and the status bit) where the tables
-// do not describe a sequence.
-__device__ __forceinline__ bool paged_seq(const PagedView &pv, const int32_t *cu, const int32_t *base_len, int total, int b,
-                                          int &r0, int &n, int &base) {
-    r0 = cu[b];
-    const int r1 = cu[b + 1];
-    base = base_len ? base_len[b] : 0;
+// New rows of a sequence: packed rows [r0, r1), first position base; n of them. False (and the status bit) where that is
+// not a sequence.
+__device__ __forceinline__ bool paged_seq_ok(const PagedView &pv, int r0, int r1, int base, int total, int &n) {
     n = r1 - r0;
     if (r0 < 0 || r1 < r0 || r1 > total || base < 0 || base > INT_MAX - n) {
         pv.raise(FBLT_PAGED_BAD_LENGTH);
@@ -79,6 +75,13 @@ __device__ __forceinline__ bool paged_seq(const PagedView &pv, const int32_t *cu
         return false;
     }
     return true;
+}
+// The same for sequence b of the tables.
+__device__ __forceinline__ bool paged_seq(const PagedView &pv, const int32_t *cu, const int32_t *base_len, int total, int b,
+                                          int &r0, int &n, int &base) {
+    r0 = cu[b];
+    base = base_len ? base_len[b] : 0;
+    return paged_seq_ok(pv, r0, cu[b + 1], base, total, n);
 }
 
 // 2^e as a float, -126 <= e <= 127.

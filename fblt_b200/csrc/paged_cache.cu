@@ -7,15 +7,17 @@
 // walk down the rows of their CTA, so that what belongs to the head (pointers, gains, the kind of work) is set up once
 // and a row costs additions (with a division per value group instead, the launch was bound by instruction issue).
 //
-// Measured (B200): norm + rotation of a prompt's q and k, 680 MB moved: 123 us, 5.5 TB/s; a prompt appended and read back
-// 354 us against 223 us of bytes (K goes through 64-bit arithmetic, and a row's page is two dependent loads); 1.26 GB read
-// back from caches 209 us, 6.1 TB/s; one token's rows 4.6 us, a launch.
+// Measured (B200): norm + rotation of a prompt's q and k, 680 MB moved: 118-121 us, 5.7 TB/s; prompts appended and read
+// back 311-323 us against 223 us of bytes (K goes through 64-bit arithmetic; half of the warps fit); 1.27 GB read back from
+// caches 202 us, 6.2 TB/s; one token's rows 4.7 us, a launch. The first values of every lane are asked for before the look-up
+// of the rows, whose two dependent loads they hide.
 #include "paged.cuh"
 
 namespace fblt {
 
 constexpr int kRowThreads = 256;
-constexpr int kMaxRows = 16; // rows of one CTA
+constexpr int kMaxRows = 8;  // rows of one CTA
+constexpr int kRowLoads = 3; // rows of a head whose values a lane has in flight (64 registers and 4 CTAs an SM: 4 spill)
 
 struct RowInfo {
     int64_t at; // row of head 0 in the pool (PagedView::row), < 0: no page
@@ -26,7 +28,7 @@ struct RowInfo {
 struct NormRopeParams {
     PagedView pv;     // append
     int64_t rows;
-    int batch, qh, kh, rows_per_cta, rope_len;
+    int batch, qh, kh, rows_per_cta, rope_len, parts; // parts: log2, see split_rows
     const float *q, *k, *v;
     int64_t qs, ks, vs;
     float *qo, *ko;
@@ -42,27 +44,24 @@ struct NormRopeParams {
 __device__ __forceinline__ RowInfo find_row(const PagedView &pv, const int32_t *cu, const int32_t *base, int batch, int total,
                                             int r, int lane) {
     RowInfo ri;
+    ri.at = ri.pos = -1;
     ri.pad = 0;
-    int lo = 0, n = batch; // the answer lies in [lo, lo + n)
-    {
-        // sequences of one length: the row says which one it is
-        const int at = (int)((int64_t)r * batch / total);
-        if (__ldg(cu + at) <= r && r < __ldg(cu + at + 1)) {
-            lo = at;
-            n = 1;
+    // sequences of one length: the row says which one it is; all that it needs of the sequence is asked for at once
+    int lo = (int)((int64_t)r * batch / total);
+    int r0 = __ldg(cu + lo), r1 = __ldg(cu + lo + 1), p0 = base ? __ldg(base + lo) : 0;
+    if (r0 > r || r >= r1) {
+        lo = 0;
+        for (int n = batch; n > 1;) { // the answer lies in [lo, lo + n)
+            const int step = (n + 31) >> 5, at = lo + lane * step;
+            const bool le = lane * step < n && __ldg(cu + at) <= r;
+            const int k = max(0, __popc(__ballot_sync(0xffffffffu, le)) - 1); // cu ascends: the lanes that say yes are the first ones
+            lo += k * step;
+            n = min(step, n - k * step);
         }
+        r0 = __ldg(cu + lo), r1 = __ldg(cu + lo + 1), p0 = base ? __ldg(base + lo) : 0;
     }
-    while (n > 1) {
-        const int step = (n + 31) >> 5, at = lo + lane * step;
-        const bool le = lane * step < n && __ldg(cu + at) <= r;
-        const int k = max(0, __popc(__ballot_sync(0xffffffffu, le)) - 1); // cu ascends: the lanes that say yes are the first ones
-        lo += k * step;
-        n = min(step, n - k * step);
-    }
-    ri.at = -1;
-    ri.pos = -1;
-    int r0, count, p0;
-    if (!paged_seq(pv, cu, base, total, lo, r0, count, p0)) return ri;
+    int count;
+    if (!paged_seq_ok(pv, r0, r1, p0, total, count)) return ri;
     if (r < r0 || r >= r0 + count) {
         pv.raise(FBLT_PAGED_BAD_LENGTH);
         return ri;
@@ -135,7 +134,7 @@ __device__ __forceinline__ double rsqrt_43(double a) {
 // by the last bits of fp32, and this way it is the code of the definition.
 template <int HD, int FMT>
 __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_kernel(const NormRopeParams p) {
-    constexpr int LPH = HD / 4, GROUPS = kRowThreads / LPH, U = FMT < 0 ? 4 : 2;
+    constexpr int LPH = HD / 4, GROUPS = kRowThreads / LPH, U = kRowLoads;
     constexpr bool APPEND = FMT >= 0;
     __shared__ RowInfo info[kMaxRows];
     const int tid = threadIdx.x;
@@ -144,6 +143,33 @@ __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_kernel(const NormRop
     const int units = p.qh + (APPEND ? 2 : 1) * p.kh;
     const int group = tid / LPH, lane = tid % LPH;
     const uint32_t mask = LPH == 32 ? 0xffffffffu : ((1u << (LPH & 31)) - 1) << ((tid & 31) / LPH * LPH);
+    const int nkv = APPEND ? 2 * p.kh : p.kh;
+    // K first, then V, then Q: the long way through 64 bits runs beside the others' work, not behind it
+    int kind, head;
+    int64_t ss;
+    const float *src;
+    int row_a, row_b;
+    const auto item_of = [&](int item) {
+        const int unit = item >> p.parts, part = item & ((1 << p.parts) - 1), per = (p.rows_per_cta + (1 << p.parts) - 1) >> p.parts;
+        row_a = min(part * per, nrows);
+        row_b = min(row_a + per, nrows);
+        kind = unit >= nkv ? 0 : unit < p.kh ? 1 : 2;
+        head = unit - (kind == 0 ? nkv : kind == 1 ? 0 : p.kh);
+        ss = kind == 0 ? p.qs : kind == 1 ? p.ks : p.vs;
+        src = (kind == 0 ? p.q : kind == 1 ? p.k : p.v) + (row0 + row_a) * ss + head * HD + lane * 4;
+    };
+    float4 x[U];
+    const auto load = [&](int r) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (r + u < row_b) x[u] = *reinterpret_cast<const float4 *>(src + (int64_t)u * ss);
+        src += (int64_t)U * ss;
+    };
+    const int items = units << p.parts;
+    if (group < items) { // the first values travel while the rows are looked up
+        item_of(group);
+        load(row_a);
+    }
     if (APPEND) {
         for (int r = tid >> 5; r < nrows; r += kRowThreads / 32) {
             const RowInfo ri = find_row(p.pv, p.cu, p.base, p.batch, (int)p.rows, (int)row0 + r, tid & 31);
@@ -161,32 +187,34 @@ __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_kernel(const NormRop
     }
     __syncthreads();
     const float2 *cs = reinterpret_cast<const float2 *>(p.cs) + lane, *sn = reinterpret_cast<const float2 *>(p.sn) + lane;
-    for (int unit = group; unit < units; unit += GROUPS) {
-        // K first, then V, then Q: the long way through 64 bits runs beside the others' work, not behind it
-        const int nkv = APPEND ? 2 * p.kh : p.kh;
-        const int kind = unit >= nkv ? 0 : unit < p.kh ? 1 : 2, head = unit - (kind == 0 ? nkv : kind == 1 ? 0 : p.kh);
-        const int64_t ss = kind == 0 ? p.qs : kind == 1 ? p.ks : p.vs, ds = kind == 0 ? p.qos : p.kos;
-        const float *src = (kind == 0 ? p.q : kind == 1 ? p.k : p.v) + row0 * ss + head * HD + lane * 4;
+    float2 c[U], s[U];
+    const auto load_rope = [&](int r) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (r + u >= row_b) break;
+            const int pos = info[r + u].pos;
+            if (p.cs && (unsigned)pos < (unsigned)p.rope_len) {
+                c[u] = __ldg(cs + (int64_t)pos * (HD / 4));
+                s[u] = __ldg(sn + (int64_t)pos * (HD / 4));
+            }
+        }
+    };
+    for (int item = group; item < items; item += GROUPS) {
+        if (item != group) {
+            item_of(item);
+            load(row_a);
+        }
         if (!APPEND || kind == 0) {
-            float *dst = (kind == 0 ? p.qo : p.ko) + row0 * ds + head * HD + lane * 4;
+            const int64_t ds = kind == 0 ? p.qos : p.kos;
+            float *dst = (kind == 0 ? p.qo : p.ko) + (row0 + row_a) * ds + head * HD + lane * 4;
             const float *gain = kind == 0 ? p.qg : p.kg;
             const float4 g = gain ? __ldg(reinterpret_cast<const float4 *>(gain) + lane) : make_float4(1.f, 1.f, 1.f, 1.f);
-            for (int r = 0; r < nrows; r += U) {
-                float4 x[U];
-                float2 c[U], s[U];
+            for (int r = row_a; r < row_b; r += U) {
+                if (r > row_a) load(r);
+                load_rope(r);
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    if (r + u >= nrows) break;
-                    x[u] = *reinterpret_cast<const float4 *>(src + (int64_t)u * ss);
-                    const int pos = info[r + u].pos;
-                    if (p.cs && (unsigned)pos < (unsigned)p.rope_len) {
-                        c[u] = __ldg(cs + (int64_t)pos * (HD / 4));
-                        s[u] = __ldg(sn + (int64_t)pos * (HD / 4));
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (r + u >= nrows) break;
+                    if (r + u >= row_b) break;
                     const int pos = info[r + u].pos;
                     if (gain) {
                         const float sum = group_sum<LPH>(mask, x[u].x * x[u].x + x[u].y * x[u].y + (x[u].z * x[u].z + x[u].w * x[u].w));
@@ -199,7 +227,6 @@ __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_kernel(const NormRop
                     }
                     if (!APPEND || pos >= 0) *reinterpret_cast<float4 *>(dst + (int64_t)u * ds) = x[u];
                 }
-                src += (int64_t)U * ss;
                 dst += (int64_t)U * ds;
             }
         }
@@ -209,19 +236,14 @@ __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_kernel(const NormRop
             int8_t *exps = kind == 1 ? p.pv.ke : p.pv.ve;
             const int64_t skip = (int64_t)head * p.pv.page_size; // from head 0's row of a page to this head's
             const bool norm = kind == 1 && p.kg, rope = kind == 1 && p.cs;
-            double g[4] = {1.0, 1.0, 1.0, 1.0};
-            if (norm) {
-                const float4 f = __ldg(reinterpret_cast<const float4 *>(p.kg) + lane);
-                g[0] = f.x, g[1] = f.y, g[2] = f.z, g[3] = f.w;
-            }
-            for (int r = 0; r < nrows; r += U) {
-                float4 x[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (r + u < nrows) x[u] = *reinterpret_cast<const float4 *>(src + (int64_t)u * ss);
+            float4 g = make_float4(1.f, 1.f, 1.f, 1.f);
+            if (norm) g = __ldg(reinterpret_cast<const float4 *>(p.kg) + lane);
+            for (int r = row_a; r < row_b; r += U) {
+                if (r > row_a) load(r);
+                if (rope) load_rope(r);
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    if (r + u >= nrows) break;
+                    if (r + u >= row_b) break;
                     const RowInfo ri = info[r + u];
                     float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
                     if (norm || rope) {
@@ -229,16 +251,14 @@ __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_kernel(const NormRop
                         if (norm) {
                             const double sum = group_sum<LPH>(mask, d[0] * d[0] + d[1] * d[1] + (d[2] * d[2] + d[3] * d[3]));
                             const double inv = rsqrt_43(sum * (1.0 / HD) + (double)p.eps);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) d[i] *= inv * g[i];
+                            d[0] *= inv * (double)g.x, d[1] *= inv * (double)g.y, d[2] *= inv * (double)g.z, d[3] *= inv * (double)g.w;
                         }
                         if (rope && (unsigned)ri.pos < (unsigned)p.rope_len) {
-                            const float2 c = __ldg(cs + (int64_t)ri.pos * (HD / 4)), s = __ldg(sn + (int64_t)ri.pos * (HD / 4));
                             const double a = d[0], b = d[2];
-                            d[0] = a * (double)c.x - d[1] * (double)s.x;
-                            d[1] = d[1] * (double)c.x + a * (double)s.x;
-                            d[2] = b * (double)c.y - d[3] * (double)s.y;
-                            d[3] = d[3] * (double)c.y + b * (double)s.y;
+                            d[0] = a * (double)c[u].x - d[1] * (double)s[u].x;
+                            d[1] = d[1] * (double)c[u].x + a * (double)s[u].x;
+                            d[2] = b * (double)c[u].y - d[3] * (double)s[u].y;
+                            d[3] = d[3] * (double)c[u].y + b * (double)s[u].y;
                         }
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v[i] = round_odd(d[i]);
@@ -251,7 +271,6 @@ __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_kernel(const NormRop
                         if (lane == 0) exps[at] = (int8_t)e;
                     }
                 }
-                src += (int64_t)U * ss;
             }
         }
     }
@@ -259,7 +278,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_kernel(const NormRop
 
 struct ReadParams {
     PagedView pv;
-    int rows, batch, rows_per_cta;
+    int rows, batch, rows_per_cta, parts;
     const int32_t *cu, *start;
     void *ko, *vo;
     int64_t kos, vos;
@@ -278,20 +297,22 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(const ReadParam
     }
     __syncthreads();
     const int kh = p.pv.kvh, units = (p.ko && p.vo ? 2 : 1) * kh, group = tid / LPH, lane = tid % LPH;
-    for (int unit = group; unit < units; unit += GROUPS) {
+    const int items = units << p.parts, per = (p.rows_per_cta + (1 << p.parts) - 1) >> p.parts;
+    for (int item = group; item < items; item += GROUPS) {
+        const int unit = item >> p.parts, row_a = (item & ((1 << p.parts) - 1)) * per, row_b = min(row_a + per, nrows);
         const bool is_v = !p.ko || unit >= kh;
         const int head = unit >= kh ? unit - kh : unit;
         const int64_t skip = (int64_t)head * p.pv.page_size, ds = is_v ? p.vos : p.kos;
         const uint8_t *codes = (is_v ? p.pv.vc : p.pv.kc) + skip * HD + lane * 4;
         const int8_t *exps = (is_v ? p.pv.ve : p.pv.ke) + skip;
-        int64_t to = row0 * ds + head * HD + lane * 4;
+        int64_t to = (row0 + row_a) * ds + head * HD + lane * 4;
         void *dst = is_v ? p.vo : p.ko;
-        for (int r = 0; r < nrows; r += U) {
+        for (int r = row_a; r < row_b; r += U) {
             uint32_t w[U];
             int e[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (r + u >= nrows) break;
+                if (r + u >= row_b) break;
                 const int64_t at = info[r + u].at;
                 w[u] = 0;
                 e[u] = 0;
@@ -302,7 +323,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(const ReadParam
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (r + u >= nrows) break;
+                if (r + u >= row_b) break;
                 if (info[r + u].pos < 0) continue;
                 const float4 x = kv_values<FMT>(w[u], kv_scale<FMT>(e[u]));
                 if (BF16) {
@@ -320,11 +341,26 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(const ReadParam
     }
 }
 
-// Rows of one CTA: one while that fills the GPU, more when the launch is long anyway (the row look-up is then shared
-// and the loop has loads to overlap).
-static int rows_per_cta(int64_t rows) {
-    const int64_t r = rows / (148 * 16);
-    return r < 1 ? 1 : r > kMaxRows ? kMaxRows : (int)r;
+// Rows of one CTA: one while that fills the GPU, more when the launch is long anyway: the row look-up is then shared,
+// and a row's loads overlap the others' (in whole batches of `loads`, since a last, short batch waits as long as a full one).
+// Norm and append, 4 CTAs an SM: 4 rows of 2048 sequences 40 us at 6 rows a CTA, 49 us at 3; prompts (30 k rows appended and
+// read back) 314 us at 6 rows, 328 us at 12; norm alone (16 k rows) 118 us at 6, 127 us at 12. Reading, 8 CTAs an SM: 204 us
+// at 8 rows, 232 us at 4, 210 us at 16.
+static int rows_per_cta(int64_t rows, int64_t ctas, int loads, int most) {
+    const int64_t r = rows / ctas;
+    if (r < loads) return r < 1 ? 1 : (int)r;
+    return (r > most ? most : (int)r) / loads * loads;
+}
+
+// A CTA's groups share `units` heads x `rows` rows in items of one head and 1 / 2^parts of the rows: the split whose
+// busiest group has the fewest rows.
+static int split_rows(int units, int rows, int groups) {
+    int best = 0, least = INT_MAX;
+    for (int lp = 0; lp == 0 || (1 << lp) <= rows; ++lp) {
+        const int64_t rounds = (((int64_t)units << lp) + groups - 1) / groups, per = (rows + (1 << lp) - 1) >> lp;
+        if (rounds * per < least) least = (int)(rounds * per), best = lp;
+    }
+    return best;
 }
 
 static bool aligned16(const void *p) { return !(((uintptr_t)p) & 15); }
@@ -368,7 +404,8 @@ int validate_paged_cache(const fblt_paged_cache &c, int batch, const char *who) 
 
 template <int HD, int FMT>
 static int launch_norm_rope(NormRopeParams &p, cudaStream_t s, const char *what) {
-    p.rows_per_cta = rows_per_cta(p.rows);
+    p.rows_per_cta = rows_per_cta(p.rows, 148 * 8, kRowLoads, 2 * kRowLoads);
+    p.parts = split_rows(p.qh + (FMT < 0 ? 1 : 2) * p.kh, p.rows_per_cta, kRowThreads / (HD / 4));
     const int64_t grid = (p.rows + p.rows_per_cta - 1) / p.rows_per_cta;
     if (grid > INT_MAX) return fail(FBLT_ERR_LIMIT, "%s: too many rows", what);
     norm_rope_kernel<HD, FMT><<<(unsigned)grid, kRowThreads, 0, s>>>(p);
@@ -378,7 +415,8 @@ static int launch_norm_rope(NormRopeParams &p, cudaStream_t s, const char *what)
 
 template <int HD, int FMT>
 static int launch_read(ReadParams &p, bool bf16, cudaStream_t s) {
-    p.rows_per_cta = rows_per_cta(p.rows);
+    p.rows_per_cta = rows_per_cta(p.rows, 148 * 4, 1, 8);
+    p.parts = split_rows((p.ko && p.vo ? 2 : 1) * p.pv.kvh, p.rows_per_cta, kRowThreads / (HD / 4));
     const unsigned grid = (unsigned)((p.rows + p.rows_per_cta - 1) / p.rows_per_cta);
     if (bf16) paged_read_kernel<HD, FMT, true><<<grid, kRowThreads, 0, s>>>(p);
     else paged_read_kernel<HD, FMT, false><<<grid, kRowThreads, 0, s>>>(p);
