@@ -20,12 +20,13 @@
 //     neighbouring codes of a K row, lane g 1/8 of a V row, and the 16 keys of one product are 4 of each group, so
 //     that with the 32-byte skew V's column-wise reads touch every bank once.
 //
-// Measured (B200): one token of 256 sequences of up to 4 k keys, 16 kv heads, head_dim 64, int8: 281-288 us, 3.9 TB/s of
-// the cache's bytes; 8 rows x 4 heads over 64 caches of up to 8 k keys, head_dim 128, e4m3: 545-552 us. HBM's bound would be 171 and 102 us:
-// what is left is the conversion of codes to halves (five instructions for four int8 codes) and its latency with 8 to
-// 12 warps on an SM, which registers limit (146 and 167 a thread): issue slots are 53 and 41 % busy, and warps that
-// share keys each convert all of them. Measured and slower: a producer warp where warps share nothing 332 us; stages of 32
-// keys at head_dim 64 531 us; three CTAs an SM at head_dim 128 with spilled registers no faster (537 against 548 us).
+// Measured (B200): one token of 256 sequences of up to 4 k keys, 16 kv heads, head_dim 64, int8: 273-281 us, 4.0 TB/s of
+// the cache's bytes; 8 rows x 4 heads over 64 caches of up to 8 k keys, head_dim 128, e4m3: 414-429 us. HBM's bound would
+// be 171 and 102 us: what is left is the conversion of codes to halves (five instructions for four int8 codes) and its
+// latency with 12 warps on an SM, which registers limit: issue slots are half busy, and warps that share keys each convert
+// all of them. Measured and slower: a producer warp where warps share nothing 332 us; stages of 32 keys at head_dim 64
+// 531 us; a warp's 8 rows in steps of 16 keys instead of 32 456 us; four CTAs an SM at head_dim 128 519 us; a maximum that
+// moves with every larger score (not by 2^4 at least) 8 us more.
 #include "paged.cuh"
 #include "tc5.cuh"
 
@@ -40,6 +41,7 @@ __device__ unsigned int g_paged_error; // 0 = ok; otherwise (code << 24) | block
 // after so many keys what they hold is added, rounded, to sums of its own.
 constexpr int kPsFold = 256;
 constexpr int kPsHead = 10, kPsNoUnit = -(1 << 20);
+constexpr float kPsLazy = 4.0f; // a row's m moves, and what it holds is rescaled, once a score lies 2^4 above it
 
 template <int HD>
 struct PsShape {
@@ -49,7 +51,17 @@ struct PsShape {
     static constexpr int kPitch = kGroup + 32;          // see the bank skew above
     static constexpr int kOffV = 4 * kPitch, kOffE = 8 * kPitch;
     static constexpr int kStage = 8 * kPitch + 128; // K groups, V groups, exponents
-    static constexpr int kStages = 8; // of the CTA; a warp's own: kStages / 4
+};
+
+template <int HD, int RB, int WR>
+struct PsCta {
+    // Where 64 tensor core accumulators a thread and 32 folded sums would leave room for few warps, the sums, touched every
+    // 256 keys, live in shared memory (8 rows x 4 heads, head_dim 128: two CTAs with sums in registers 526 us, three with
+    // shared ones 516 us, and with the pieces below 459 and 429 us; 6 rows x 4 heads, head_dim 64: 327 and 266 us).
+    static constexpr bool kSharedSum = RB * HD >= 128 && WR > 1;
+    static constexpr int kMin = !kSharedSum ? 1 : HD == 128 ? 3 : 2;        // CTAs of an SM
+    static constexpr int kStages = kSharedSum && HD == 128 ? 4 : 8; // of the CTA; a warp's own: a quarter
+    static constexpr int kBytes = kStages * PsShape<HD>::kStage + RB * WR * (HD / 16) * 512 + (kSharedSum ? RB * (HD / 8) * 1024 : 0);
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
@@ -68,10 +80,11 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 template <int HD, int FMT, int RB, int WR>
-__global__ void __launch_bounds__(WR == 1 ? 128 : 160) paged_stream_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) paged_stream_kernel(const PagedAttnParams p) {
     using F = KvFormat<FMT>;
     using S = PsShape<HD>;
-    constexpr int WK = 4 / WR, RT = 8 * RB * WR, KS = HD / 16, NB = HD / 8, PR = HD + 4, NS = S::kStages;
+    constexpr int WK = 4 / WR, RT = 8 * RB * WR, KS = HD / 16, NB = HD / 8, PR = HD + 4, NS = PsCta<HD, RB, WR>::kStages;
+    constexpr bool SS = PsCta<HD, RB, WR>::kSharedSum;
     constexpr int U = RB * HD >= 256 ? 1 : 2; // products of 16 keys that go through the softmax together
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem;
@@ -193,7 +206,13 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160) paged_stream_kernel(const
 
         float m[RB], l[RB], c[RB];
         float o[RB][NB][4]; // the tensor cores' sums, a plane in each half
-        float2 sum[RB][NB]; // columns 2t and 2t + 1 of every block: what was folded
+        // columns 2t and 2t + 1 of every block: what was folded
+        float2 *ssum = reinterpret_cast<float2 *>(sq + RB * WR * KS * 32) + tid;
+        float2 rsum[RB][SS ? 1 : NB];
+        const auto sum = [&](int rb, int j) -> float2 & {
+            if constexpr (SS) return ssum[(rb * NB + j) * 128];
+            else return rsum[rb][j];
+        };
         int lo[RB], span[RB], R[RB]; // o holds sums of p v in units of 2^R
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
@@ -209,7 +228,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160) paged_stream_kernel(const
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
                 o[rb][j][0] = o[rb][j][1] = o[rb][j][2] = o[rb][j][3] = 0.0f;
-                sum[rb][j] = make_float2(0.0f, 0.0f);
+                sum(rb, j) = make_float2(0.0f, 0.0f);
             }
         }
         int held = 0; // stages in o
@@ -218,7 +237,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160) paged_stream_kernel(const
             for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
-                    sum[rb][j] = __fadd2_rn(sum[rb][j], __fadd2_rn(make_float2(o[rb][j][0], o[rb][j][1]), make_float2(o[rb][j][2], o[rb][j][3])));
+                    sum(rb, j) = __fadd2_rn(sum(rb, j), __fadd2_rn(make_float2(o[rb][j][0], o[rb][j][1]), make_float2(o[rb][j][2], o[rb][j][3])));
                     o[rb][j][0] = o[rb][j][1] = o[rb][j][2] = o[rb][j][3] = 0.0f;
                 }
             held = 0;
@@ -345,7 +364,8 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160) paged_stream_kernel(const
                     mn[rb] = fmaxf(mn[rb], __shfl_xor_sync(0xffffffffu, mn[rb], 1));
                     mn[rb] = fmaxf(mn[rb], __shfl_xor_sync(0xffffffffu, mn[rb], 2));
                     mn[rb] = fmaxf(mn[rb], m[rb]);
-                    moved |= mn[rb] > m[rb];
+                    moved |= mn[rb] > m[rb] + kPsLazy;
+                    mn[rb] = mn[rb] > m[rb] + kPsLazy ? mn[rb] : m[rb];
                 }
                 if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -359,7 +379,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160) paged_stream_kernel(const
 #pragma unroll
                         for (int j = 0; j < NB; ++j) {
                             o[rb][j][0] *= f, o[rb][j][1] *= f, o[rb][j][2] *= f, o[rb][j][3] *= f;
-                            sum[rb][j] = __fmul2_rn(sum[rb][j], make_float2(f, f));
+                            sum(rb, j) = __fmul2_rn(sum(rb, j), make_float2(f, f));
                         }
                     }
                 }
@@ -398,7 +418,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160) paged_stream_kernel(const
 #pragma unroll
                         for (int j = 0; j < NB; ++j) {
                             o[rb][j][0] *= f, o[rb][j][1] *= f, o[rb][j][2] *= f, o[rb][j][3] *= f;
-                            sum[rb][j] = __fmul2_rn(sum[rb][j], make_float2(f, f));
+                            sum(rb, j) = __fmul2_rn(sum(rb, j), make_float2(f, f));
                         }
                     }
                 }
@@ -523,10 +543,10 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160) paged_stream_kernel(const
 #pragma unroll
                 for (int j = 0; j < NB; j += 4) {
                     float4 v;
-                    v.x = (h ? sum[rb][j].y : sum[rb][j].x) * kDown * unit;
-                    v.y = (h ? sum[rb][j + 1].y : sum[rb][j + 1].x) * kDown * unit;
-                    v.z = (h ? sum[rb][j + 2].y : sum[rb][j + 2].x) * kDown * unit;
-                    v.w = (h ? sum[rb][j + 3].y : sum[rb][j + 3].x) * kDown * unit;
+                    v.x = (h ? sum(rb, j).y : sum(rb, j).x) * kDown * unit;
+                    v.y = (h ? sum(rb, j + 1).y : sum(rb, j + 1).x) * kDown * unit;
+                    v.z = (h ? sum(rb, j + 2).y : sum(rb, j + 2).x) * kDown * unit;
+                    v.w = (h ? sum(rb, j + 3).y : sum(rb, j + 3).x) * kDown * unit;
                     *reinterpret_cast<float4 *>(part + row * PR + (2 * t + h) * NB + j) = v;
                 }
         }
@@ -636,16 +656,20 @@ static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
     const int64_t rows = (int64_t)d->max_new * (d->num_heads / d->cache.num_kv_heads);
     const int64_t units = (int64_t)d->batch * d->cache.num_kv_heads;
     int64_t s = d->splits;
-    // 64 caches of 1.5 to 8 k keys, 8 kv heads, head_dim 64 / 128: 32 rows 339 / 551 us streamed, 395 / 623 us as a chunk;
-    // 48 rows 630 / 882 us and 396 / 640 us (a streaming CTA's warps each read all keys once more for every 8 or 16 rows).
+    // 64 caches of 1.5 to 8 k keys, 8 kv heads, head_dim 64 / 128: 32 rows 266 / 426 us streamed, 395 / 623 us as a chunk;
+    // 48 rows 406 / 731 us and 401 / 647 us (a streaming CTA's warps each read all keys once more for every 8 or 16 rows).
     pl.chunk = rows > 32;
     if (pl.chunk) {
         pl.rb = pl.wr = 0;
         pl.row_tiles = (int)((rows + 255) / 256);
         if (s == 0) {
-            // one CTA an SM: the number of pieces (of at least 1024 keys) that leaves the fewest SMs idle in the last wave
+            // One CTA an SM: the number of pieces (of at least 1024 keys) that leaves the fewest SMs idle in the last wave;
+            // one, where tiles of a sequence are three waves by themselves (a prompt of 8 k rows x 16 heads, 512 CTAs, in
+            // 1 / 2 / 4 pieces: 346 / 400 / 467 us; ragged chunks 324 / 332 / 385 us; 2048 rows behind 30 k keys, 128
+            // CTAs, in 1 / 8 pieces: 672 / 646 us).
+            const int64_t most = pl.row_tiles > 1 && units * pl.row_tiles >= 148 * 3 ? 1 : 8;
             double best = 0.0;
-            for (int64_t c = 1; c <= 8 && (c == 1 || d->max_len / c >= 1024); ++c) {
+            for (int64_t c = 1; c <= most && (c == 1 || d->max_len / c >= 1024); ++c) {
                 const int64_t ctas = units * pl.row_tiles * c, waves = (ctas + 147) / 148;
                 const double use = (double)ctas / (double)(waves * 148) - 0.01 * (double)(c - 1);
                 if (use > best) {
@@ -656,16 +680,21 @@ static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
         }
     } else {
         // Two blocks of 8 rows a warp while their output (64 registers a block at head_dim 128) leaves room for more than
-        // one CTA on an SM: at 128 one block (block of 8 rows x 4 heads over 64 caches: 557 us, two blocks 708 us).
+        // one CTA on an SM: at 128 one block (two of them took 708 us where one took 557, before the sums
+        // moved to shared memory).
         pl.rb = rows <= 8 || d->cache.head_dim == 128 ? 1 : 2;
         pl.wr = rows <= 8 * pl.rb ? 1 : rows <= 16 * pl.rb ? 2 : 4; // 4: head_dim 128 alone, 17 .. 32 rows
         const int rt = 8 * pl.rb * pl.wr;
         pl.row_tiles = (int)((rows + rt - 1) / rt);
         if (s == 0) {
-            const int64_t ctas = units * pl.row_tiles, target = 148 * 4;
-            s = ctas >= target ? 1 : target / ctas;
-            const int64_t cap = d->max_len / 256; // a piece is worth a few stages
-            if (s > cap) s = cap;
+            // The GPU is filled first, as long as a piece is worth a few stages; sequences of different lengths then want
+            // many times as many CTAs as run at once, as long as a piece has 512 KB of keys and values. Blocks of 8 rows x
+            // 4 heads over 64 caches of 1.5 to 8 k keys, head_dim 128, in 1 / 2 / 4 / 8 pieces: 526 / 444 / 414 / 424 us;
+            // 512 pieces of head_dim 64: 160 / 143 / 147 / 174 us; one token over 4 k keys: 55 / 59 us in 1 / 2 pieces.
+            const int64_t ctas = units * pl.row_tiles, key_max = d->max_len, worth = 256 * 1024 / d->cache.head_dim;
+            const int64_t fill = std::min((int64_t)148 * 4 / ctas, key_max / 256);
+            const int64_t even = std::min(((int64_t)148 * 14 + ctas - 1) / ctas, key_max / worth);
+            s = std::max(fill, even);
         }
     }
     pl.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
@@ -675,8 +704,8 @@ static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
 
 template <int HD, int FMT, int RB, int WR>
 static int launch_stream_t(const PagedAttnParams &p, cudaStream_t s) {
-    constexpr int smem = PsShape<HD>::kStages * PsShape<HD>::kStage + RB * WR * (HD / 16) * 512;
-    static_assert(4 / WR * 8 * RB * WR * (HD + 4) * 4 <= smem, "the merge area fits the ring");
+    constexpr int smem = PsCta<HD, RB, WR>::kBytes;
+    static_assert(4 / WR * 8 * RB * WR * (HD + 4) * 4 <= PsCta<HD, RB, WR>::kStages * PsShape<HD>::kStage, "the merge area fits the ring");
     static std::atomic<uint64_t> done{0};
     if (const int st = allow_smem((const void *)paged_stream_kernel<HD, FMT, RB, WR>, smem, done)) return st;
     const dim3 grid((unsigned)p.pv.kvh, (unsigned)p.splits, (unsigned)(p.batch * p.row_tiles));

@@ -20,7 +20,7 @@
 // Q's planes are TMEM operands (head_dim 128: the first one; the other stays in shared memory).
 //
 // Measured (B200): 2048 new rows x 16 heads, head_dim 64, behind 31 k keys: 641-657 us, 400 TFLOP/s of the formula's
-// products and twice that on the tensor cores (two planes); ragged chunks at head_dim 128: 326-331 us. What bounds it is
+// products and twice that on the tensor cores (two planes); ragged chunks at head_dim 128: 324-331 us. What bounds it is
 // the chain of one query tile: a step of 128 keys takes 4960 cycles, of which its 512 exponentials a scheduler 2150
 // (8 cycles a warp instruction), the wait for P V and the next S 1250, reading scores and their maximum 470, rescaling 450,
 // folding 330 (head_dim 128, whose sums fold into output rows: 850). Issue slots are 46 %, tensor cores 35 % busy (small
