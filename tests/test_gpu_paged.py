@@ -648,3 +648,86 @@ def test_bindings_refuse_wrong_tensors(cuda_lib):
     d.device = 1  # as if the tensors were on another device than the current one
     with pytest.raises(ValueError):
         ops.paged_append(d)
+
+
+# ------------------------------------------------------------------------------------------------ long launches
+
+@pytest.mark.parametrize("hd,heads,kv,rows", [(32, 1, 1, 4001), (64, 16, 4, 7301), (128, 5, 3, 3600), (64, 2, 7, 15000)])
+def test_a_long_launch_gives_what_short_ones_give(cuda_lib, hd, heads, kv, rows):
+    """CTAs that take several rows and share heads and rows among their threads: the bits of launches of a row a CTA."""
+    g = gen(rows)
+    cuts = np.unique(np.concatenate([[0, rows], np.random.default_rng(rows).integers(1, rows, 23)]))
+    new = np.diff(cuts).tolist()
+    base = [7 * b % 50 for b in range(len(new))]
+    caches = [make_cache(95, "int8", [b + n for b, n in zip(base, new)], kv, hd, 16) for _ in range(2)]
+    qkv = randn(g, rows, (heads + 2 * kv) * hd)
+    q, k, v = qkv[:, :heads * hd], qkv[:, heads * hd:(heads + kv) * hd], qkv[:, (heads + kv) * hd:]
+    cos, sin = tables(4000, hd)  # some positions lie outside of them
+    gain = 1 + 0.3 * randn(g, hd)
+    outs = [torch.full((rows + 2, heads * hd), 7.0, device="cuda") for _ in range(2)]
+
+    def append(c, lo, hi, out):  # sequences lo .. hi
+        a, b = int(cuts[lo]), int(cuts[hi])
+        part = ops.PagedKvCache(c.k_codes, c.v_codes, c.k_exp, c.v_exp, c.page_table[lo:hi], c.fmt)
+        ops.paged_append(ops.make_paged_append(part, cu(new[lo:hi]), i32(base[lo:hi]), k[a:b], v[a:b], q=q[a:b], num_heads=heads,
+                                               q_out=out[1 + a:1 + b], q_gain=gain, k_gain=gain, eps=1e-6, rope_cos=cos, rope_sin=sin))
+
+    append(caches[0], 0, len(new), outs[0])
+    for i in range(len(new)):
+        append(caches[1], i, i + 1, outs[1])
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[1]) and bool((outs[0][0] == 7).all() and (outs[0][-1] == 7).all())
+    for name in ("k_codes", "v_codes", "k_exp", "v_exp"):
+        assert torch.equal(getattr(caches[0], name), getattr(caches[1], name)), name
+    c = caches[0]
+    ko, vo = (torch.full((rows + 2, kv * hd), 7.0, device="cuda") for _ in range(2))
+    ops.paged_read(ops.make_paged_read(c, cu(new), ko[1:-1], vo[1:-1], start=i32(base)))
+    only = torch.full((rows + 2, kv * hd), 7.0, device="cuda")
+    ops.paged_read(ops.make_paged_read(c, cu(new), None, only[1:-1], start=i32(base)))
+    torch.cuda.synchronize()
+    assert torch.equal(vo, only)
+    for o, w in ((ko, "k"), (vo, "v")):
+        want = torch.cat([stored(c, b, p + n, w)[p:].flatten(1) for b, (n, p) in enumerate(zip(new, base))])
+        assert torch.equal(o[1:-1].double().cpu(), want) and bool((o[0] == 7).all() and (o[-1] == 7).all())
+    pos = torch.randint(-5, 4100, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    long, short = torch.empty(rows, heads * hd, device="cuda"), torch.empty(rows, heads * hd, device="cuda")
+    ops.qk_norm_rope(ops.make_qk_norm_rope(q, None, pos, heads, 0, hd, q_out=long, q_gain=gain, eps=1e-6, rope_cos=cos, rope_sin=sin))
+    for a in range(0, rows, 1000):
+        b = min(rows, a + 1000)
+        ops.qk_norm_rope(ops.make_qk_norm_rope(q[a:b], None, pos[a:b], heads, 0, hd, q_out=short[a:b], q_gain=gain, eps=1e-6,
+                                               rope_cos=cos, rope_sin=sin))
+    torch.cuda.synchronize()
+    assert torch.equal(long, short)
+
+
+@pytest.mark.parametrize("hd,n", [(128, 1), (128, 3), (128, 8), (64, 6), (64, 8), (32, 8)])
+@pytest.mark.parametrize("step", [0.02, 0.4])
+@pytest.mark.parametrize("falling", [False, True])
+def test_scores_that_rise_or_fall_slowly(cuda_lib, hd, n, step, falling):
+    """Every key a little above the one before it (a maximum that grows by less than the rescaling waits for), or below."""
+    heads, kv, base = 4, 1, 700
+    L_ = base + n
+    c = make_cache(97, "int8", [L_], kv, hd, 16)
+    u = torch.ones(hd, device="cuda")
+    ramp = torch.arange(L_, device="cuda").float() * step / hd
+    k = (ramp.flip(0) if falling else ramp)[:, None] * u
+    v = randn(gen(98), L_, hd)
+    ops.paged_append(ops.make_paged_append(c, cu([L_]), i32([0]), k.contiguous(), v))
+    q = u.repeat(heads)[None, :] * (1 + 0.1 * torch.arange(n, device="cuda").float()[:, None])
+    for splits in (1, 3):
+        _, out = attend(c, [n], [base], heads, 0, q=q.contiguous(), scale=1.0, splits=splits)
+        check_attention(c, q, out, [n], [base], heads, scale=1.0)
+
+
+@pytest.mark.parametrize("hd,heads,kv,batch,new,max_len", [
+    (128, 32, 8, 75, 8, 8192), (64, 16, 4, 160, 5, 12000), (64, 8, 4, 41, 300, 4096)])
+def test_many_short_sequences_in_a_launch_planned_for_long_ones(cuda_lib, hd, heads, kv, batch, new, max_len):
+    """Pieces without a key, and tiles that are not split: the plan follows max_len and the batch, not the lengths."""
+    base = [(37 * b) % 200 for b in range(batch)]
+    news = [new if b % 3 else new // 2 for b in range(batch)]
+    lens = [b + n for b, n in zip(base, news)]
+    c = make_cache(99, "e4m3", lens, kv, hd, 32)
+    fill_cache(c, 100, lens)
+    q, out = attend(c, news, base, heads, 101, max_new=new, max_len=max_len)
+    assert c.status_bits() == 0
+    check_attention(c, q, out, news, base, heads)
