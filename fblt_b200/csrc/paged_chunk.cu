@@ -131,6 +131,19 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
     const int st0 = min(steps, split * per), nst = min(steps, st0 + per) - st0;
     const int kb0 = first + st0 * BN;
     const uint32_t sbase = smem_u32(smem);
+    // A piece without a key: zeros, of weight 0 where pieces are merged. It is left before anything is staged: the products,
+    // which order a warp's use of the shared memory that another one's query rows came through, are what such a piece lacks.
+    if (nst == 0) {
+        const int here = min(2 * kPcRows, rows - row0);
+        for (int it = tid; it < here * (HD / 4); it += kPcThreads) {
+            const int r = row0 + it / (HD / 4), d = it % (HD / 4) * 4, i = r / p.G, head = kvh * p.G + (r - i * p.G);
+            float *dst = p.splits > 1 ? p.ws + (((int64_t)(r0 + i) * p.H + head) * p.splits + split) * PR
+                                      : p.out + (int64_t)(r0 + i) * p.os + (int64_t)head * HD;
+            *reinterpret_cast<float4 *>(dst + d) = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (p.splits > 1 && d == 0) *reinterpret_cast<float2 *>(dst + HD) = make_float2(-INFINITY, 0.0f);
+        }
+        return;
+    }
 
     auto give_up = [&](unsigned code) {
         *(volatile int *)&s_abort = 1;
@@ -254,7 +267,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             };
             float m = -INFINITY, l = 0.0f;
             int R = 0;
-            bool ok = nst == 0 || mbar_wait_abort(&bars.kv_full[0], 0, abortp);
+            bool ok = mbar_wait_abort(&bars.kv_full[0], 0, abortp);
             if (!ok && lane == 0) give_up(0x55);
             for (int j = 0; j < nst && ok; ++j) { // the tile's scales are there: waited for at the end of the step before
                 const int st = j & 1, kb = kb0 + j * BN;
@@ -425,7 +438,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                     ok = false;
                 }
             }
-            if (ok && nst > 0 && !mbar_wait_abort(&bars.o_full, 0, abortp)) {
+            if (ok && !mbar_wait_abort(&bars.o_full, 0, abortp)) {
                 if (lane == 0) give_up(0x52);
                 ok = false;
             }
@@ -447,10 +460,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) {
                     float o[32];
-                    if (nst > 0) {
-                        tmem_ld32(trow + S::kO + c * 32, o);
-                        tc_wait_ld();
-                    }
+                    tmem_ld32(trow + S::kO + c * 32, o);
+                    tc_wait_ld();
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const float4 w = v[8 * c + k];
@@ -590,7 +601,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 __syncwarp();
             };
             bool ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.q_full, 0, abortp));
-            if (ok && nst > 0) {
+            if (ok) {
                 ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.kv_full[0], 0, abortp));
                 if (ok) {
                     tc_fence_after();

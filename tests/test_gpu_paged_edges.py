@@ -1,0 +1,58 @@
+"""The paged cache's operators where they could go wrong between calls of their ordinary tests: pieces and tiles without
+keys, stages that are used again, scales at both ends of fp32, limits of a launch, and precision over long ranges."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as R
+from fblt_b200 import lib as L
+from fblt_b200 import ops
+from test_gpu_paged import attend, check_attention, cu, fill_cache, gen, i32, make_cache, randn
+
+pytestmark = pytest.mark.gpu
+
+FMTS = ["e4m3", "int8"]
+
+
+# ------------------------------------------------------------------------------------------------ pieces without keys
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd,heads,kv", [(32, 8, 2), (64, 8, 2), (128, 8, 2), (64, 2, 2)])
+@pytest.mark.parametrize("new,base,splits", [([300, 70, 0, 150], [0, 9, 4, 2100], 8), ([129, 257], [0, 3000], 5)])
+def test_queries_that_are_not_finite_beside_pieces_without_keys(cuda_lib, fmt, hd, heads, kv, new, base, splits):
+    """A prompt's first rows in a launch cut for a long sequence: most pieces have no key. A query row that is not finite
+    gives zeros, and every other row the bits that it has without it."""
+    lens = [b + n for b, n in zip(base, new)]
+    c = make_cache(200, fmt, lens, kv, hd, 48)
+    fill_cache(c, 201, lens)
+    q = randn(gen(202), sum(new), heads * hd)
+    _, want = attend(c, new, base, heads, 0, q=q.clone(), splits=splits)
+    bad = q.clone().view(-1, heads, hd)
+    where = torch.zeros(sum(new), heads, dtype=torch.bool, device="cuda")
+    for r in range(0, sum(new), 3):
+        for h in range(heads):
+            if (r + h) % 4 == 0:
+                bad[r, h, (5 * r + h) % hd] = (math.nan, math.inf, -math.inf)[(r // 3 + h) % 3]
+                where[r, h] = True
+    for _ in range(5):
+        _, got = attend(c, new, base, heads, 0, q=bad.view(-1, heads * hd), splits=splits)
+        got = got.view(-1, heads, hd)
+        assert bool((got[where] == 0).all())
+        assert torch.equal(got[~where], want.view(-1, heads, hd)[~where])
+    check_attention(c, q, want, new, base, heads)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_a_tile_without_any_key(cuda_lib, hd, splits):
+    """Rows whose window has left the page table: zeros, whatever the queries hold."""
+    n, heads = 260, 2
+    c = make_cache(203, "int8", [64], 2, hd, 16, extra_cols=0)
+    fill_cache(c, 204, [64])
+    q = randn(gen(205), n, heads * hd)
+    q[::5, 3], q[1::7, hd + 1] = math.nan, math.inf
+    for _ in range(5):
+        _, out = attend(c, [n], [5000], heads, 0, q=q, window=100, splits=splits)
+        assert bool((out == 0).all()) and c.status_bits() == L.PAGED_BAD_PAGE
