@@ -259,6 +259,8 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
                         *reinterpret_cast<uint4 *>(stage + S::kOffV + grp * S::kPitch + (k % S::kPer) * HD + (i % (HD / 16)) * 16) =
                             make_uint4(0, 0, 0, 0);
                 }
+                // the producer's next bulk copy into this stage goes through the async proxy: it comes behind these stores
+                if (WR > 1) fence_async_smem();
             }
             // ---- scales of the stage's keys; V's relative to the largest, 2^et
             int et = kPsNoUnit;

@@ -56,3 +56,26 @@ def test_a_tile_without_any_key(cuda_lib, hd, splits):
     for _ in range(5):
         _, out = attend(c, [n], [5000], heads, 0, q=q, window=100, splits=splits)
         assert bool((out == 0).all()) and c.status_bits() == L.PAGED_BAD_PAGE
+
+
+# ------------------------------------------------------------------------------------------------ stages that are used again
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd,heads,kv,new", [(32, 4, 1, 5), (64, 4, 1, 6), (64, 8, 2, 8), (128, 4, 2, 6), (128, 4, 1, 4), (128, 4, 1, 8)])
+@pytest.mark.parametrize("window", [0, 1003, 2041])
+def test_stages_whose_values_were_cleared_are_used_again(cuda_lib, fmt, hd, heads, kv, new, window):
+    """Warps that share keys: the first stage of a window and the stages around a missing page hold cleared rows of V, and
+    their shared memory takes the keys of later stages, many times over."""
+    news, base = [new, new - 1, new], [2500, 2077, 1300]
+    lens = [b + n for b, n in zip(base, news)]
+    c = make_cache(210, fmt, lens, kv, hd, 16)
+    fill_cache(c, 211, lens)
+    gone = [(0, 1600, 1616), (0, 1680, 1696), (1, 1200, 1216), (2, 16, 32), (2, 640, 656)]
+    keep = c.page_table.clone()
+    for b, lo, _ in gone:
+        c.page_table[b, lo // 16] = -1
+    for _ in range(3):
+        q, out = attend(c, news, base, heads, 212, window=window, splits=1)
+        assert c.status_bits() == L.PAGED_BAD_PAGE
+    c.page_table.copy_(keep)
+    check_attention(c, q, out, news, base, heads, window=window, missing=gone)
