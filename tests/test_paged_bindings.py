@@ -1,0 +1,41 @@
+"""What the torch-side holders of the paged cache refuse, on tensors without memory: no GPU is needed."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from fblt_b200 import ops
+
+pytestmark = pytest.mark.filterwarnings("ignore:Accessing the data pointer")
+
+
+@pytest.fixture(autouse=True)
+def fake():
+    with FakeTensorMode():
+        yield
+
+
+def pool(**device):
+    """The tensors of a cache of 8 pages of 16 positions, 2 kv heads of 64."""
+    on = lambda name: device.get(name, "cuda:0")  # noqa: E731
+    t = {n: torch.empty(8, 2, 16, 64, dtype=torch.uint8, device=on(n)) for n in ("k_codes", "v_codes")}
+    t.update({n: torch.empty(8, 2, 16, dtype=torch.int8, device=on(n)) for n in ("k_exp", "v_exp")})
+    t["page_table"] = torch.empty(3, 4, dtype=torch.int32, device=on("page_table"))
+    return t
+
+
+def test_page_tables_whose_rows_overlap_are_refused():
+    t = pool()
+    row = torch.empty(1, 4, dtype=torch.int32, device="cuda")
+    for table in (row.expand(3, 4), torch.empty(12, dtype=torch.int32, device="cuda").as_strided((3, 4), (3, 1))):
+        with pytest.raises(ValueError, match="page_table"):
+            ops.PagedKvCache(**{**t, "page_table": table}, fmt="int8")
+
+
+def test_page_tables_that_are_accepted():
+    t = pool()
+    wide = torch.empty(6, 9, dtype=torch.int32, device="cuda")
+    for table, stride in ((wide[:, :4], 9), (wide[::2, 2:6], 18), (wide[:1, :4], 9), (wide[:3, :0], 9),
+                          (torch.empty(1, 1, dtype=torch.int32, device="cuda").expand(1, 1), 1),
+                          (torch.empty(4, dtype=torch.int32, device="cuda").as_strided((1, 4), (1, 1)), 4)):
+        c = ops.PagedKvCache(**{**t, "page_table": table}, fmt="e4m3")
+        assert (c.batch, c.desc.max_pages, c.desc.page_table_stride) == (*table.shape, stride)
