@@ -619,6 +619,8 @@ class PagedKvCache:
             raise ValueError("page_table: a CUDA int32 [batch, max_pages] tensor with unit column stride is needed")
         if page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
             raise ValueError("page_table: rows that overlap (an expanded table); every sequence needs a row of its own")
+        if len({t.device for t in (k_codes, v_codes, k_exp, v_exp, page_table)}) != 1:
+            raise ValueError("codes, exponents and page_table: tensors on different devices")
         self.k_codes, self.v_codes, self.k_exp, self.v_exp, self.page_table, self.fmt = k_codes, v_codes, k_exp, v_exp, page_table, fmt
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = (int(n) for n in shape)
         self.batch = int(page_table.shape[0])

@@ -39,3 +39,9 @@ def test_page_tables_that_are_accepted():
                           (torch.empty(4, dtype=torch.int32, device="cuda").as_strided((1, 4), (1, 1)), 4)):
         c = ops.PagedKvCache(**{**t, "page_table": table}, fmt="e4m3")
         assert (c.batch, c.desc.max_pages, c.desc.page_table_stride) == (*table.shape, stride)
+
+
+@pytest.mark.parametrize("name", ["k_codes", "v_codes", "k_exp", "v_exp", "page_table"])
+def test_a_cache_lies_on_one_device(name):
+    with pytest.raises(ValueError, match="device"):
+        ops.PagedKvCache(**pool(**{name: "cuda:1"}), fmt="int8")
