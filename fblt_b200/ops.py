@@ -754,8 +754,10 @@ def paged_attn_workspace(d: L.PagedAttnDesc) -> Optional[torch.Tensor]:
 
 
 def paged_attn(d: L.PagedAttnDesc, workspace: Optional[torch.Tensor] = None, stream=None) -> None:
+    if workspace is not None and not (workspace.is_cuda and workspace.device.index == d.device and workspace.is_contiguous()):
+        raise ValueError(f"workspace: a contiguous tensor on device {d.device} is needed")
     wp = workspace.data_ptr() if workspace is not None else None
-    wn = workspace.numel() if workspace is not None else 0
+    wn = workspace.numel() * workspace.element_size() if workspace is not None else 0
     L.check(L.load().fblt_paged_attn(C.byref(d), wp, wn, _stream_on(d, stream)))
 
 

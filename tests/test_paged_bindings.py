@@ -45,3 +45,18 @@ def test_page_tables_that_are_accepted():
 def test_a_cache_lies_on_one_device(name):
     with pytest.raises(ValueError, match="device"):
         ops.PagedKvCache(**pool(**{name: "cuda:1"}), fmt="int8")
+
+
+def attn(cache, rows=3):
+    i32 = lambda n: torch.empty(n, dtype=torch.int32, device="cuda")  # noqa: E731
+    q, out = (torch.empty(rows, 256, device="cuda") for _ in range(2))
+    return ops.make_paged_attn(cache, i32(4), i32(3), q, out, 4, 1, 64, 0.125, splits=4)
+
+
+def test_workspaces_elsewhere_are_refused():
+    d = attn(ops.PagedKvCache(**pool(), fmt="int8"))
+    byte = dict(dtype=torch.uint8)
+    for ws in (torch.empty(1 << 20, device="cpu", **byte), torch.empty(1 << 20, device="cuda:1", **byte),
+               torch.empty(1 << 21, device="cuda", **byte)[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            ops.paged_attn(d, ws)
