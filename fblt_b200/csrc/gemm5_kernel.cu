@@ -504,19 +504,27 @@ extern "C" int fblt_matmul_pack_weights(const float *b, int64_t ldb, int64_t K, 
 }
 
 namespace fblt {
-static int matmul_impl(const float *a, int64_t lda, const void *packed_b, const float *bias, float *out, int64_t ldo,
-                       int64_t M, int64_t K, int64_t N, int32_t precision, void *stream, const QkvScatter &sc) {
-    if (M < 0 || K <= 0 || N <= 0 || lda < K || (sc.enabled != 1 && ldo < N)) return fail(FBLT_ERR_ARG, "matmul: bad shape or stride");
+// What a product's arguments are refused for.
+int matmul_check(const float *a, int64_t lda, const void *packed_b, const float *out, int64_t ldo, int64_t M, int64_t K, int64_t N) {
+    if (M < 0 || K <= 0 || N <= 0 || lda < K || ldo < N) return fail(FBLT_ERR_ARG, "matmul: bad shape or stride");
     if (M == 0) return FBLT_OK;
     if (!a || !packed_b || !out) return fail(FBLT_ERR_ARG, "matmul: buffers must not be NULL");
     if ((K & 3) || (lda & 3) || ((uintptr_t)a & 15))
         return fail(FBLT_ERR_UNSUPPORTED, "matmul: K and lda must be multiples of 4 and a 16-byte aligned");
     if ((uintptr_t)packed_b & 15) return fail(FBLT_ERR_ARG, "matmul: packed weights must be 16-byte aligned");
     if (K > (1 << 24) || N > (1 << 24) || M > (int64_t)INT32_MAX) return fail(FBLT_ERR_LIMIT, "matmul: shape too large");
+    if (ceil_div(M, kGM) * ceil_div(N, kGN) > (int64_t)INT32_MAX) return fail(FBLT_ERR_LIMIT, "matmul: too many tiles");
+    return FBLT_OK;
+}
+
+static int matmul_impl(const float *a, int64_t lda, const void *packed_b, const float *bias, float *out, int64_t ldo,
+                       int64_t M, int64_t K, int64_t N, int32_t precision, void *stream, const QkvScatter &sc) {
+    // (the scatter epilogue has row strides of its own)
+    int st = matmul_check(a, lda, packed_b, out, sc.enabled == 1 ? N : ldo, M, K, N);
+    if (st != FBLT_OK || M == 0) return st;
     const int ksteps = (int)ceil_div(K, kGK), ntn = (int)ceil_div(N, kGN);
     const int64_t tiles = ceil_div(M, kGM) * ntn;
-    if (tiles > (int64_t)INT32_MAX) return fail(FBLT_ERR_LIMIT, "matmul: too many tiles");
-    const int st = gemm5_configure();
+    st = gemm5_configure();
     if (st != FBLT_OK) return st;
     const int vec_out = !((ldo & 3) || ((uintptr_t)out & 15) || (bias && ((uintptr_t)bias & 15)));
     CUtensorMap a_map;

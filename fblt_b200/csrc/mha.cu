@@ -13,6 +13,9 @@
 namespace fblt {
 int paged_append_check(const fblt_paged_append_desc *d); // paged_cache.cu
 int paged_attn_check(const fblt_paged_attn_desc *d);     // paged_attn.cu
+int paged_attn_check_call(const fblt_paged_attn_desc *d, const void *workspace, size_t workspace_bytes);
+int matmul_check(const float *a, int64_t lda, const void *packed_b, const float *out, int64_t ldo, int64_t M, int64_t K,
+                 int64_t N); // gemm5_kernel.cu
 } // namespace fblt
 
 namespace fblt {
@@ -231,7 +234,6 @@ extern "C" int fblt_paged_self_attention_step(const fblt_paged_step_desc *d, voi
     w.k = d->qkv_work + E;
     w.v = d->qkv_work + E + d->cache.num_kv_heads * hd;
     w.q_stride = w.q_out_stride = w.k_stride = w.v_stride = W;
-    w.q_out = d->qkv_work;
     w.q_gain = d->q_gain;
     w.k_gain = d->k_gain;
     w.eps = d->eps;
@@ -267,6 +269,11 @@ extern "C" int fblt_paged_self_attention_step(const fblt_paged_step_desc *d, voi
     if (d->input_stride < E || d->output_stride < E) return fail(FBLT_ERR_ARG, "paged step: row strides below embed_dim");
     if (d->max_new < 1) return fail(FBLT_ERR_ARG, "paged step: max_new must bound the new rows");
     if (fblt_paged_attn_workspace(&a) > d->workspace_bytes || !d->workspace) a.splits = 1;
+    if ((st = paged_attn_check_call(&a, d->workspace, d->workspace_bytes)) != FBLT_OK) return st;
+    st = matmul_check(d->input, d->input_stride, d->packed_qkv, d->qkv_work, W, d->total_rows, E, W);
+    if (st != FBLT_OK) return st;
+    st = matmul_check(d->combined_work, E, d->packed_proj, d->output, d->output_stride, d->total_rows, E, E);
+    if (st != FBLT_OK) return st;
 
     st = fblt_matmul(d->input, d->input_stride, d->packed_qkv, nullptr, d->qkv_work, W, d->total_rows, E, W, d->precision, stream);
     if (st != FBLT_OK) return st;

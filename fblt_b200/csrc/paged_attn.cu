@@ -704,6 +704,27 @@ static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
     return pl;
 }
 
+static int paged_plan_check(const fblt_paged_attn_desc *d, const PagedPlan &pl, const void *workspace, size_t workspace_bytes) {
+    if (pl.need > 0) {
+        if (!workspace || workspace_bytes < pl.need)
+            return fail(FBLT_ERR_WORKSPACE, "paged_attn: %zu bytes of workspace needed (fblt_paged_attn_workspace), got %zu", pl.need,
+                        workspace_bytes);
+        if ((uintptr_t)workspace & 15) return fail(FBLT_ERR_ARG, "paged_attn: workspace must be 16-byte aligned");
+    }
+    if ((int64_t)d->batch * pl.row_tiles > 65535)
+        return fail(FBLT_ERR_LIMIT, "paged_attn: batch * row tiles (%d) exceed 65535 per launch", pl.row_tiles);
+    if (pl.splits > 1 && (int64_t)d->total_rows * d->num_heads * (d->cache.head_dim / 4) / 256 >= INT_MAX)
+        return fail(FBLT_ERR_LIMIT, "paged_attn: too many rows to merge in one launch");
+    return FBLT_OK;
+}
+
+// Everything that fblt_paged_attn refuses a call for, for a caller that launches other work before it.
+int paged_attn_check_call(const fblt_paged_attn_desc *d, const void *workspace, size_t workspace_bytes) {
+    const int st = paged_attn_check(d);
+    if (st != FBLT_OK || d->batch == 0 || d->total_rows == 0 || d->max_new == 0) return st;
+    return paged_plan_check(d, paged_plan(d), workspace, workspace_bytes);
+}
+
 template <int HD, int FMT, int RB, int WR>
 static int launch_stream_t(const PagedAttnParams &p, cudaStream_t s) {
     constexpr int smem = PsCta<HD, RB, WR>::kBytes;
@@ -757,16 +778,7 @@ extern "C" int fblt_paged_attn(const fblt_paged_attn_desc *d, void *workspace, s
     if (st != FBLT_OK) return st;
     if (d->batch == 0 || d->total_rows == 0 || d->max_new == 0) return FBLT_OK;
     const PagedPlan pl = paged_plan(d);
-    if (pl.need > 0) {
-        if (!workspace || workspace_bytes < pl.need)
-            return fail(FBLT_ERR_WORKSPACE, "paged_attn: %zu bytes of workspace needed (fblt_paged_attn_workspace), got %zu", pl.need,
-                        workspace_bytes);
-        if ((uintptr_t)workspace & 15) return fail(FBLT_ERR_ARG, "paged_attn: workspace must be 16-byte aligned");
-    }
-    if ((int64_t)d->batch * pl.row_tiles > 65535)
-        return fail(FBLT_ERR_LIMIT, "paged_attn: batch * row tiles (%d) exceed 65535 per launch", pl.row_tiles);
-    if (pl.splits > 1 && (int64_t)d->total_rows * d->num_heads * (d->cache.head_dim / 4) / 256 >= INT_MAX)
-        return fail(FBLT_ERR_LIMIT, "paged_attn: too many rows to merge in one launch");
+    if ((st = paged_plan_check(d, pl, workspace, workspace_bytes)) != FBLT_OK) return st;
     PagedAttnParams p;
     memset(&p, 0, sizeof(p));
     p.pv = paged_view(d->cache);
