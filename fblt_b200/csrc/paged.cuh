@@ -180,6 +180,23 @@ struct PagedAttnParams {
     float qscale; // scale * log2(e)
 };
 
+// A CTA's place: kv heads of a piece side by side, then the pieces, then (sequence, tile of rows) -- in one dimension of the
+// grid, whose other two end at 65535.
+struct PagedCtaAt {
+    int kvh, split, unit;
+};
+__device__ __forceinline__ PagedCtaAt paged_cta(const PagedAttnParams &p) {
+    PagedCtaAt at;
+    const unsigned r = blockIdx.x / (unsigned)p.pv.kvh;
+    at.kvh = (int)(blockIdx.x - r * (unsigned)p.pv.kvh);
+    at.unit = (int)(r / (unsigned)p.splits);
+    at.split = (int)(r - (unsigned)at.unit * (unsigned)p.splits);
+    return at;
+}
+inline unsigned paged_grid(const PagedAttnParams &p) { // paged_plan_check: fits
+    return (unsigned)((int64_t)p.pv.kvh * p.splits * p.batch * p.row_tiles);
+}
+
 // Keys that rows [row0, row0 + rows) of a sequence with n new rows at `base` see between them. Positions beyond the page
 // table hold no key, and however large a length is, nothing walks past them (nor past where a stage's last key would leave
 // 32 bits).

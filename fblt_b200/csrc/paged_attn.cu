@@ -96,15 +96,16 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
     __shared__ int s_abort;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int kvh = blockIdx.x, split = blockIdx.y, b = blockIdx.z / p.row_tiles, rt = blockIdx.z - b * p.row_tiles;
+    const PagedCtaAt at = paged_cta(p);
+    const int kvh = at.kvh, split = at.split, b = at.unit; // one tile of rows: the plan's RT holds them all
     int r0, n, base;
     if (!paged_seq(p.pv, p.cu, p.base, p.total, b, r0, n, base)) return;
     if (n > p.max_new) {
         if (tid == 0) p.pv.raise(FBLT_PAGED_BAD_LENGTH);
     }
-    const int rows = min(n, p.max_new) * p.G, row0 = rt * RT;
-    if (row0 >= rows) return;
-    const RowRange rr = tile_range(p, base, n, row0, min(RT, rows - row0));
+    const int rows = min(n, p.max_new) * p.G;
+    if (rows == 0) return;
+    const RowRange rr = tile_range(p, base, n, 0, rows);
     // this split's stages (a stage starts at a multiple of 16, a page too)
     const int first = rr.lo & ~15, stages = (rr.hi - first + S::kKeys - 1) / S::kKeys, per = (stages + p.splits - 1) / p.splits;
     const int st0 = min(stages, split * per), nst = min(stages, st0 + per) - st0;
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
         const int g = lane >> 2, t = lane & 3, wr = warp / WK, wk = warp % WK;
         // query fragments: a warp per block of 8 rows; row g's values at this lane's head_dim positions
         for (int rb = warp; rb < RB * WR; rb += 4) {
-            const int r = row0 + rb * 8 + g;
+            const int r = rb * 8 + g;
             float4 x[KS];
             float a = 0.0f;
             const bool live = r < rows;
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             // a row past the last one has zeros for a query and sees what the last one sees; it is not written
-            const int ri = (wr * RB + rb) * 8 + g, pos = base + min(row0 + ri, rows - 1) / p.G;
+            const int ri = (wr * RB + rb) * 8 + g, pos = base + min(ri, rows - 1) / p.G;
             const int hi = p.block_mode ? base + n : pos + 1;
             lo[rb] = p.block_mode || p.window <= 0 ? 0 : max(0, pos - p.window + 1);
             span[rb] = hi - lo[rb];
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (WR > 1 && *(volatile int *)&s_abort) return;
         for (int it = tid; it < RT * (HD / 4); it += 128) {
-            const int ri = it / (HD / 4), d = (it - ri * (HD / 4)) * 4, r = row0 + ri;
+            const int ri = it / (HD / 4), d = (it - ri * (HD / 4)) * 4, r = ri;
             if (r >= rows) continue;
             float M = -INFINITY;
 #pragma unroll
@@ -686,14 +687,13 @@ static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
         // moved to shared memory).
         pl.rb = rows <= 8 || d->cache.head_dim == 128 ? 1 : 2;
         pl.wr = rows <= 8 * pl.rb ? 1 : rows <= 16 * pl.rb ? 2 : 4; // 4: head_dim 128 alone, 17 .. 32 rows
-        const int rt = 8 * pl.rb * pl.wr;
-        pl.row_tiles = (int)((rows + rt - 1) / rt);
+        pl.row_tiles = 1;
         if (s == 0) {
             // The GPU is filled first, as long as a piece is worth a few stages; sequences of different lengths then want
             // many times as many CTAs as run at once, as long as a piece has 512 KB of keys and values. Blocks of 8 rows x
             // 4 heads over 64 caches of 1.5 to 8 k keys, head_dim 128, in 1 / 2 / 4 / 8 pieces: 526 / 444 / 414 / 424 us;
             // 512 pieces of head_dim 64: 160 / 143 / 147 / 174 us; one token over 4 k keys: 55 / 59 us in 1 / 2 pieces.
-            const int64_t ctas = units * pl.row_tiles, key_max = d->max_len, worth = 256 * 1024 / d->cache.head_dim;
+            const int64_t ctas = units, key_max = d->max_len, worth = 256 * 1024 / d->cache.head_dim;
             const int64_t fill = std::min((int64_t)148 * 4 / ctas, key_max / 256);
             const int64_t even = std::min(((int64_t)148 * 14 + ctas - 1) / ctas, key_max / worth);
             s = std::max(fill, even);
@@ -711,8 +711,10 @@ static int paged_plan_check(const fblt_paged_attn_desc *d, const PagedPlan &pl, 
                         workspace_bytes);
         if ((uintptr_t)workspace & 15) return fail(FBLT_ERR_ARG, "paged_attn: workspace must be 16-byte aligned");
     }
-    if ((int64_t)d->batch * pl.row_tiles > 65535)
-        return fail(FBLT_ERR_LIMIT, "paged_attn: batch * row tiles (%d) exceed 65535 per launch", pl.row_tiles);
+    // at most 65535 * 2^22 tiles * 64 pieces * 1024 heads
+    if ((int64_t)d->batch * pl.row_tiles * pl.splits * d->cache.num_kv_heads > INT_MAX)
+        return fail(FBLT_ERR_LIMIT, "paged_attn: batch * row tiles (%d) * pieces (%d) * kv heads exceed 2^31 - 1 per launch", pl.row_tiles,
+                    pl.splits);
     if (pl.splits > 1 && (int64_t)d->total_rows * d->num_heads * (d->cache.head_dim / 4) / 256 >= INT_MAX)
         return fail(FBLT_ERR_LIMIT, "paged_attn: too many rows to merge in one launch");
     return FBLT_OK;
@@ -731,8 +733,7 @@ static int launch_stream_t(const PagedAttnParams &p, cudaStream_t s) {
     static_assert(4 / WR * 8 * RB * WR * (HD + 4) * 4 <= PsCta<HD, RB, WR>::kStages * PsShape<HD>::kStage, "the merge area fits the ring");
     static std::atomic<uint64_t> done{0};
     if (const int st = allow_smem((const void *)paged_stream_kernel<HD, FMT, RB, WR>, smem, done)) return st;
-    const dim3 grid((unsigned)p.pv.kvh, (unsigned)p.splits, (unsigned)(p.batch * p.row_tiles));
-    paged_stream_kernel<HD, FMT, RB, WR><<<grid, WR == 1 ? 128 : 160, smem, s>>>(p);
+    paged_stream_kernel<HD, FMT, RB, WR><<<paged_grid(p), WR == 1 ? 128 : 160, smem, s>>>(p);
     count_launch();
     return check_launch("paged_stream_kernel");
 }

@@ -118,8 +118,9 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
     const volatile int *abortp = &s_abort;
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int kvh = blockIdx.x, split = blockIdx.y, b = blockIdx.z / p.row_tiles;
-    const int rt = p.row_tiles - 1 - (blockIdx.z - b * p.row_tiles); // later rows see more keys: they go first
+    const PagedCtaAt at = paged_cta(p);
+    const int kvh = at.kvh, split = at.split, b = at.unit / p.row_tiles;
+    const int rt = p.row_tiles - 1 - (at.unit - b * p.row_tiles); // later rows see more keys: they go first
     int r0, n, base;
     if (!paged_seq(p.pv, p.cu, p.base, p.total, b, r0, n, base)) return;
     if (n > p.max_new && tid == 0) p.pv.raise(FBLT_PAGED_BAD_LENGTH);
@@ -653,8 +654,7 @@ template <int HD, int FMT>
 static int launch_chunk_t(const PagedAttnParams &p, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     if (const int st = allow_smem((const void *)paged_chunk_kernel<HD, FMT>, PcShape<HD>::kSmem, done)) return st;
-    const dim3 grid((unsigned)p.pv.kvh, (unsigned)p.splits, (unsigned)(p.batch * p.row_tiles));
-    paged_chunk_kernel<HD, FMT><<<grid, kPcThreads, PcShape<HD>::kSmem, s>>>(p);
+    paged_chunk_kernel<HD, FMT><<<paged_grid(p), kPcThreads, PcShape<HD>::kSmem, s>>>(p);
     count_launch();
     return check_launch("paged_chunk_kernel");
 }

@@ -79,3 +79,18 @@ def test_stages_whose_values_were_cleared_are_used_again(cuda_lib, fmt, hd, head
         assert c.status_bits() == L.PAGED_BAD_PAGE
     c.page_table.copy_(keep)
     check_attention(c, q, out, news, base, heads, window=window, missing=gone)
+
+
+# ------------------------------------------------------------------------------------------------ large launches
+
+@pytest.mark.parametrize("splits", [0, 2])
+def test_single_tokens_of_many_sequences_beside_a_long_chunk(cuda_lib, splits):
+    """1100 sequences x 64 tiles of rows, more than a grid's second and third dimension hold."""
+    new, heads, kv, hd = [1] * 700 + [2048] + [1] * 399, 8, 1, 32
+    base = [(29 * b) % 90 for b in range(len(new))]
+    lens = [b + n for b, n in zip(base, new)]
+    c = make_cache(220, "int8", lens, kv, hd, 32)
+    fill_cache(c, 221, lens)
+    q, out = attend(c, new, base, heads, 222, splits=splits)
+    assert c.status_bits() == 0
+    check_attention(c, q, out, new, base, heads)
