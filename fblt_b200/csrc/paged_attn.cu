@@ -711,10 +711,12 @@ static int paged_plan_check(const fblt_paged_attn_desc *d, const PagedPlan &pl, 
                         workspace_bytes);
         if ((uintptr_t)workspace & 15) return fail(FBLT_ERR_ARG, "paged_attn: workspace must be 16-byte aligned");
     }
-    // at most 65535 * 2^22 tiles * 64 pieces * 1024 heads
-    if ((int64_t)d->batch * pl.row_tiles * pl.splits * d->cache.num_kv_heads > INT_MAX)
-        return fail(FBLT_ERR_LIMIT, "paged_attn: batch * row tiles (%d) * pieces (%d) * kv heads exceed 2^31 - 1 per launch", pl.row_tiles,
-                    pl.splits);
+    // A tile of every sequence is launched for every tile that max_new allows: beyond this many, nearly all of them empty, a
+    // launch would only take milliseconds to find that out.
+    const int64_t units = (int64_t)d->batch * pl.row_tiles;
+    if (units >= (1 << 22) || units * pl.splits * d->cache.num_kv_heads > INT_MAX)
+        return fail(FBLT_ERR_LIMIT, "paged_attn: batch * row tiles (%d) exceed 2^22 - 1, or with %d pieces and the kv heads 2^31 - 1, per launch",
+                    pl.row_tiles, pl.splits);
     if (pl.splits > 1 && (int64_t)d->total_rows * d->num_heads * (d->cache.head_dim / 4) / 256 >= INT_MAX)
         return fail(FBLT_ERR_LIMIT, "paged_attn: too many rows to merge in one launch");
     return FBLT_OK;
