@@ -86,6 +86,12 @@ __device__ __forceinline__ bool paged_seq(const PagedView &pv, const int32_t *cu
 
 // 2^e as a float, -126 <= e <= 127.
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }
+// The same for any e <= 127, below 2^-149 zero.
+__device__ __forceinline__ float exp2_low(int e) { return e >= -126 ? exp2_int(e) : e < -149 ? 0.0f : __int_as_float(1 << (e + 149)); }
+
+// Scales of V within a stage or tile, 2^(e - et) with et the largest, span 247 powers of two, the mask may take the largest
+// ones out of a row's sum, and p 2^(e - et) has to be a float for every p up to 2^4: they are kept 2^kVUp higher.
+constexpr int kVUp = 123, kVSpan = 247;
 
 template <int FMT>
 struct KvFormat;

@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
                 // the producer's next bulk copy into this stage goes through the async proxy: it comes behind these stores
                 if (WR > 1) fence_async_smem();
             }
-            // ---- scales of the stage's keys; V's relative to the largest, 2^et
+            // ---- scales of the stage's keys; V's in units of 2^et, kVUp below the largest
             int et = kPsNoUnit;
             {
                 constexpr int KL = S::kKeys / 32; // keys of a lane
@@ -277,7 +277,8 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
                 }
                 et = __reduce_max_sync(0xffffffffu, et);
 #pragma unroll
-                for (int i = 0; i < KL; ++i) vscale[lane * KL + i] = exp2_int(min(max(e[i] - et, -126), 0));
+                for (int i = 0; i < KL; ++i) vscale[lane * KL + i] = exp2_int(min(max(e[i] - et, -kVSpan), 0) + kVUp);
+                et -= kVUp;
             }
             __syncwarp();
 #pragma unroll 1
@@ -409,13 +410,15 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
                 }
                 bool raise = false;
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) raise |= top[rb] > 0.0f && (__float_as_int(top[rb]) >> 23) - 127 + et > R[rb] + 4;
+                for (int rb = 0; rb < RB; ++rb) // (or where R lies below its least, see there)
+                    raise |= top[rb] > 0.0f && max(__float_as_int(top[rb]) >> 23, kPsHead + 4) > R[rb] + 4 + 127 - et;
                 if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb) {
                         float w = fmaxf(top[rb], __shfl_xor_sync(0xffffffffu, top[rb], 1));
                         w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 2));
-                        const int Rn = w > 0.0f ? max(R[rb], (__float_as_int(w) >> 23) - 127 + et) : R[rb];
+                        // (R not so low that 2^(et - R + kPsHead) below is no float: 2^-3 and 2^10 are held alike in two halves)
+                        const int Rn = w > 0.0f ? max(R[rb], et + max((__float_as_int(w) >> 23) - 127, kPsHead - 127)) : R[rb];
                         const float f = R[rb] - Rn < -126 ? 0.0f : exp2_int(R[rb] - Rn);
                         R[rb] = Rn;
 #pragma unroll
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
                     // p 2^(ev - et) in units of 2^(R - kPsHead); a row without a weight has only zeros
-                    const float f = exp2_int(min(max(et - R[rb] + kPsHead, -126), 126));
+                    const float f = exp2_low(min(et - R[rb] + kPsHead, 127));
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
                         split_half2(x[rb][u][0].x * f, x[rb][u][0].y * f, pa[rb][u].x, pa[rb][u].y);

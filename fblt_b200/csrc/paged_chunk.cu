@@ -366,6 +366,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 }
                 const float mref = m == -INFINITY ? 0.0f : -m;
                 int top = et + (int)floorf(fminf(fmaxf(mx + mref, -4096.0f), 64.0f)); // the tile's largest p 2^et
+                int far = top; // what has to lie above R + 4 for R to follow
                 if (wide) {
                     float w = 0.0f;
 #pragma unroll
@@ -375,9 +376,11 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                             w = fmaxf(w, t5_ex2(fmaf(y[c][k].x, down, mref)) * vscale[st][c * 32 + 2 * k]);
                             w = fmaxf(w, t5_ex2(fmaf(y[c][k].y, down, mref)) * vscale[st][c * 32 + 2 * k + 1]);
                         }
-                    top = w > 0.0f ? et + (__float_as_int(w) >> 23) - 127 : R;
+                    // (R not so low that 2^lift below is no float: 2^-3 and 2^10 are held alike in two halves)
+                    top = w > 0.0f ? et + max((__float_as_int(w) >> 23) - 127, kPcHead - 127) : R;
+                    far = w > 0.0f ? max(top, et + kPcHead + 4 - 127) : R;
                 }
-                const bool raise = mx > -INFINITY && top > R + 4;
+                const bool raise = mx > -INFINITY && far > R + 4;
                 if (raise) {
                     f *= R - top < -126 ? 0.0f : exp2_int(R - top);
                     R = top;
@@ -396,7 +399,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                     }
                 }
                 // ---- weights in units of 2^(R - head), their sum, and their two planes over the scores
-                const int lift = min(max(et - R + kPcHead, -4096), 126); // p 2^et 2^-(R - head) = 2^(s - m + lift)
+                const int lift = max(et - R + kPcHead, -4096); // p 2^et 2^-(R - head) = 2^(s - m + lift)
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                 if (!__any_sync(0xffffffffu, wide || lift < -64)) {
                     const float ref = mref + (float)lift;
@@ -413,9 +416,9 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         tmem_st16(trow + c * 32, ph);
                         tmem_st16(trow + c * 32 + 16, pl);
                     }
-                    l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) * exp2_int(-lift);
+                    l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) * exp2_int(-min(lift, 126)); // (past 126 it is less than 2^-112 either way)
                 } else { // the sum is taken before V's scales
-                    const float fw = lift < -126 ? 0.0f : exp2_int(lift);
+                    const float fw = exp2_low(min(lift, 127)), fx = exp2_int(min(max(lift - 127, 0), 127)); // (past 127 in a narrow tile alone)
 #pragma unroll
                     for (int c = 0; c < CH; ++c) {
                         uint32_t ph[16], pl[16];
@@ -423,7 +426,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         for (int k = 0; k < 16; ++k) {
                             const float2 w = make_float2(t5_ex2(fmaf(y[c][k].x, down, mref)), t5_ex2(fmaf(y[c][k].y, down, mref)));
                             sum[k & 1] = __fadd2_rn(sum[k & 1], w);
-                            const float a = wide ? vscale[st][c * 32 + 2 * k] : 1.0f, e = wide ? vscale[st][c * 32 + 2 * k + 1] : 1.0f;
+                            const float a = wide ? vscale[st][c * 32 + 2 * k] : fx, e = wide ? vscale[st][c * 32 + 2 * k + 1] : fx;
                             split_half2(w.x * a * fw, w.y * e * fw, ph[k], pl[k]);
                         }
                         tmem_st16(trow + c * 32, ph);
@@ -518,6 +521,13 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 ev = min(max((int)p.pv.ve[row], F::kEmin), F::kEmax);
             }
         };
+        // whether this thread's part of a row holds anything but zeros
+        auto any_value = [&](const uint4(&raw)[NP]) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) w |= raw[i].x | raw[i].y | raw[i].z | raw[i].w;
+            return (FMT == FBLT_KV_E4M3 ? w & 0x7f7f7f7fu : w) != 0;
+        };
         load(look(0));
         int64_t next = look(1);
         for (int j = 0; j < nst; ++j) {
@@ -526,8 +536,12 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             if (lost && lane == 0) give_up(0x53);
             // ---- the tile's range of exponents (keys that are there)
             {
-                // (a row with the least exponent, as a row of zeros has, does not make a tile wide)
-                const bool sk = here && ek > F::kEmin, sv = here && ev > F::kEmin;
+                // (a row of zeros has the least exponent: it does not make a tile wide)
+                bool sk = here && ek > F::kEmin, sv = here && ev > F::kEmin;
+                if (__any_sync(0xffffffffu, here && !(sk && sv))) {
+                    sk = here && (sk || any_value(kr));
+                    sv = here && (sv || any_value(vr));
+                }
                 const int4 r = make_int4(__reduce_max_sync(0xffffffffu, here ? ek : -1000), __reduce_min_sync(0xffffffffu, sk ? ek : 1000),
                                          __reduce_max_sync(0xffffffffu, here ? ev : -1000), __reduce_min_sync(0xffffffffu, sv ? ev : 1000));
                 if (lane == 0) range[st][warp - 8] = r;
@@ -539,17 +553,13 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 const int4 r = range[st][i];
                 e = make_int4(max(e.x, r.x), min(e.y, r.y), max(e.z, r.z), min(e.w, r.w));
             }
-            // Beside rows 2^60 larger, a row with the least exponent is one of zeros; nearer to it the tile counts as wide.
-            auto is_wide = [&](int most, int least) {
-                return most > F::kEmin && (most < F::kEmin + 60 ? most - F::kEmin > kPcNarrow : most - least > kPcNarrow);
-            };
-            const bool none = e.x < F::kEmin, kwide = is_wide(e.x, e.y), vwide = is_wide(e.z, e.w);
+            const bool none = e.x < F::kEmin, kwide = e.x - e.y > kPcNarrow, vwide = e.z - e.w > kPcNarrow;
             const int kbelow = here ? e.x - ek : 0, vbelow = here ? e.z - ev : 0; // 2^-below: into the halves or the columns
-            if (ct == 0) *reinterpret_cast<int4 *>(top_of[st]) = make_int4(none ? 0 : e.x, none ? 0 : e.z, kwide, vwide);
+            if (ct == 0) *reinterpret_cast<int4 *>(top_of[st]) = make_int4(none ? 0 : e.x, none ? 0 : e.z - (vwide ? kVUp : 0), kwide, vwide);
             const uint32_t vote = __ballot_sync(0xffffffffu, here);
             if (piece0 == 0) {
                 kscale[st][key] = kbelow > 126 ? 0.0f : exp2_int(-kbelow);
-                vscale[st][key] = vbelow > 126 ? 0.0f : exp2_int(-vbelow);
+                vscale[st][key] = exp2_int(kVUp - vbelow);
                 if ((lane & 15) == 0) present[st][key / 16] = ((vote >> lane) & 0xffff) != 0;
             }
             auto put = [&](uint8_t *dst, const uint4(&raw)[NP], __half2 s) {

@@ -94,3 +94,64 @@ def test_single_tokens_of_many_sequences_beside_a_long_chunk(cuda_lib, splits):
     q, out = attend(c, new, base, heads, 222, splits=splits)
     assert c.status_bits() == 0
     check_attention(c, q, out, new, base, heads)
+
+
+# ------------------------------------------------------------------------------------------------ scales at both ends of fp32
+
+def append_all(c, k, v):
+    ops.paged_append(ops.make_paged_append(c, cu([k.shape[0]]), i32([0]), k, v))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("n", [1, 5, 20, 150, 300])
+@pytest.mark.parametrize("low,high", [(-100, 100), (-107, 120), (-117, 122)])
+def test_values_at_both_ends_of_the_range(cuda_lib, fmt, hd, n, low, high):
+    """Rows that see only very small values, beside very large ones that the mask or the softmax takes out: first the large
+    rows lie behind the small ones (a causal mask), then before them (a window), then among them with weights of 0."""
+    if fmt == "e4m3":
+        low = max(low, -107)  # 448 * 2^-117 is the largest value of the least exponent
+    heads, base = 2, 90
+    L_ = base + n
+    g = gen(230)
+    for where in ("behind", "before", "among"):
+        c = make_cache(231, fmt, [L_], 1, hd, 16)
+        k, v, q = randn(g, L_, hd), randn(g, L_, hd).clamp(-2, 2), randn(g, n, heads * hd)
+        big = torch.zeros(L_, dtype=torch.bool, device="cuda")
+        window = 0
+        if where == "behind":
+            big[base + n // 2 + 1:] = True  # the first half of the new rows sees small values alone
+        elif where == "before":
+            big[:60], window = True, 31     # (row base sees 60 ..)
+        else:
+            big[7::16] = True
+            u = torch.ones(hd, device="cuda")
+            k[big] = -40 * u
+            q = (0.9 + 0.2 * torch.rand(q.shape, generator=g, device="cuda"))  # scores of about -40 sqrt(hd): e^-226 or less
+        v *= torch.where(big, 2.0 ** high, 2.0 ** low)[:, None]
+        append_all(c, k, v)
+        for splits in (1, 2):
+            q, out = attend(c, [n], [base], heads, 0, q=q, window=window, splits=splits)
+            assert c.status_bits() == 0
+            check_attention(c, q, out, [n], [base], heads, window=window)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [1, 20, 200])
+@pytest.mark.parametrize("every", [16, 128])
+def test_small_weights_that_make_up_for_the_size_of_values(cuda_lib, fmt, hd, n, every):
+    """Keys of weight 2^-118 or so whose values are 2^120 times the others': both count, whichever tile they lie in."""
+    heads, base = 2, 256
+    L_ = base + n
+    c = make_cache(240, fmt, [L_], 1, hd, 16)
+    g = gen(241)
+    big = torch.arange(L_, device="cuda") // every % 2 == 1
+    k = 0.05 * randn(g, L_, hd)
+    k -= torch.where(big, 82.0 / math.sqrt(hd), 0.0)[:, None]
+    v = randn(g, L_, hd) * torch.where(big, 2.0 ** 111, 2.0 ** -9)[:, None]
+    append_all(c, k, v)
+    q = 1 + 0.01 * randn(g, n, heads * hd)
+    for splits in (1, 2):
+        q, out = attend(c, [n], [base], heads, 0, q=q, splits=splits)
+        check_attention(c, q, out, [n], [base], heads)
