@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
         for (int rb = warp; rb < RB * WR; rb += 4) {
             const int r = rb * 8 + g;
             float4 x[KS];
-            float a = 0.0f;
+            float a = 0.0f, odd = 0.0f; // odd: NaN once a value is not finite
             const bool live = r < rows;
             const int i = live ? r / p.G : 0;
             const float *src = p.q + (int64_t)(r0 + i) * p.qs + (int64_t)(kvh * p.G + (r - i * p.G)) * HD;
@@ -187,10 +187,15 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
                 x[s] = live ? *reinterpret_cast<const float4 *>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
                 const float v[4] = {x[s].x, x[s].y, x[s].z, x[s].w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) a = finite_f(v[e]) ? fmaxf(a, fabsf(v[e])) : a;
+                for (int e = 0; e < 4; ++e) {
+                    a = finite_f(v[e]) ? fmaxf(a, fabsf(v[e])) : a;
+                    odd = fmaf(v[e], 0.0f, odd);
+                }
             }
             a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
             a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+            odd += __shfl_xor_sync(0xffffffffu, odd, 1);
+            odd += __shfl_xor_sync(0xffffffffu, odd, 2);
             // q * 2^e with its largest value in [2^13, 2^14): halves keep the row's small values too
             const int e = min(13 - ((__float_as_int(a) >> 23) - 127), 126);
             const float up = exp2_int(e);
@@ -201,7 +206,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
                 split_half2(x[s].z * up, x[s].w * up, f.z, f.w);
                 sq[(rb * KS + s) * 32 + lane] = f;
             }
-            if (t == 0) crow[rb * 8 + g] = p.qscale * exp2_int(-e);
+            if (t == 0) crow[rb * 8 + g] = p.qscale * exp2_int(-e) + odd; // (NaN for a row that is not finite)
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");
 
@@ -340,7 +345,8 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
                         for (int nb = 0; nb < 2; ++nb) {
                             const float(&v)[4] = s[rb][u][nb];
                             float2 y = __fadd2_rn(make_float2(v[0], v[1]), make_float2(v[2], v[3]));
-                            y = __fmul2_rn(__fmul2_rn(y, nb ? make_float2(ks.z, ks.w) : make_float2(ks.x, ks.y)), make_float2(c[rb], c[rb]));
+                            // both powers of two first: one of them may be what keeps the other's product in fp32's range
+                            y = __fmul2_rn(y, __fmul2_rn(nb ? make_float2(ks.z, ks.w) : make_float2(ks.x, ks.y), make_float2(c[rb], c[rb])));
                             x[rb][u][nb] = y;
                             odd = fmaf(y.x, 0.0f, fmaf(y.y, 0.0f, odd));
                             mn[rb] = fmaxf(mn[rb], fmaxf(y.x, y.y));
@@ -356,6 +362,9 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
                             for (int nb = 0; nb < 2; ++nb) {
                                 float2 &y = x[rb][u][nb];
                                 const int k = kb + kl + 4 * u + 2 * nb - lo[rb];
+                                // a product of 0 times a scale past fp32's range
+                                if (isnan(y.x) && !isnan(c[rb])) y.x = 0.0f;
+                                if (isnan(y.y) && !isnan(c[rb])) y.y = 0.0f;
                                 y.x = there && (unsigned)k < (unsigned)span[rb] && finite_f(y.x) ? y.x : -INFINITY;
                                 y.y = there && (unsigned)(k + 1) < (unsigned)span[rb] && finite_f(y.y) ? y.y : -INFINITY;
                                 mn[rb] = fmaxf(mn[rb], fmaxf(y.x, y.y));

@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
     constexpr int BN = S::BN, CH = BN / 32, PR = HD + 4, kFold = kPcFold / BN;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ PcBars bars;
-    __shared__ __align__(16) float kscale[2][BN], vscale[2][BN];
+    __shared__ __align__(16) float vscale[2][BN];
+    __shared__ int kunder[2][BN]; // a key's exponent below the tile's largest
     __shared__ __align__(16) int top_of[2][4]; // largest exponent of the tile's K, of its V; whether each is too wide for its halves
     __shared__ int4 range[2][4];
     __shared__ __align__(8) uint8_t present[2][8]; // groups of 16 keys whose page exists and that the CTA reads
@@ -329,11 +330,15 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         peak[(k & 2) + 1] = max3(peak[(k & 2) + 1], y[c][k + 1].x, y[c][k + 1].y);
                     }
                 const int4 tops = *reinterpret_cast<const int4 *>(top_of[st]);
-                const float down = exp2_int(min(max(tops.x + F::kShift - qe, -126), 126));
+                const int sc = tops.x - qe; // a score is y 2^sc
+                float down = exp2_int(min(max(sc, -126), 126));
                 float mx = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3])) * down;
                 // Sums of 8-bit codes times query planes below 2^14 stay far from overflow, so a score is not finite only
                 // where the query row is not, or where the scales took it past fp32's range (-inf weighs 0 by itself).
-                if (__any_sync(0xffffffffu, masked || tops.z || qbad || !(mx < INFINITY))) {
+                if (__any_sync(0xffffffffu, masked || tops.z || qbad || sc > 126 || !(mx < INFINITY))) {
+                    // where one float does not hold the scales, they are taken key by key in two
+                    const bool apart = __any_sync(0xffffffffu, tops.z || sc > 126);
+                    if (apart) down = 1.0f;
                     mx = -INFINITY;
 #pragma unroll
                     for (int c = 0; c < CH; ++c)
@@ -341,9 +346,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         for (int k = 0; k < 16; ++k) {
                             const int d = kb + c * 32 + 2 * k - lo;
                             const bool there = present[st][c * 2 + k / 8] != 0;
-                            if (tops.z) {
-                                y[c][k].x *= kscale[st][c * 32 + 2 * k];
-                                y[c][k].y *= kscale[st][c * 32 + 2 * k + 1];
+                            if (apart) {
+                                const int ex = sc - (tops.z ? kunder[st][c * 32 + 2 * k] : 0), ey = sc - (tops.z ? kunder[st][c * 32 + 2 * k + 1] : 0);
+                                y[c][k].x = y[c][k].x * exp2_int(min(max(ex, -126), 126)) * exp2_int(min(max(ex, 126) - 126, 127));
+                                y[c][k].y = y[c][k].y * exp2_int(min(max(ey, -126), 126)) * exp2_int(min(max(ey, 126) - 126, 127));
                             }
                             y[c][k].x = there && (unsigned)d < (unsigned)span && finite_f(y[c][k].x * down) ? y[c][k].x : -INFINITY;
                             y[c][k].y = there && (unsigned)(d + 1) < (unsigned)span && finite_f(y[c][k].y * down) ? y[c][k].y : -INFINITY;
@@ -558,7 +564,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             if (ct == 0) *reinterpret_cast<int4 *>(top_of[st]) = make_int4(none ? 0 : e.x, none ? 0 : e.z - (vwide ? kVUp : 0), kwide, vwide);
             const uint32_t vote = __ballot_sync(0xffffffffu, here);
             if (piece0 == 0) {
-                kscale[st][key] = kbelow > 126 ? 0.0f : exp2_int(-kbelow);
+                kunder[st][key] = kbelow;
                 vscale[st][key] = exp2_int(kVUp - vbelow);
                 if ((lane & 15) == 0) present[st][key / 16] = ((vote >> lane) & 0xffff) != 0;
             }

@@ -155,3 +155,44 @@ def test_small_weights_that_make_up_for_the_size_of_values(cuda_lib, fmt, hd, n,
     for splits in (1, 2):
         q, out = attend(c, [n], [base], heads, 0, q=q, splits=splits)
         check_attention(c, q, out, [n], [base], heads)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("n", [1, 6, 15, 150])
+def test_keys_at_both_ends_of_the_range(cuda_lib, fmt, hd, n):
+    """Scores of ordinary size from very small queries and very large keys, and from very large queries over very small
+    keys beside keys whose scores pass fp32 (those weigh 0)."""
+    heads, base = 2, 130
+    L_ = base + n
+    g = gen(250)
+    small, large = 2.0 ** -107, 2.0 ** 118
+    for keys, queries, over in (("large", 2.0 ** -118, ()), ("small", 2.0 ** 107, ()), ("small", 2.0 ** 107, (3, 16, 17, 60, 128))):
+        c = make_cache(251, fmt, [L_], 1, hd, 16)
+        k, v, q = randn(g, L_, hd).clamp(-4, 4), randn(g, L_, hd), randn(g, n, heads * hd).clamp(-4, 4)
+        k *= large if keys == "large" else small
+        for j in over:
+            k[j] = k[j] * 2.0 ** 100 * 2.0 ** 100  # (2^200 is no float)
+        append_all(c, k, v)
+        q *= queries
+        for splits in (1, 2):
+            q, out = attend(c, [n], [base], heads, 0, q=q, splits=splits)
+            assert c.status_bits() == 0
+            check_attention(c, q, out, [n], [base], heads, missing=[(0, j, j + 1) for j in over])
+
+
+@pytest.mark.parametrize("hd", [32, 128])
+@pytest.mark.parametrize("n", [1, 6, 15, 150])
+def test_scores_that_are_zero_between_scores_that_pass_fp32(cuda_lib, hd, n):
+    """One-hot queries and keys of 2^100: a score is 0 or not finite, and the zeros share the weight."""
+    heads, base = 2, 100
+    L_ = base + n
+    c = make_cache(252, "int8", [L_], 1, hd, 16)
+    k, q = torch.zeros(L_, hd, device="cuda"), torch.zeros(n, heads * hd, device="cuda")
+    hit = torch.arange(L_, device="cuda") % 3 == 1
+    k[hit, 2], k[~hit, 5] = 2.0 ** 100, 2.0 ** 100
+    q[:, 2::hd] = 2.0 ** 100
+    v = randn(gen(253), L_, hd)
+    append_all(c, k, v)
+    q, out = attend(c, [n], [base], heads, 0, q=q)
+    check_attention(c, q, out, [n], [base], heads, missing=[(0, j, j + 1) for j in hit.nonzero().flatten().tolist()])
