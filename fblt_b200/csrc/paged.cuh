@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "tc5.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -171,6 +172,11 @@ __device__ __forceinline__ void split_half2(float x, float y, uint32_t &hi, uint
     const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// A bounded wait of a whole warp, with one answer: lanes that gave up alone would leave the others' shuffles without partners.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, const volatile int *abort_word) {
+    return __all_sync(0xffffffffu, mbar_wait_abort(bar, parity, abort_word));
 }
 
 // What the attention kernels get. The rows of one kv head are numbered r = i * G + g: head kvh * G + g of token i.

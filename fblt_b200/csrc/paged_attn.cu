@@ -28,7 +28,6 @@
 // 531 us; a warp's 8 rows in steps of 16 keys instead of 32 456 us; four CTAs an SM at head_dim 128 519 us; a maximum that
 // moves with every larger score (not by 2^4 at least) 8 us more.
 #include "paged.cuh"
-#include "tc5.cuh"
 
 namespace fblt {
 
@@ -528,7 +527,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
         } else {
             for (int st = wk; st < nst; st += WK) { // a stage belongs to the WR warps of one key share
                 const int slot = st % NS;
-                if (!mbar_wait_abort(&full[slot], (st / NS) & 1, (const volatile int *)&s_abort)) {
+                if (!warp_wait(&full[slot], (st / NS) & 1, (const volatile int *)&s_abort)) {
                     *(volatile int *)&s_abort = 1;
                     if (lane == 0) atomicCAS(&g_paged_error, 0u, (0x42u << 24) | (blockIdx.x & 0xffffffu));
                     break;

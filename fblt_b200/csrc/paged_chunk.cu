@@ -27,7 +27,6 @@
 // case). Measured and slower: three bf16 planes of P 757 us; S beside P instead of under it, tiles of 96 keys 715 us;
 // two threads a row 704 us; the query tiles in turns 695 us; a share of the exponentials as polynomials 649-698 us.
 #include "paged.cuh"
-#include "tc5.cuh"
 
 namespace fblt {
 
@@ -269,15 +268,18 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
             };
             float m = -INFINITY, l = 0.0f;
             int R = 0;
-            bool ok = mbar_wait_abort(&bars.kv_full[0], 0, abortp);
-            if (!ok && lane == 0) give_up(0x55);
-            for (int j = 0; j < nst && ok; ++j) { // the tile's scales are there: waited for at the end of the step before
+            // A lane whose wait has run out goes on with the others, without waiting, and nothing is written in the end: leaving
+            // alone it would take the partner of their shuffles away (and a vote on every wait costs 5 %).
+            unsigned lost = 0; // which wait
+            auto wait = [&](uint64_t *bar, uint32_t parity, unsigned code) {
+                if (lost || mbar_wait_abort(bar, parity, abortp)) return;
+                *(volatile int *)&s_abort = 1;
+                lost = code;
+            };
+            wait(&bars.kv_full[0], 0, 0x55);
+            for (int j = 0; j < nst; ++j) { // the tile's scales are there: waited for at the end of the step before
                 const int st = j & 1, kb = kb0 + j * BN;
-                if (!mbar_wait_abort(&bars.s_full[T], j & 1, abortp)) {
-                    if (lane == 0) give_up(0x51);
-                    ok = false;
-                    break;
-                }
+                wait(&bars.s_full[T], j & 1, 0x51);
                 tc_fence_after();
                 if (j > 0 && j % kFold == 0) { // O is complete: S came behind it
                     constexpr int W = HD == 128 ? 16 : 8; // fours of columns whose sums are read together
@@ -443,16 +445,11 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 tc_wait_st();
                 tc_fence_before();
                 mbar_arrive(&bars.p_ready[T]);
-                if (j + 1 < nst && !mbar_wait_abort(&bars.kv_full[st ^ 1], ((j + 1) >> 1) & 1, abortp)) {
-                    if (lane == 0) give_up(0x55);
-                    ok = false;
-                }
+                if (j + 1 < nst) wait(&bars.kv_full[st ^ 1], ((j + 1) >> 1) & 1, 0x55);
             }
-            if (ok && !mbar_wait_abort(&bars.o_full, 0, abortp)) {
-                if (lane == 0) give_up(0x52);
-                ok = false;
-            }
-            if (__all_sync(0xffffffffu, ok)) {
+            wait(&bars.o_full, 0, 0x52);
+            if (lost) give_up(lost);
+            if (__all_sync(0xffffffffu, lost == 0)) {
                 tc_fence_after();
                 // 2^(R - head) in two steps: it may lie below what one float holds
                 const float inv = (l > 0.0f ? 1.0f / l : 0.0f) * (1.0f / (1 << kPcHead)), unit = R < -126 ? 0.0f : exp2_int(min(R, 127));
@@ -617,9 +614,9 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 }
                 __syncwarp();
             };
-            bool ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.q_full, 0, abortp));
+            bool ok = warp_wait(&bars.q_full, 0, abortp);
             if (ok) {
-                ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.kv_full[0], 0, abortp));
+                ok = warp_wait(&bars.kv_full[0], 0, abortp);
                 if (ok) {
                     tc_fence_after();
                     for (int T = 0; T < tiles; ++T) issue_s(T, 0);
@@ -627,7 +624,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                 for (int j = 0; j < nst && ok; ++j) {
                     const int st = j & 1;
                     for (int T = 0; T < tiles; ++T) {
-                        ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.p_ready[T], j & 1, abortp));
+                        ok = warp_wait(&bars.p_ready[T], j & 1, abortp);
                         if (!ok) break;
                         tc_fence_after();
                         // O += P V: 16 keys are two 8-row core matrices of V, 128 bytes apart; 8 columns of O the next BN rows on
@@ -645,7 +642,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedA
                         __syncwarp();
                         if (j + 1 < nst) {
                             if (T == 0) {
-                                ok = __all_sync(0xffffffffu, mbar_wait_abort(&bars.kv_full[st ^ 1], ((j + 1) >> 1) & 1, abortp));
+                                ok = warp_wait(&bars.kv_full[st ^ 1], ((j + 1) >> 1) & 1, abortp);
                                 if (!ok) break;
                                 tc_fence_after();
                             }
