@@ -6,10 +6,10 @@ import numpy as np
 import pytest
 import torch
 
-import paged_ref as R
+import paged_precision as A
 from fblt_b200 import lib as L
 from fblt_b200 import ops
-from test_gpu_paged import attend, check_attention, cu, fill_cache, gen, i32, make_cache, randn
+from test_gpu_paged import attend, check_attention, cu, fill_cache, gen, i32, make_cache, randn, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -196,3 +196,61 @@ def test_scores_that_are_zero_between_scores_that_pass_fp32(cuda_lib, hd, n):
     append_all(c, k, v)
     q, out = attend(c, [n], [base], heads, 0, q=q)
     check_attention(c, q, out, [n], [base], heads, missing=[(0, j, j + 1) for j in hit.nonzero().flatten().tolist()])
+
+
+# ------------------------------------------------------------------------------------------------ precision over long ranges
+
+LONG = [(32, 1, 1), (64, 1, 1), (128, 1, 1), (64, 4, 3), (32, 4, 7), (64, 4, 8), (128, 4, 3), (128, 4, 8), (32, 4, 40), (64, 4, 40), (128, 4, 40)]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd,heads,n", LONG)
+@pytest.mark.parametrize("sink", [False, True])
+def test_average_error_over_long_ranges(cuda_lib, fmt, hd, heads, n, sink):
+    """Both planes of Q and P are there, and the sums are folded: averages that a lost one would raise by far
+    (test_paged_precision). `sink`: the first keys are small and their values smaller, as a model's first tokens are, so that
+    exponents of a tile lie far apart."""
+    L_, kv = 8000 + n, 1
+    chunk = n * heads // kv > 32
+    c = make_cache(260, fmt, [L_], kv, hd, 64)
+    g = gen(261)
+    k, v, q = randn(g, L_, hd), randn(g, L_, hd), randn(g, n, heads * hd)
+    if sink:
+        k[:4] *= 2.0 ** -6
+        v[:4] *= 2.0 ** -9
+    for sign in (False, True):
+        append_all(c, k, v.abs() if sign else v)
+        _, out = attend(c, [n], [L_ - n], heads, 0, q=q, splits=1)
+        kk, vv = stored(c, 0, L_, "k").cuda(), stored(c, 0, L_, "v").cuda()
+        want, size = A.exact(q.view(n, heads, hd), kk, vv, L_ - n, np.float32(1 / math.sqrt(hd)).item())
+        got = out.view(n, heads, hd)
+        if sign:
+            pull, bound = A.pull(got, want), A.pull_bound(chunk, hd, L_)
+            assert abs(pull) <= bound, f"mean signed error {pull:.3g}, bound {bound:.3g}"
+        else:
+            r, bound = A.ratio(got, want), A.rms_bound(chunk, hd, L_, size)
+            assert r <= bound, f"rms error {r:.3g} of the rms output, bound {bound:.3g}"
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_cuts_into_chunks_agree_on_average(cuda_lib, fmt, hd):
+    """A prompt at once, in chunks and token by token: outputs that differ by what their errors allow, no more."""
+    heads, kv, T = 4, 2, 311
+    g = gen(262)
+    q, k, v = randn(g, T, heads * hd), randn(g, T, kv * hd), randn(g, T, kv * hd)
+    outs = []
+    for cuts in ([T], [100, 1, 77, 133], [1] * 20 + [291], [17] * 18 + [5]):
+        c, at, parts = make_cache(263, fmt, [T], kv, hd, 16), 0, []
+        for m in cuts:
+            ops.paged_append(ops.make_paged_append(c, cu([m]), i32([at]), k[at:at + m], v[at:at + m]))
+            parts.append(attend(c, [m], [at], heads, 0, q=q[at:at + m])[1])
+            at += m
+        outs.append(torch.cat(parts))
+    kk, vv = stored(c, 0, T, "k").cuda(), stored(c, 0, T, "v").cuda()
+    want, size = A.exact(q.view(T, heads, hd), kk, vv, 0, np.float32(1 / math.sqrt(hd)).item())
+    bound = A.rms_bound(True, hd, T, size)
+    for o in outs:
+        assert A.ratio(o.view(T, heads, hd), want) <= bound
+    for o in outs[1:]:
+        assert A.ratio(o, outs[0].double()) <= 2 * bound
