@@ -571,6 +571,11 @@ def _rows(t: torch.Tensor, cols: int, what: str, dtypes=(torch.float32,)) -> tor
     return t
 
 
+def _row_stride(t: torch.Tensor) -> int:
+    """Row stride of a view that _rows has passed; a single row's is any number at all (a transposed column's is 1)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def _table(t: torch.Tensor, n: int, what: str) -> torch.Tensor:
     if not (t.is_cuda and t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] >= n and (t.stride(0) == 1 or n <= 1)):
         raise ValueError(f"{what}: a contiguous CUDA int32 tensor of {n} entries is needed")
@@ -665,9 +670,9 @@ def make_qk_norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], pos:
             if t.shape[0] != rows:
                 raise ValueError("q, k and their outputs have one row count")
         setattr(d, name, x.data_ptr())
-        setattr(d, name + "_stride", x.stride(0))
+        setattr(d, name + "_stride", _row_stride(x))
         setattr(d, name + "_out", out.data_ptr())
-        setattr(d, name + "_out_stride", out.stride(0))
+        setattr(d, name + "_out_stride", _row_stride(out))
     d.q_gain, d.k_gain = _vector(q_gain, head_dim, "q_gain"), _vector(k_gain, head_dim, "k_gain")
     _rope(d, rope_cos, rope_sin, head_dim)
     if pos is not None:
@@ -691,12 +696,12 @@ def make_paged_append(cache: PagedKvCache, cu_new: torch.Tensor, base_len: torch
     hd, kc, rows = cache.head_dim, cache.num_kv_heads * cache.head_dim, int(k.shape[0])
     d.cache, d.batch, d.num_heads, d.total_rows, d.eps = cache.desc, cache.batch, num_heads, rows, float(eps)
     d.cu_new, d.base_len = _table(cu_new, cache.batch + 1, "cu_new").data_ptr(), _table(base_len, cache.batch, "base_len").data_ptr()
-    d.k, d.k_stride = _rows(k, kc, "k").data_ptr(), k.stride(0)
-    d.v, d.v_stride = _rows(v, kc, "v").data_ptr(), v.stride(0)
+    d.k, d.k_stride = _rows(k, kc, "k").data_ptr(), _row_stride(k)
+    d.v, d.v_stride = _rows(v, kc, "v").data_ptr(), _row_stride(v)
     out = q if q_out is None else q_out
     if q is not None:
-        d.q, d.q_stride = _rows(q, num_heads * hd, "q").data_ptr(), q.stride(0)
-        d.q_out, d.q_out_stride = _rows(out, num_heads * hd, "q_out").data_ptr(), out.stride(0)
+        d.q, d.q_stride = _rows(q, num_heads * hd, "q").data_ptr(), _row_stride(q)
+        d.q_out, d.q_out_stride = _rows(out, num_heads * hd, "q_out").data_ptr(), _row_stride(out)
     if any(t is not None and t.shape[0] != rows for t in (v, q, out)):
         raise ValueError("q, q_out, k and v have one row count")
     d.q_gain, d.k_gain = _vector(q_gain, hd, "q_gain"), _vector(k_gain, hd, "k_gain")
@@ -722,7 +727,7 @@ def make_paged_read(cache: PagedKvCache, cu_rows: torch.Tensor, k_out: Optional[
     for name, t in (("k_out", k_out), ("v_out", v_out)):
         if t is not None:
             setattr(d, name, _rows(t, cache.num_kv_heads * cache.head_dim, name, (torch.float32, torch.bfloat16)).data_ptr())
-            setattr(d, name + "_stride", t.stride(0))
+            setattr(d, name + "_stride", _row_stride(t))
     return _keep(d, cache, cu_rows, k_out, v_out, start)
 
 
@@ -740,8 +745,8 @@ def make_paged_attn(cache: PagedKvCache, cu_new: torch.Tensor, base_len: torch.T
     d.cache, d.batch, d.num_heads, d.total_rows = cache.desc, cache.batch, num_heads, int(q.shape[0])
     d.max_new, d.max_len, d.block_mode, d.window, d.splits = max_new, max_len, int(block_mode), int(window), splits
     d.cu_new, d.base_len = _table(cu_new, cache.batch + 1, "cu_new").data_ptr(), _table(base_len, cache.batch, "base_len").data_ptr()
-    d.q, d.q_stride = _rows(q, cols, "q").data_ptr(), q.stride(0)
-    d.out, d.out_stride = _rows(out, cols, "out").data_ptr(), out.stride(0)
+    d.q, d.q_stride = _rows(q, cols, "q").data_ptr(), _row_stride(q)
+    d.out, d.out_stride = _rows(out, cols, "out").data_ptr(), _row_stride(out)
     if q.shape[0] != out.shape[0]:
         raise ValueError("q and out have one row count")
     d.scale = float(scale)

@@ -60,3 +60,20 @@ def test_workspaces_elsewhere_are_refused():
                torch.empty(1 << 21, device="cuda", **byte)[::2]):
         with pytest.raises(ValueError, match="workspace"):
             ops.paged_attn(d, ws)
+
+
+def test_a_single_row_of_any_stride():
+    """What a transposed column, or a slice of one row, gives for a row stride is not looked at."""
+    cache = ops.PagedKvCache(**pool(), fmt="int8")
+    i32 = lambda n: torch.empty(n, dtype=torch.int32, device="cuda")  # noqa: E731
+    col = lambda n, **kw: torch.empty(n, 1, device="cuda", **kw).t()  # noqa: E731
+    a = ops.make_paged_attn(cache, i32(4), i32(3), col(256), torch.empty(4, 259, device="cuda")[:1, :256], 4, 1, 64, 0.125)
+    assert (a.q_stride, a.out_stride) == (256, 256)
+    w = ops.make_paged_append(cache, i32(4), i32(3), col(128), col(128), q=col(256), num_heads=4)
+    assert (w.k_stride, w.v_stride, w.q_stride, w.q_out_stride) == (128, 128, 256, 256)
+    r = ops.make_paged_read(cache, i32(4), col(128, dtype=torch.bfloat16), None)
+    assert r.k_out_stride == 128
+    n = ops.make_qk_norm_rope(col(256), col(128), i32(1), 4, 2, 64)
+    assert (n.q_stride, n.q_out_stride, n.k_stride, n.k_out_stride) == (256, 256, 128, 128)
+    two = torch.empty(2, 300, device="cuda")[:, :256]
+    assert ops.make_qk_norm_rope(two, None, i32(2), 4, 0, 64).q_stride == 300
