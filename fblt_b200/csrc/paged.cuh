@@ -13,6 +13,8 @@
 
 namespace fblt {
 
+constexpr int kPlanSms = 148; // SMs of a B200, which the plans are made for
+
 struct PagedView {
     uint8_t *kc, *vc;
     int8_t *ke, *ve;
@@ -101,8 +103,6 @@ struct KvFormat;
 template <>
 struct KvFormat<FBLT_KV_E4M3> {
     static constexpr int kEmin = -117, kEmax = 119, kQmax = 448;
-    // value = half * 2^(e + kShift)
-    static constexpr int kShift = 0;
     // least e with a <= 448 * 2^e, from the bits of a = 1.m * 2^x: x - 8, one more where the significand passes 1.75
     static __device__ __forceinline__ int exponent(float a) {
         const int b = __float_as_int(a);
@@ -127,7 +127,6 @@ struct KvFormat<FBLT_KV_E4M3> {
 template <>
 struct KvFormat<FBLT_KV_INT8> {
     static constexpr int kEmin = -126, kEmax = 121, kQmax = 127;
-    static constexpr int kShift = 0;
     // least e with a <= 127 * 2^e: x - 6, one more where the significand passes 127 / 64
     static __device__ __forceinline__ int exponent(float a) {
         const int b = __float_as_int(a);
@@ -152,7 +151,7 @@ struct KvFormat<FBLT_KV_INT8> {
     }
 };
 
-// Four codes of one word -> their values, `s` = 2^(e + kShift).
+// Four codes of one word -> their values, `s` = 2^e.
 template <int FMT>
 __device__ __forceinline__ float4 kv_values(uint32_t w, float s) {
     uint32_t a, b;
@@ -162,7 +161,7 @@ __device__ __forceinline__ float4 kv_values(uint32_t w, float s) {
 }
 template <int FMT>
 __device__ __forceinline__ float kv_scale(int e) { // exponents outside the format's range are not written by the library
-    return exp2_int(min(max(e, KvFormat<FMT>::kEmin), KvFormat<FMT>::kEmax) + KvFormat<FMT>::kShift);
+    return exp2_int(min(max(e, KvFormat<FMT>::kEmin), KvFormat<FMT>::kEmax));
 }
 
 // x, y -> (hi, lo) planes of two halves each: 22 bits of a value of ordinary size

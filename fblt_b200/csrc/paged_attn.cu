@@ -1,12 +1,12 @@
 // Attention of new query rows over the 8-bit paged KV cache (fblt_paged_attn): the streaming kernel for few rows per
-// (sequence, kv head) -- one token, a drafted block, with grouped heads up to 64 rows -- the merge of a split key
+// (sequence, kv head) -- one token, a drafted block, with grouped heads up to 32 rows -- the merge of a split key
 // range, and the dispatch.
 //
 // out = sum_k p_k v_k / sum_k p_k, p_k = 2^(s_k - m), s_k = scale log2(e) q . k, in one pass over the keys with the
 // running maximum m. A cache row is used by at most G * n_new query rows, so the bytes of the cache bound this: the
 // stream has to be read at HBM speed and everything else has to fit beside it.
 //
-//   * CTA = (sequence, kv head, key range, tile of query rows); the rows of one kv head are its G query heads of every
+//   * CTA = (sequence, kv head, key range); the rows of one kv head are its G query heads of every
 //     new token, so grouped heads and drafted blocks read a key once.
 //   * Stages of 64 keys (head_dim 128: 32), four groups that lie in one page each, are copied ahead into shared memory:
 //     by every warp for itself, or, where warps share the keys, by a producer warp; group i lies 32 bytes further round
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
 #pragma unroll
                 for (int i = 0; i < KL; ++i) {
                     const int k = lane * KL + i;
-                    kscale[k] = exp2_int(min(max((int)(int8_t)stage[S::kOffE + k], F::kEmin), F::kEmax) + F::kShift);
+                    kscale[k] = exp2_int(min(max((int)(int8_t)stage[S::kOffE + k], F::kEmin), F::kEmax));
                     e[i] = min(max((int)(int8_t)stage[S::kOffE + S::kKeys + k], F::kEmin), F::kEmax);
                     if (kb + k >= rr.lo && kb + k < rr.hi && ((here >> (k / S::kPer)) & 1)) et = max(et, e[i]);
                 }
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(WR == 1 ? 128 : 160, PsCta<HD, RB, WR>::kMin) 
                 sm[row] = m[rb];
                 sl[row] = l[rb];
             }
-            constexpr float kDown = (float)(1 << F::kShift) / (float)(1 << kPsHead);
+            constexpr float kDown = 1.0f / (float)(1 << kPsHead);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -681,11 +681,11 @@ static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
             // one, where tiles of a sequence are three waves by themselves (a prompt of 8 k rows x 16 heads, 512 CTAs, in
             // 1 / 2 / 4 pieces: 346 / 400 / 467 us; ragged chunks 324 / 332 / 385 us; 2048 rows behind 30 k keys, 128
             // CTAs, in 1 / 8 pieces: 672 / 646 us).
-            const int64_t most = pl.row_tiles > 1 && units * pl.row_tiles >= 148 * 3 ? 1 : 8;
+            const int64_t most = pl.row_tiles > 1 && units * pl.row_tiles >= kPlanSms * 3 ? 1 : 8;
             double best = 0.0;
             for (int64_t c = 1; c <= most && (c == 1 || d->max_len / c >= 1024); ++c) {
-                const int64_t ctas = units * pl.row_tiles * c, waves = (ctas + 147) / 148;
-                const double use = (double)ctas / (double)(waves * 148) - 0.01 * (double)(c - 1);
+                const int64_t ctas = units * pl.row_tiles * c, waves = (ctas + kPlanSms - 1) / kPlanSms;
+                const double use = (double)ctas / (double)(waves * kPlanSms) - 0.01 * (double)(c - 1);
                 if (use > best) {
                     best = use;
                     s = c;
@@ -705,8 +705,8 @@ static PagedPlan paged_plan(const fblt_paged_attn_desc *d) {
             // 4 heads over 64 caches of 1.5 to 8 k keys, head_dim 128, in 1 / 2 / 4 / 8 pieces: 526 / 444 / 414 / 424 us;
             // 512 pieces of head_dim 64: 160 / 143 / 147 / 174 us; one token over 4 k keys: 55 / 59 us in 1 / 2 pieces.
             const int64_t ctas = units, key_max = d->max_len, worth = 256 * 1024 / d->cache.head_dim;
-            const int64_t fill = std::min((int64_t)148 * 4 / ctas, key_max / 256);
-            const int64_t even = std::min(((int64_t)148 * 14 + ctas - 1) / ctas, key_max / worth);
+            const int64_t fill = std::min((int64_t)kPlanSms * 4 / ctas, key_max / 256);
+            const int64_t even = std::min(((int64_t)kPlanSms * 14 + ctas - 1) / ctas, key_max / worth);
             s = std::max(fill, even);
         }
     }
@@ -760,8 +760,7 @@ static int launch_paged(const PagedAttnParams &p, const PagedPlan &pl, bool e4, 
     else if (pl.rb == 1 && pl.wr == 1) st = FBLT_PS(1, 1);
     else if (pl.wr == 1) st = FBLT_PS(B, 1);
     else if (pl.wr == 2) st = FBLT_PS(B, 2);
-    else if constexpr (B == 1) st = FBLT_PS(B, 4);
-    else return fail(FBLT_ERR_UNSUPPORTED, "paged_attn: no kernel for this tile of rows");
+    else st = FBLT_PS(B, B == 1 ? 4 : 2); // 17 .. 32 rows: four warps of one block, or (the case before) two of two
 #undef FBLT_PS
     if (st != FBLT_OK || p.splits <= 1) return st;
     const int64_t units = (int64_t)p.total * p.H, per = 256 / (HD / 4);

@@ -404,7 +404,7 @@ int validate_paged_cache(const fblt_paged_cache &c, int batch, const char *who) 
 
 template <int HD, int FMT>
 static int launch_norm_rope(NormRopeParams &p, cudaStream_t s, const char *what) {
-    p.rows_per_cta = rows_per_cta(p.rows, 148 * 8, kRowLoads, 2 * kRowLoads);
+    p.rows_per_cta = rows_per_cta(p.rows, kPlanSms * 8, kRowLoads, 2 * kRowLoads);
     p.parts = split_rows(p.qh + (FMT < 0 ? 1 : 2) * p.kh, p.rows_per_cta, kRowThreads / (HD / 4));
     const int64_t grid = (p.rows + p.rows_per_cta - 1) / p.rows_per_cta;
     if (grid > INT_MAX) return fail(FBLT_ERR_LIMIT, "%s: too many rows", what);
@@ -415,7 +415,7 @@ static int launch_norm_rope(NormRopeParams &p, cudaStream_t s, const char *what)
 
 template <int HD, int FMT>
 static int launch_read(ReadParams &p, bool bf16, cudaStream_t s) {
-    p.rows_per_cta = rows_per_cta(p.rows, 148 * 4, 1, 8);
+    p.rows_per_cta = rows_per_cta(p.rows, kPlanSms * 4, 1, 8);
     p.parts = split_rows((p.ko && p.vo ? 2 : 1) * p.pv.kvh, p.rows_per_cta, kRowThreads / (HD / 4));
     const unsigned grid = (unsigned)((p.rows + p.rows_per_cta - 1) / p.rows_per_cta);
     if (bf16) paged_read_kernel<HD, FMT, true><<<grid, kRowThreads, 0, s>>>(p);

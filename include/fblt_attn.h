@@ -711,8 +711,8 @@ enum {
  * The pages. Page p of kv head h holds page_size consecutive positions of one sequence:
  *   codes [num_pages, num_kv_heads, page_size, head_dim] bytes, exponents [num_pages, num_kv_heads, page_size] int8.
  * Position j of sequence b lives in page page_table[b * page_table_stride + j / page_size], slot j % page_size.
- * A page may appear in the tables of several sequences (a shared prefix) as long as nobody appends to it; entries
- * beyond a sequence's last page are not read. Page ids are checked by the kernels (see the status bits).
+ * A page may appear in the tables of several sequences (a shared prefix) as long as nobody appends to it, but every
+ * sequence has a table row of its own (page_table_stride >= max_pages); entries beyond a sequence's last page are not read. Page ids are checked by the kernels (see the status bits).
  */
 typedef struct {
     int32_t format; /* fblt_kv_format */
@@ -830,11 +830,15 @@ int fblt_paged_read(const fblt_paged_read_desc *desc, void *stream);
  *   block_mode == 0: j <= p && (window == 0 || p - j < window)
  *   block_mode == 1: every key of the sequence, j < base_len[b] + new rows (window is ignored)
  * Scores that are not finite weigh 0 and a row without any key gives zeros (ops/vecmath_cpu.c:16-53). Products carry
- * at least 22 bits of q and of the probabilities and all of the cache's; sums are fp32. The result does not depend on
- * how a prompt was cut into chunks beyond fp32 rounding.
- * max_new and max_len are host-known bounds of the new rows and of base_len[b] + new rows. splits: pieces the key range
- * of a (sequence, kv head) is cut into, merged by a second launch; 0 = choose. Workspace: fblt_paged_attn_workspace()
- * bytes, 16-byte aligned, not shared by calls that may overlap. The call only enqueues launches.
+ * at least 22 bits of q and of the probabilities and all of the cache's; sums are fp32, and so are scale * log2(e) * q and
+ * the weights (2^-126 of a row's largest and less is 0). The result does not depend on how a prompt was cut into chunks
+ * beyond fp32 rounding. out overlaps neither q nor the cache.
+ * max_new and max_len are host-known bounds of the new rows and of base_len[b] + new rows. max_new * num_heads /
+ * num_kv_heads chooses the kernel for the whole call: up to 32 rows stream through the cache, more go in tiles of 256, each
+ * with its own set-up; many single tokens beside a long chunk are two calls' work. batch * ceil(those rows / 256) is at
+ * most 2^22 - 1. splits: pieces the key range of a (sequence, kv head) is cut into, merged by a second launch; 0 = choose,
+ * more than 64 = 64. Workspace: fblt_paged_attn_workspace() bytes, 16-byte aligned, not shared by calls that may overlap.
+ * The call only enqueues launches.
  */
 typedef struct {
     fblt_paged_cache cache;
