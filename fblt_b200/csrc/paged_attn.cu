@@ -20,8 +20,8 @@
 //     neighbouring codes of a K row, lane g 1/8 of a V row, and the 16 keys of one product are 4 of each group, so
 //     that with the 32-byte skew V's column-wise reads touch every bank once.
 //
-// Measured (B200): one token of 256 sequences of up to 4 k keys, 16 kv heads, head_dim 64, int8: 273-281 us, 4.0 TB/s of
-// the cache's bytes; 8 rows x 4 heads over 64 caches of up to 8 k keys, head_dim 128, e4m3: 414-429 us. HBM's bound would
+// Measured (B200): one token of 256 sequences of up to 4 k keys, 16 kv heads, head_dim 64, int8: 273-284 us, 4.0 TB/s of
+// the cache's bytes; 8 rows x 4 heads over 64 caches of up to 8 k keys, head_dim 128, e4m3: 403-408 us. HBM's bound would
 // be 171 and 102 us: what is left is the conversion of codes to halves (five instructions for four int8 codes) and its
 // latency with 12 warps on an SM, which registers limit: issue slots are half busy, and warps that share keys each convert
 // all of them. Measured and slower: a producer warp where warps share nothing 332 us; stages of 32 keys at head_dim 64

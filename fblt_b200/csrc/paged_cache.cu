@@ -8,7 +8,7 @@
 // and a row costs additions (with a division per value group instead, the launch was bound by instruction issue).
 //
 // Measured (B200): norm + rotation of a prompt's q and k, 680 MB moved: 118-121 us, 5.7 TB/s; prompts appended and read
-// back 311-323 us against 223 us of bytes (K goes through 64-bit arithmetic; half of the warps fit); 1.27 GB read back from
+// back 311-326 us against 223 us of bytes (K goes through 64-bit arithmetic; half of the warps fit); 1.27 GB read back from
 // caches 202 us, 6.2 TB/s; one token's rows 4.7 us, a launch. The first values of every lane are asked for before the look-up
 // of the rows, whose two dependent loads they hide.
 #include "paged.cuh"

@@ -19,11 +19,11 @@
 //   issuer (1 warp)        while one query tile's softmax runs, the tensor cores have the other tile's products
 // Q's planes are TMEM operands (head_dim 128: the first one; the other stays in shared memory).
 //
-// Measured (B200): 2048 new rows x 16 heads, head_dim 64, behind 31 k keys: 641-657 us, 400 TFLOP/s of the formula's
-// products and twice that on the tensor cores (two planes); ragged chunks at head_dim 128: 324-331 us. What bounds it is
+// Measured (B200): 2048 new rows x 16 heads, head_dim 64, behind 31 k keys: 632-650 us, 405 TFLOP/s of the formula's
+// products and twice that on the tensor cores (two planes); ragged chunks at head_dim 128: 315-330 us. What bounds it is
 // the chain of one query tile: a step of 128 keys takes 4960 cycles, of which its 512 exponentials a scheduler 2150
 // (8 cycles a warp instruction), the wait for P V and the next S 1250, reading scores and their maximum 470, rescaling 450,
-// folding 330 (head_dim 128, whose sums fold into output rows: 850). Issue slots are 46 %, tensor cores 35 % busy (small
+// folding 330 (head_dim 128, whose sums fold into output rows: 850). Issue slots are 43 %, tensor cores 34 % busy (small
 // case). Measured and slower: three bf16 planes of P 757 us; S beside P instead of under it, tiles of 96 keys 715 us;
 // two threads a row 704 us; the query tiles in turns 695 us; a share of the exponentials as polynomials 649-698 us.
 #include "paged.cuh"

@@ -606,7 +606,8 @@ class PagedKvCache:
     """K and V in 8 bits with one power-of-two exponent for every (position, kv head), in pages.
 
     k_codes / v_codes: uint8 [num_pages, num_kv_heads, page_size, head_dim]; k_exp / v_exp: int8 [num_pages,
-    num_kv_heads, page_size]; page_table: int32 [batch, max_pages], page of positions j * page_size ... of a sequence.
+    num_kv_heads, page_size]; page_table: int32 [batch, max_pages], page of positions j * page_size ... of a sequence (rows of
+    their own: sequences share pages, not table rows). All on one device.
     fmt: "e4m3" or "int8". `status` collects the FBLT_PAGED_* bits that kernels raise (status_bits() reads them)."""
 
     def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor,

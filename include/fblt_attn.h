@@ -712,7 +712,8 @@ enum {
  *   codes [num_pages, num_kv_heads, page_size, head_dim] bytes, exponents [num_pages, num_kv_heads, page_size] int8.
  * Position j of sequence b lives in page page_table[b * page_table_stride + j / page_size], slot j % page_size.
  * A page may appear in the tables of several sequences (a shared prefix) as long as nobody appends to it, but every
- * sequence has a table row of its own (page_table_stride >= max_pages); entries beyond a sequence's last page are not read. Page ids are checked by the kernels (see the status bits).
+ * sequence has a table row of its own (page_table_stride >= max_pages); entries beyond a sequence's last page are not
+ * read. Page ids are checked by the kernels (see the status bits).
  */
 typedef struct {
     int32_t format; /* fblt_kv_format */
